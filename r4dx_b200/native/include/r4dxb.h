@@ -111,6 +111,29 @@ int r4dxb_attn_decode(const void* q, const void* qg, const void* cache, const in
                       const float* k_descale, const float* v_descale, float* part_acc, float* part_ml, void* out,
                       int T, int Hq, int Hkv, int D, int splits, int gated, void* stream);
 
+/* ---- attention over a 4-bit paged KV cache (kv4.cuh: 16-token blocks, 64 channels to a scale) ---- */
+/* Pool: uint8 [pool][Hkv][2][9 D], 16-byte aligned, D in {64, 128, 256}.  block_tables: int [slots][table_length]; row_slot (may be
+ * null: all rows belong to table 0): the table of each row.  Rows whose position, table entry or slot is out of range are not
+ * written; read back, or attended to, they are NaN.  16-byte aligned rows throughout. */
+/* q_out = rope(norm(q)) bf16; rope(norm(k)) and v enter the cache at positions[t].  q_norm / k_norm may be null; Hq = 0 with
+ * rotary_dim = 0: k and v as they are.  q_stride: elements between heads of qg (2 D with a gate half).  Positions of one sequence
+ * within a call must differ. */
+int r4dxb_attn_precore_kv4(const void* qg, const void* k, const void* v, const void* q_norm, const void* k_norm, const int* positions,
+                           const int* block_tables, const int* row_slot, int slots, int table_length, int pool, void* q_out, void* cache, int T,
+                           int Hq, int Hkv, int D, int rotary_dim, float theta, float eps, int q_stride, void* stream);
+/* k, v [T, Hkv, D] bf16: what the cache holds at positions[t] */
+int r4dxb_kv4_read(const void* cache, const int* block_tables, const int* row_slot, int slots, int table_length, int pool, const int* positions,
+                   void* k, void* v, int T, int Hkv, int D, void* stream);
+/* T (<= 32) rows of one sequence, or (row_slot given, T = 1) one row of each of `batch` sequences; a position of -1 sees nothing and
+ * gives zeros.  qg null: no output gate.  scratch (splits > 1): batch * T * Hq * splits * (D + 2) floats, 16-byte aligned. */
+int r4dxb_attn_decode_kv4(const void* q, const void* qg, const void* cache, const int* block_tables, const int* row_slot, int slots,
+                          int table_length, int pool, const int* positions, float* scratch, void* out, int T, int batch, int Hq, int Hkv, int D,
+                          int splits, int window, int* status, void* stream);
+/* T rows at positions pos0 .. pos0 + T - 1 (already written), causal; window 0 or the number of keys a row sees; key_limit as for
+ * r4dxb_attn_prefill_ex; status as for r4dxb_attn_prefill_tc. */
+int r4dxb_attn_prefill_kv4(const void* q, const void* qg, const void* cache, const int* block_table, int table_length, int pool, void* out, int T,
+                           int Hq, int Hkv, int D, int pos0, int window, const int* key_limit, int* status, void* stream);
+
 /* Sibling projections in one launch of the weight-streaming kernel: `count` (2 or 3) trellis weights of the same K and
  * bit width read the same rows x through the same prologue; weight i writes y[i] [T, n[i]] (no residual). */
 int r4dxb_trellis_gemv_siblings(int count, const void* const* words, const void* const* suh, const void* const* svh,

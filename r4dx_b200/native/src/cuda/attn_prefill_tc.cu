@@ -33,6 +33,7 @@
 // The reference's counterpart is a query-tiled WMMA kernel (reference:
 // third_party/libr4d/r4d_attn_prefill_h256_gqa6.hip:112); nothing is shared with it.
 #include "common.cuh"
+#include "kv4.cuh"
 #include "sm100_ptx.cuh"
 
 namespace r4dxb {
@@ -62,6 +63,9 @@ struct TcArgs {
   int T, Hq, Hkv, pos0, gated, window;
   int by_head;                 // a pair is two query heads of a kv head over the same rows, else two row tiles of a head
   int* status;
+  // 4-bit cache only
+  kv4::Table table;
+  const int* key_limit;        // [T] or null: row t also sees this call's keys up to that position
 };
 
 struct Control {
@@ -71,6 +75,7 @@ struct Control {
   uint32_t tmem_base;
   int abort_flag;
   float row[2][2][kQRows];                               // [tile parity][half of the keys]: what the two warps of a row exchange
+  int nan_groups[kQRows];                                // 4-bit cache: groups of 64 columns in which the row sees a NaN among the values
 };
 
 __device__ __forceinline__ uint32_t Fp8x2Bits(uint32_t v16) {
@@ -95,7 +100,32 @@ __device__ __forceinline__ int Sw128(int r, int c) { return (r >> 3) * 1024 + (r
 template <int D>
 __device__ __forceinline__ int GateChunk(int r, int c) { return r * 2 * D + ((c ^ (r & 7)) << 4); }
 
-template <int D>
+// the bits of a flag word in one of the two CTAs' shared memory
+__device__ __forceinline__ void OrRemote(uint32_t addr, uint32_t bits) {
+  asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(addr), "r"(bits) : "memory");
+}
+
+// Four code pairs of a 4-bit word (codes i and i + 4 in the halves of result i) as fp16 values n s + lo: the codes enter the mantissa of
+// 1024 (or, where they lie four bits higher, as 1024 + 16 n), come back out exactly, and one fma rounds to fp16.
+__device__ __forceinline__ __half2 AsHalf2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+__device__ __forceinline__ uint32_t Bits(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
+__device__ __forceinline__ void Kv4ToHalf(uint32_t w, __half2 s, __half2 lo, uint32_t (&h)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const uint32_t x = w >> (4 * i);
+    const __half2 n0 = __hsub2(AsHalf2((x & 0x000f000fu) | 0x64006400u), AsHalf2(0x64006400u));
+    const __half2 n1 = __hfma2(AsHalf2((x & 0x00f000f0u) | 0x64006400u), AsHalf2(0x2c002c00u), AsHalf2(0xd400d400u));     // / 16 - 64
+    h[i] = Bits(__hfma2(n0, s, lo));
+    h[i + 1] = Bits(__hfma2(n1, s, lo));
+  }
+}
+
+// KV4: the 4-bit cache (kv4.cuh) in place of the fp8 one; only what the conversion warps load and store differs, and
+//   - keys enter with the channels of every eight in the order 0 4 1 5 2 6 3 7 (that of Kv4ToHalf), and so does Q;
+//   - a value group that is NaN is stored as zeros, and noted for the rows that see it: 0 x NaN would reach the rows that do not.
+//     (NaN keys need nothing: a score that a row does not see is replaced before it is used.)
+//   - pages that the table or pool does not have are NaN keys.
+template <int D, bool KV4>
 __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
   constexpr int NS = D / 64;                          // 64-dimension slabs (one 128-byte swizzle row of fp16 each)
   constexpr int kQBytes = NS * kQRows * 128;
@@ -119,7 +149,8 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
   const int q0 = a.by_head ? first_row : first_row + rank * kQRows;
   const int rows = max(0, min(kQRows, a.T - q0));
   const int kv_limit = a.pos0 + a.T;                  // tokens present in the cache
-  const int kv_end = a.pos0 + min(a.T, first_row + (a.by_head ? kQRows : 2 * kQRows));      // first key no row of the pair may see
+  const bool limits = KV4 && a.key_limit != nullptr;
+  const int kv_end = limits ? kv_limit : a.pos0 + min(a.T, first_row + (a.by_head ? kQRows : 2 * kQRows));      // first key no row of the pair may see
   const int kv_first = a.window > 0 ? max(0, a.pos0 + first_row - a.window + 1) : 0;
   const int tile0 = kv_first / kKvTile;
   const int ntiles = (kv_end + kKvTile - 1) / kKvTile - tile0;              // at least 1
@@ -137,6 +168,9 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
     ptx::MbarInit(&ctl->gates, kConvWarps);
     ctl->abort_flag = 0;
     ptx::MbarFenceInit();
+  }
+  if constexpr (KV4) {
+    if (threadIdx.x < kQRows) ctl->nan_groups[threadIdx.x] = 0;
   }
   if (warp == kMmaWarp) {
     ptx::TmemAllocPair(&ctl->tmem_base, kTmemCols);
@@ -159,15 +193,59 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
     const int ch = tid % CH, key0 = tid / CH * KI, flip = (ch >> 2) & 1;
     // V: a thread owns VD dimensions of 8 consecutive keys and turns them into VD rows of 16 bytes; the byte it starts with depends on
     // its lane, and the two halves of a warp are 4 key groups apart, for the same reason.
-    constexpr int VD = D / 32, VW = VD / 4;
+    constexpr int VD = D / 32, VW = VD >= 4 ? VD / 4 : 1;
     const int dq = lane & 15, tg = (cw & 3) + ((lane >> 4) << 2) + ((cw >> 2) << 3);
     const size_t page_bytes = static_cast<size_t>(a.Hkv) * 2 * kPage * D;
     const uint8_t* cache_k = a.cache + static_cast<size_t>(hkv) * 2 * kPage * D + ch * 16;
     const uint8_t* cache_v = a.cache + static_cast<size_t>(hkv) * 2 * kPage * D + kPage * D + rank * (D / 2) + dq * VD;
     uint4 kraw[KI];
     uint32_t vraw[8][VW];
+    // 4-bit cache.  K: a thread owns the words of channels 8 kc .. of every 32 of one key (the keys of eight lanes are 4 apart, for the
+    // banks of its stores).  V: word vw (of this CTA's half) of VT tokens, turned into eight rows of VT fp16 values; the row that it
+    // starts with depends on its word.
+    constexpr int NJ = D / 32, NG = kv4::Shape<D>::kGroups, VT = D / 32, VWords = D / 16;
+    const int kc = tid & 3, kkey = (tid >> 5) * 8 + ((tid >> 3) & 3) + (tid & 4);
+    const int vword = tid % VWords, vtok = tid / VWords * VT, vgroup = (rank * VWords + vword) >> 3;
+    uint32_t kcodes[NJ], kpairs[NG], vcodes[VT], vpairs[VT];
+    const uint32_t* cache4 = reinterpret_cast<const uint32_t*>(a.cache) + static_cast<size_t>(hkv) * (kv4::Shape<D>::kRun / 4);
+    const size_t page_words = static_cast<size_t>(a.Hkv) * (kv4::Shape<D>::kRun / 4);
     // raw bytes of a tile into registers, zeros past the last token
     auto load_k = [&](int j) {
+      if constexpr (KV4) {
+        const int kp = (tile0 + j) * kKvTile + rank * kHalfTile + kkey;
+#pragma unroll
+        for (int i = 0; i < NJ; ++i) kcodes[i] = 0u;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) kpairs[i] = 0u;
+        if (j < ntiles && kp < kv_limit) {
+          const int blk = a.table.BlockAt(kp >> 4), t = kp & 15;
+          if (blk < 0) {
+#pragma unroll
+            for (int i = 0; i < NG; ++i) kpairs[i] = 0x7fc07fc0u;
+          } else {
+            const uint32_t* at = cache4 + blk * page_words;
+            if constexpr (D == 256) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(at + kv4::Word<D, false>(t, 16 * h + kc)));
+                kcodes[4 * h] = v.x; kcodes[4 * h + 1] = v.y; kcodes[4 * h + 2] = v.z; kcodes[4 * h + 3] = v.w;
+              }
+              const uint4 p = __ldg(reinterpret_cast<const uint4*>(at + 2 * D + t * NG));
+              kpairs[0] = p.x; kpairs[1] = p.y; kpairs[2] = p.z; kpairs[3] = p.w;
+            } else if constexpr (D == 128) {
+              const uint4 v = __ldg(reinterpret_cast<const uint4*>(at + kv4::Word<D, false>(t, kc)));
+              kcodes[0] = v.x; kcodes[1] = v.y; kcodes[2] = v.z; kcodes[3] = v.w;
+              const uint2 p = __ldg(reinterpret_cast<const uint2*>(at + 2 * D + t * NG));
+              kpairs[0] = p.x; kpairs[1] = p.y;
+            } else {
+              const uint2 v = __ldg(reinterpret_cast<const uint2*>(at + kv4::Word<D, false>(t, kc)));
+              kcodes[0] = v.x; kcodes[1] = v.y;
+              kpairs[0] = __ldg(at + 2 * D + t);
+            }
+          }
+        }
+        return;
+      }
       const int kp0 = (tile0 + j) * kKvTile + rank * kHalfTile + key0;
 #pragma unroll
       for (int i = 0; i < KI; ++i) kraw[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -181,6 +259,26 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
       }
     };
     auto load_v = [&](int j) {
+      if constexpr (KV4) {
+        const int kp0 = (tile0 + j) * kKvTile + vtok;
+#pragma unroll
+        for (int t = 0; t < VT; ++t) vcodes[t] = vpairs[t] = 0u;
+        if (j < ntiles && kp0 < kv_limit) {
+          const int blk = a.table.BlockAt(kp0 >> 4);
+          if (blk >= 0) {
+            const uint32_t* at = cache4 + blk * page_words + kv4::Shape<D>::kPart / 4;
+#pragma unroll
+            for (int t = 0; t < VT; ++t) {
+              const int tok = (kp0 & 15) + t;
+              if (kp0 + t < kv_limit) {
+                vcodes[t] = __ldg(at + kv4::Word<D, true>(tok, rank * VWords + vword));
+                vpairs[t] = __ldg(at + 2 * D + tok * NG + vgroup);
+              }
+            }
+          }
+        }
+        return;
+      }
       const int kp0 = (tile0 + j) * kKvTile + tg * 8;
 #pragma unroll
       for (int t = 0; t < 8; ++t)
@@ -203,6 +301,20 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
     };
     unsigned char* k_dst = Ks + (ch >> 2) * (kHalfTile * 128);
     auto store_k = [&](int j) {
+      if constexpr (KV4) {
+        unsigned char* at = Ks + (j & 1) * kKBytes;
+#pragma unroll
+        for (int i = 0; i < NJ; ++i) {
+          const uint32_t pair = kpairs[i >> 1];
+          uint32_t h[4];
+          Kv4ToHalf(kcodes[i], __float2half2_rn(BfLo(pair)), __float2half2_rn(BfHi(pair)), h);
+          *reinterpret_cast<uint4*>(at + (i >> 1) * (kHalfTile * 128) + Sw128(kkey, (i & 1) * 4 + kc)) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        ptx::FenceProxyAsyncShared();
+        __syncwarp();
+        if (lane == 0) ptx::MbarArriveRemote(k_full + (j & 1) * 8);
+        return;
+      }
       unsigned char* at = k_dst + (j & 1) * kKBytes;
 #pragma unroll
       for (int i = 0; i < KI; ++i) {
@@ -221,6 +333,57 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
     };
     unsigned char* v_dst = Vs + (tg >> 3) * kVSlab;
     auto store_v = [&](int j) {
+      if constexpr (KV4) {
+        unsigned char* at = Vs + (j & 1) * kVBytes + (vtok >> 6) * kVSlab;
+        bool nan = false;
+#pragma unroll
+        for (int t = 0; t < VT; ++t) nan |= BfLo(vpairs[t]) != BfLo(vpairs[t]);
+        if (nan) {
+#pragma unroll
+          for (int t = 0; t < VT; ++t)
+            if (BfLo(vpairs[t]) != BfLo(vpairs[t])) {
+              vpairs[t] = 0u;
+              const int kp = (tile0 + j) * kKvTile + vtok + t;
+              if ((vword & 7) == 0)              // one of the threads of the group
+                for (int peer = 0; peer < 2; ++peer) {
+                  const int first = a.by_head ? first_row : first_row + peer * kQRows;
+                  const uint32_t flags = ptx::MapToRank(ptx::SmemAddr(&ctl->nan_groups[0]), peer);
+                  for (int r = 0; r < kQRows && first + r < a.T; ++r) {
+                    const int qpos = a.pos0 + first + r, last = limits ? max(qpos, a.key_limit[first + r]) : qpos;
+                    if (kp <= last && (a.window == 0 || kp > qpos - a.window)) OrRemote(flags + 4 * r, 1u << vgroup);
+                  }
+                }
+            }
+          asm volatile("fence.acq_rel.cluster;" ::: "memory");
+        }
+        __half2 s2[VT / 2], lo2[VT / 2];
+        uint32_t lo_codes[VT / 2], hi_codes[VT / 2];          // channels 0 .. 3 and 4 .. 7 of two tokens
+#pragma unroll
+        for (int t = 0; t < VT / 2; ++t) {
+          s2[t] = __floats2half2_rn(BfLo(vpairs[2 * t]), BfLo(vpairs[2 * t + 1]));
+          lo2[t] = __floats2half2_rn(BfHi(vpairs[2 * t]), BfHi(vpairs[2 * t + 1]));
+          lo_codes[t] = __byte_perm(vcodes[2 * t], vcodes[2 * t + 1], 0x5410);
+          hi_codes[t] = __byte_perm(vcodes[2 * t], vcodes[2 * t + 1], 0x7632);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int d = (i + vword) & 7;
+          uint32_t h[VT / 2];
+#pragma unroll
+          for (int t = 0; t < VT / 2; ++t) {
+            const uint32_t x = (d & 4 ? hi_codes[t] : lo_codes[t]) >> (4 * (d & 3));
+            h[t] = Bits(__hfma2(__hsub2(AsHalf2((x & 0x000f000fu) | 0x64006400u), AsHalf2(0x64006400u)), s2[t], lo2[t]));
+          }
+          unsigned char* dst = at + Sw128(vword * 8 + d, (vtok >> 3) & 7) + (vtok & 7) * 2;
+          if constexpr (VT == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
+          else if constexpr (VT == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(h[0], h[1]);
+          else *reinterpret_cast<uint32_t*>(dst) = h[0];
+        }
+        ptx::FenceProxyAsyncShared();
+        __syncwarp();
+        if (lane == 0) ptx::MbarArriveRemote(v_full + (j & 1) * 8);
+        return;
+      }
       unsigned char* at = v_dst + (j & 1) * kVBytes;
 #pragma unroll
       for (int s = 0; s < VD; ++s) {
@@ -238,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
 
     load_k(0);
     {
-      const float scale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f * a.k_descale[hkv];
+      const float scale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f * (KV4 ? 1.f : a.k_descale[hkv]);
 #pragma unroll 4
       for (int i = tid; i < kQRows * (D / 8); i += kConvThreads) {
         const int r = i / (D / 8), c = i % (D / 8);
@@ -252,7 +415,10 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
             const __half2 p = __floats2half2_rn(BfLo(w[j]) * scale, BfHi(w[j]) * scale);
             h[j] = *reinterpret_cast<const uint32_t*>(&p);
           }
-          o = make_uint4(h[0], h[1], h[2], h[3]);
+          if constexpr (KV4)                    // channels 0 4 1 5 2 6 3 7
+            o = make_uint4(__byte_perm(h[0], h[2], 0x5410), __byte_perm(h[0], h[2], 0x7632), __byte_perm(h[1], h[3], 0x5410), __byte_perm(h[1], h[3], 0x7632));
+          else
+            o = make_uint4(h[0], h[1], h[2], h[3]);
         }
         *reinterpret_cast<uint4*>(Qs + (c >> 3) * (kQRows * 128) + Sw128(r, c & 7)) = o;
       }
@@ -350,6 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
     // ---------------- softmax warps: thread = query row = TMEM lane, two warps share a row ----------------
     const int half = warp >> 2, r = (warp & 3) * 32 + lane;
     const int qp = a.pos0 + q0 + r;                               // position of this row's query
+    const int last_key = limits && r < rows ? max(qp, min(a.key_limit[q0 + r], kv_limit - 1)) : qp;
     const uint32_t t_lane = tbase + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t p_full = ptx::MapToRank(ptx::SmemAddr(&ctl->p_full[0]), 0);
     float m_used = -INFINITY, l_run = 0.f;
@@ -374,13 +541,13 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
         ptx::TmemLoadWait();
         const int kv0 = (tile0 + j) * kKvTile, k_lo = kv0 + half * 64;
         // tiles that reach past the row's own position (or start before its window) need the mask
-        if ((kv0 + kKvTile - 1 > a.pos0 + q0) || (a.window > 0 && kv0 < a.pos0 + q0 + kQRows - a.window)) {
+        if ((kv0 + kKvTile - 1 > a.pos0 + q0) || (a.window > 0 && kv0 < a.pos0 + q0 + kQRows - a.window) || limits) {
           const int lo = a.window > 0 ? qp - a.window : -1;         // visible: lo < kp <= qp
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
             const int k0 = k_lo + c, k1 = k_lo + 32 + c;
-            if (!(k0 <= qp && k0 > lo)) s0[c] = 0xff800000u;        // -inf
-            if (!(k1 <= qp && k1 > lo)) s1[c] = 0xff800000u;
+            if (!(k0 <= last_key && k0 > lo)) s0[c] = 0xff800000u;  // -inf
+            if (!(k1 <= last_key && k1 > lo)) s1[c] = 0xff800000u;
           }
         }
         float mx2 = -INFINITY;
@@ -445,7 +612,8 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
     if (ok) ok = ptx::WarpMbarWait(&ctl->o_final, 0, abort_flag, 9);
     if (ok) {
       ptx::TcFenceAfter();
-      const float inv = (l > 0.f ? 1.f / l : 0.f) * a.v_descale[hkv];
+      const float inv = (l > 0.f ? 1.f / l : 0.f) * (KV4 ? 1.f : a.v_descale[hkv]);
+      const int nan_groups = KV4 ? ctl->nan_groups[r] : 0;
       // a lane's half row, staged where Q (first half) or V (second) was and sent off as one copy
       constexpr int kHalfRow = D / 2 * 2, kStageRow = kHalfRow + 16;
       static_assert(kQRows * kStageRow <= kQBytes && kQRows * kStageRow <= 2 * kVBytes, "the output tile fits");
@@ -461,6 +629,12 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
             float x[8];
 #pragma unroll
             for (int c = 0; c < 8; ++c) x[c] = __uint_as_float(o[8 * v + c]) * inv;
+            if constexpr (KV4) {
+              if (nan_groups >> ((half * (D / 2) + c0) >> 6) & 1) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) x[c] = __uint_as_float(0x7fc00000u);
+              }
+            }
             if (a.gated) {
               const uint4 g = *reinterpret_cast<const uint4*>(Ks + GateChunk<D>(r, (half * (D / 2) + c0) / 8 + v));
               const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
@@ -497,14 +671,14 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
   }
 }
 
-template <int D>
+template <int D, bool KV4 = false>
 int LaunchTc(const TcArgs& a, cudaStream_t s) {
   constexpr int NS = D / 64;
   // kClusterAlone: so much of an SM's shared memory that no other CTA shares the SM whose cluster may wait with tensor memory in its
   // hands (sm100_ptx.cuh).  More would cost L1: 8192 rows of 32 heads of 128 columns take 808 us with 131 KB, 821 with 156, 878 with 227.
   constexpr size_t kSmem = NS * kQRows * 128 + 2 * NS * kHalfTile * 128 + 2 * D * 128 + sizeof(Control) + 1024;
   constexpr size_t smem = kSmem > ptx::kClusterAlone ? kSmem : ptx::kClusterAlone;
-  auto kern = AttnPrefillTcKernel<D>;
+  auto kern = AttnPrefillTcKernel<D, KV4>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return static_cast<int>(e);
   cudaLaunchConfig_t cfg = {};
@@ -534,7 +708,7 @@ extern "C" int r4dxb_attn_prefill_tc(const void* q, const void* qg, const void* 
                                      const float* k_descale, const float* v_descale, void* out, int T, int Hq, int Hkv, int D,
                                      int pos0, int flags, int* status, void* stream) {
   if (T < 1 || Hq % Hkv || (D != 256 && D != 128)) return R4DXB_BAD_ARG;
-  TcArgs a;
+  TcArgs a = {};
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.qg = static_cast<const __nv_bfloat16*>(qg);
   a.cache = static_cast<const uint8_t*>(cache);
@@ -547,4 +721,27 @@ extern "C" int r4dxb_attn_prefill_tc(const void* q, const void* qg, const void* 
   a.status = status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return D == 256 ? LaunchTc<256>(a, s) : LaunchTc<128>(a, s);
+}
+
+/* The same over the 4-bit cache (kv4.cuh), head dimensions 64, 128 and 256; key_limit as for r4dxb_attn_prefill_ex. */
+extern "C" int r4dxb_attn_prefill_kv4(const void* q, const void* qg, const void* cache, const int* block_table, int table_length, int pool, void* out,
+                                      int T, int Hq, int Hkv, int D, int pos0, int window, const int* key_limit, int* status, void* stream) {
+  if (T < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || (D != 64 && D != 128 && D != 256) || pos0 < 0 || pos0 > 0x7fffffff - T - kKvTile || window < 0 ||
+      table_length < 1 || pool < 1 || q == nullptr || cache == nullptr || block_table == nullptr || out == nullptr)
+    return R4DXB_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out)) & 15 || reinterpret_cast<uintptr_t>(qg) & 3)
+    return R4DXB_BAD_ARG;
+  if (Hq > 32767 || (T + kQRows - 1) / kQRows > 65535) return R4DXB_TOO_LARGE;
+  TcArgs a = {};
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.qg = static_cast<const __nv_bfloat16*>(qg);
+  a.cache = static_cast<const uint8_t*>(cache);
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.pos0 = pos0; a.gated = qg != nullptr; a.window = window;
+  a.by_head = Hq / Hkv % 2 == 0;
+  a.status = status;
+  a.table = {block_table, table_length, pool};
+  a.key_limit = key_limit;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return D == 256 ? LaunchTc<256, true>(a, s) : (D == 128 ? LaunchTc<128, true>(a, s) : LaunchTc<64, true>(a, s));
 }

@@ -45,6 +45,8 @@ const R4dxbConstraint c32[] = {{"T", R4DXB_C_LE, 8, nullptr}, {"D", R4DXB_C_LE, 
 const R4dxbConstraint c33[] = {{"D", R4DXB_C_LE, 256, nullptr}};
 const R4dxbConstraint c34[] = {{"D", R4DXB_C_IN, 0, "128 256"}};
 const R4dxbConstraint c35[] = {{"D", R4DXB_C_IN, 0, "64 128 256"}, {"gqa", R4DXB_C_LE, 8, nullptr}};
+const R4dxbConstraint ckv4[] = {{"D", R4DXB_C_IN, 0, "64 128 256"}};
+const R4dxbConstraint ckv4d[] = {{"T", R4DXB_C_LE, 32, nullptr}, {"D", R4DXB_C_IN, 0, "64 128 256"}};
 const R4dxbConstraint c39[] = {{"k", R4DXB_C_LE, 16, nullptr}, {"E", R4DXB_C_LE, 1024, nullptr}};
 const R4dxbConstraint c40[] = {{"k", R4DXB_C_LE, 16, nullptr}};
 const R4dxbConstraint c43[] = {{"world", R4DXB_C_LE, 8, nullptr}};
@@ -181,6 +183,14 @@ const R4dxbKernelInfo kKernels[] = {
      "head dim 128 / 256", "bf16 q, e4m3 cache", "tcgen05", c34, 1},
     {"attn_prefill_ex", "attn", "paged_prefill_attention", "the mma.sync kernel: other head dims and per-row key limits (image blocks)",
      "head dim 64 / 128 / 256, gqa <= 8", "bf16 q, e4m3 cache", "mma.sync", c35, 2},
+    {"attn_precore_kv4", "attn", "qk_norm_rope_kv_write_4bit", "per-head norms, partial rope, rows quantised into the 4-bit paged cache (one sequence or one row of each)",
+     "D 64 / 128 / 256", "bf16 in, 4-bit codes with bf16 scale / low end per 64 channels", "simt", ckv4, 1},
+    {"kv4_read", "attn", "kv_read_4bit", "rows of the 4-bit paged cache brought back at any positions",
+     "D 64 / 128 / 256", "4-bit cache, bf16 out", "simt", ckv4, 1},
+    {"attn_decode_kv4", "attn", "paged_decode_attention_4bit", "split-KV decode attention over the 4-bit paged cache: rows of one sequence or one row of each of many",
+     "rows <= 32, D 64 / 128 / 256", "bf16 q, 4-bit cache", "mma.sync+bulk-copy", ckv4d, 2},
+    {"attn_prefill_kv4", "attn", "paged_prefill_attention_4bit", "causal / windowed prefill attention over the 4-bit paged cache, per-row key limits included",
+     "D 64 / 128 / 256", "bf16 q, 4-bit cache", "tcgen05", ckv4, 1},
     {"vit_attention", "attn", "vision_attention", "non-causal attention over variable-length image segments",
      "", "bf16", "simt", nullptr, 0},
     {"vit_rope", "attn", "vision_rope", "2-D rotary embedding of the fused qkv rows",

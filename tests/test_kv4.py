@@ -1,0 +1,85 @@
+"""The 4-bit KV cache's format and the calls that are refused before anything runs (CPU)."""
+import math
+
+import pytest
+import torch
+
+from r4dx_b200.quant import kv4
+
+BF = torch.bfloat16
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("values", [False, True])
+def test_every_word_has_a_place_of_its_own(D, values):
+    assert sorted(kv4.word_places(D, values).flatten().tolist()) == list(range(2 * D))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_rows_read_back_as_the_round_trip_and_touch_nothing_else(D):
+    g = torch.Generator().manual_seed(D)
+    pool = torch.randint(0, 256, kv4.pool_shape(3, 2, D), generator=g, dtype=torch.uint8)
+    k, v = torch.randn(20, 2, D, generator=g).to(BF), torch.randn(20, 2, D, generator=g).to(BF)
+    block, tok = torch.tensor([2] * 16 + [0] * 4), torch.arange(20) % 16
+    before = pool.clone()
+    kv4.write_rows(pool, k, v, block, tok)
+    rk, rv = kv4.read_rows(pool, block, tok)
+    assert torch.equal(rk, kv4.round_trip(k)) and torch.equal(rv, kv4.round_trip(v))
+    assert torch.equal(pool[1], before[1])
+    free = torch.arange(4, 16)
+    for a, b in zip(kv4.read_rows(pool, torch.zeros(12), free), kv4.read_rows(before, torch.zeros(12), free)):
+        assert torch.equal(a.nan_to_num(), b.nan_to_num())
+    assert torch.equal(kv4.read_rows(torch.zeros_like(pool), block, tok)[0], torch.zeros(20, 2, D))
+
+
+def test_rounding_is_half_a_step():
+    """Half a step, and 15 steps' worth of the scale's rounding (2^-8) at the top code."""
+    x = (torch.randn(500, 256, generator=torch.Generator().manual_seed(0)) * 3).to(BF)
+    n, s, lo = kv4.quantise(x)
+    assert int(n.min()) == 0 and int(n.max()) == 15
+    bound = (0.5 + 15 * 2.0 ** -8) * s.float().repeat_interleave(64, -1) * (1 + 2.0 ** -8)
+    assert ((kv4.round_trip(x) - x.float()).abs() <= bound).all()
+
+
+def test_values_at_the_edges():
+    x = torch.zeros(6, 64, dtype=BF)
+    x[0] = 2.5                                   # one value: exact
+    x[1, 3], x[1, 9] = math.inf, -math.inf       # saturate
+    x[2, 7] = math.nan
+    x[3, 0] = 3e38
+    x[4] = torch.linspace(-1e-30, 1e-30, 64).to(BF)
+    y = kv4.round_trip(x)
+    assert (y[0] == 2.5).all() and (y[5] == 0).all()
+    assert y[1, 9] == -32768 and 32768 <= y[1, 3] < 65504 and y[1].isfinite().all()
+    assert y[2].isnan().all()
+    assert abs(float(y[3, 0]) - 32768) <= 15 * 2.0 ** -8 * 32768 / 15
+    assert ((y[4] - x[4].float()).abs() <= 0.6 * 2e-30 / 15).all()
+
+
+def test_head_dimensions():
+    for D in (32, 96, 512):
+        with pytest.raises(ValueError):
+            kv4.pool_shape(1, 1, D)
+    assert kv4.pool_shape(7, 2, 128) == (7, 2, 2, 1152)
+
+
+def test_calls_without_a_gpu_pool_are_refused():
+    from r4dx_b200.ops import kernels as K
+    cache = torch.zeros(kv4.pool_shape(2, 1, 64), dtype=torch.uint8)
+    table, pos = torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    q = torch.zeros(1, 1, 64, dtype=BF)
+    for call in (lambda: K.attn_decode_kv4(q, None, cache, table, pos, q, 1, 1, 1, 64, False), lambda: K.kv4_read(cache, table, pos),
+                 lambda: K.kv4_write(q, q, pos, table, cache), lambda: K.attn_prefill_kv4(q, None, cache, table, q, 1, 1, 1, 64, 0, False),
+                 lambda: K.attn_precore_kv4(q, q, q, None, None, pos, table, q, cache, 1, 1, 1, 64, 0, 1e4, q_stride=64)):
+        with pytest.raises(K.KernelError):
+            call()
+
+
+def test_splits_fill_the_chip_once():
+    from r4dx_b200.ops import kernels as K
+    for rows in (1, 6, 48):
+        for heads in (1, 2, 8):
+            for batch in (1, 3, 64):
+                for length in (1, 8, 9, 5000):
+                    s = K.kv4_splits(rows, heads, batch, length)
+                    assert 1 <= s <= 148 and s <= max(1, (length + 7) // 8) and (s == 1 or s * heads * batch * -(-rows // 8) <= 148)
