@@ -1,15 +1,16 @@
 // Attention of few query rows (decode steps, speculative windows, batches of one row a sequence) over the 4-bit paged cache (kv4.cuh).
 //
-// Split-KV: a CTA has eight query rows of a kv head (of the G = rows x query heads per kv head) and a share of the sequence's blocks; each
+// Split-KV: a CTA has 8 NT query rows of a kv head (of the G = rows x query heads per kv head) and a share of the sequence's blocks; each
 // of its warps walks blocks of its own, which arrive as one bulk copy per block into the warp's ring of shared memory.  Per block
-//   scores   S^T[16 tokens x 8 rows] = K Q^T on mma.m16n8k16 (bf16): A = the codes, widened by a mask and an or to 128 + n, B = the query
-//            rows as they are (held in registers).  The sum starts at -136 sum(q), so a group gives sum q (n - 8), exactly up to fp32
-//            sums; then s (that) + (lo + 8 s) sum(q) per group, token and row.
+//   scores   S^T[16 tokens x 8 rows] = K Q^T on mma.m16n8k16 (fp16): A = the codes as they lie, since four bits at the bottom of a half are
+//            the subnormal n 2^-24 and four bits above them n 2^-20: one AND for two codes, and no conversion at all.  B = the query rows
+//            times 2^-4 (2^-8 under the codes that carry a 16), exact down to 2^-6.  A group gives 2^-28 sum q n; then s (that) in fp32.
+//            sum_g lo sum(q): one product of the pairs as they lie (bf16) with the sums' upper and lower parts.
 //   softmax  running maximum per row in the log2 domain, moved only when a score is more than 8 above it (p <= 2^8), so that most blocks
 //            need no exchange between lanes; sums in fp32 per lane.
-//   values   O^T[D x 8 rows] += (n - 8) (p s):  A = codes of token pairs, 128 + n less 136, exact in bf16; B = p s rounded to bf16 (2^-9
-//            of each product, random in sign: below the rounding of the output), turned from scores' to operand order with movmatrix.
-//            sum p (lo + 8 s) per group in fp32.  (Codes left at 128 + n would have the sums at 30 to 40 times their result.)
+//   values   O^T[D x 8 rows] += n (p s):  A = codes of token pairs, again as subnormals; B = p s times a power of two that brings the largest
+//            scale met so far to 1 .. 2, rounded to fp16 (2^-11 of 15 steps at most), turned from scores' to operand order with movmatrix.
+//            sum p lo per group in fp32.
 // The warps' results meet in shared memory, the splits' in a second kernel; a sequence short enough for one CTA is finished by it.
 // A row with no visible token (position -1) gives zeros; a block that the table or pool does not have gives NaN to the rows that see it.
 #include "kv4.cuh"
@@ -18,9 +19,8 @@
 namespace r4dxb {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kRows = 8;               // query rows of a CTA
 constexpr float kRescaleStep = 8.f;
+constexpr float kUnit = 1.f / (1 << 28);       // of the scores before the softmax: 2^-4 from q, 2^-24 from the codes
 
 struct DecodeArgs {
   const __nv_bfloat16* q;      // [T, Hq, D]
@@ -34,36 +34,55 @@ struct DecodeArgs {
   __nv_bfloat16* out;          // [T, Hq, D]
   int* status;
   int T, Hq, Hkv, splits, slots, window;
+  int warps;                   // of a CTA
 };
 
-template <int D>
-struct Ring {
-  static constexpr int kStages = D == 256 ? 4 : 8;               // blocks in flight per warp
-  static constexpr int kBytes = kWarps * kStages * kv4::Shape<D>::kRun;
+// Warps of a CTA and blocks in flight per warp, by head dimension and row tiles.
+template <int D, int NT>
+struct Plan {
+  static constexpr int kWarps = D == 256 ? (NT == 1 ? 12 : 8) : (D == 128 ? (NT == 1 ? 16 : (NT == 2 ? 12 : 8)) : (NT == 4 ? 12 : 16));
+  static constexpr int kStages = D == 256 ? (NT == 1 ? 3 : 4) : 4;
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kRing = kWarps * kStages * kv4::Shape<D>::kRun;
   static constexpr int kStride = D + 4;                          // floats between rows of the merge
-  static constexpr size_t kSmem = kBytes + kWarps * kStages * 8 + kWarps * kRows * 8 + 16;
-  static_assert(kWarps * kRows * kStride * 4 <= kBytes, "the warps' results fit where the ring was");
+  static constexpr int kMerge = kWarps * kRows * kStride * 4;
+  static constexpr int kQuery = NT * (D / 32) * 512;             // operand B of the scores
+  static constexpr int kBody = kRing > kMerge ? kRing : kMerge;
+  static constexpr size_t kSmem = kBody + kQuery + kWarps * kStages * 8 + kWarps * kRows * 8 + kRows * 4 + 16;
+  static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
 // The blocks that the rows of a call may see and the number of CTAs that share them: a block per warp at least.
 struct Span {
-  int first, blocks, active, low, high;
+  int first, blocks, active;
 };
-__device__ __forceinline__ Span Visible(const int* positions, int T, int window, int splits) {
+__device__ __forceinline__ Span Visible(const int* positions, int T, int window, int splits, int warps) {
   const int lane = threadIdx.x & 31;
   const int p = lane < T ? positions[lane] : -1;
   Span s;
-  s.high = __reduce_max_sync(0xffffffffu, p);
-  s.low = __reduce_min_sync(0xffffffffu, p < 0 ? 0x7fffffff : p);
-  s.first = window > 0 && s.high >= 0 ? max(0, s.low - window + 1) / kv4::kBlock : 0;
-  s.blocks = s.high >= 0 ? s.high / kv4::kBlock + 1 - s.first : 0;
-  s.active = max(1, min(splits, (s.blocks + kWarps - 1) / kWarps));
+  const int high = __reduce_max_sync(0xffffffffu, p), low = __reduce_min_sync(0xffffffffu, p < 0 ? 0x7fffffff : p);
+  s.first = window > 0 && high >= 0 ? max(0, low - window + 1) / kv4::kBlock : 0;
+  s.blocks = high >= 0 ? high / kv4::kBlock + 1 - s.first : 0;
+  s.active = max(1, min(splits, (s.blocks + warps - 1) / warps));
   return s;
 }
 
-__device__ __forceinline__ void MmaBf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+struct Frag {
+  float x[4];
+};
+__device__ __forceinline__ Frag MmaF16(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const Frag& c) {
+  Frag d;
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d.x[0]), "=f"(d.x[1]), "=f"(d.x[2]), "=f"(d.x[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x[0]), "f"(c.x[1]), "f"(c.x[2]), "f"(c.x[3]));
+  return d;
+}
+__device__ __forceinline__ Frag MmaBf16(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const Frag& c) {
+  Frag d;
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d.x[0]), "=f"(d.x[1]), "=f"(d.x[2]), "=f"(d.x[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x[0]), "f"(c.x[1]), "f"(c.x[2]), "f"(c.x[3]));
+  return d;
 }
 __device__ __forceinline__ uint32_t Transpose8x8(uint32_t x) {
   uint32_t y;
@@ -75,13 +94,12 @@ __device__ __forceinline__ float Exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// codes i and i + 4 of a word as the bf16 pair 128 + n
-__device__ __forceinline__ uint32_t CodePair(uint32_t w, int i) { return (w >> (4 * i) & 0x000f000fu) | 0x43004300u; }
-__device__ __forceinline__ uint32_t Centred(uint32_t pair) {           // 128 + n -> n - 8
-  const uint32_t c = 0x43084308u;
-  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&pair), *reinterpret_cast<const __nv_bfloat162*>(&c));
-  return *reinterpret_cast<const uint32_t*>(&d);
-}
+__device__ __forceinline__ __half2 AsHalf2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+__device__ __forceinline__ uint32_t Bits(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
+__device__ __forceinline__ uint32_t PackHalf(float lo, float hi) { return Bits(__floats2half2_rn(lo, hi)); }
+// codes of the lowest bits of a word's halves (n 2^-24 as fp16), of the next four (n 2^-20)
+__device__ __forceinline__ uint32_t Codes(uint32_t w) { return w & 0x000f000fu; }
+__device__ __forceinline__ uint32_t Codes16(uint32_t w) { return w & 0x00f000f0u; }
 
 template <int N>
 __device__ __forceinline__ void LoadWords(const uint32_t* p, uint32_t (&w)[N]) {
@@ -96,16 +114,18 @@ __device__ __forceinline__ void LoadWords(const uint32_t* p, uint32_t (&w)[N]) {
   }
 }
 
-template <int D>
-__global__ void __launch_bounds__(kWarps * 32, 1) DecodeKv4Kernel(DecodeArgs a) {
+template <int D, int NT>
+__global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(DecodeArgs a) {
   PdlEnter();
   using S = kv4::Shape<D>;
-  using R = Ring<D>;
-  constexpr int NG = S::kGroups, NJ = D / 32;
+  using P = Plan<D, NT>;
+  constexpr int NG = S::kGroups, NJ = D / 32, kWarps = P::kWarps, kRows = P::kRows, kStages = P::kStages;
   extern __shared__ __align__(128) unsigned char smem[];
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + R::kBytes);
-  float2* ml = reinterpret_cast<float2*>(bars + kWarps * R::kStages);           // [warps][rows]
-  volatile int* abort_flag = reinterpret_cast<int*>(ml + kWarps * kRows);
+  uint4* query = reinterpret_cast<uint4*>(smem + P::kBody);                     // [row tile][32 channels][lane]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + P::kBody + P::kQuery);
+  float2* ml = reinterpret_cast<float2*>(bars + kWarps * kStages);              // [warps][rows]
+  int* nan_groups = reinterpret_cast<int*>(ml + kWarps * kRows);                // [rows]: groups in which the row sees a NaN among the values
+  volatile int* abort_flag = nan_groups + kRows;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x, hkv = blockIdx.y % a.Hkv, row0 = blockIdx.y / a.Hkv * kRows, seq = blockIdx.z;
   bool known = true;           // the sequence has a table
@@ -119,27 +139,28 @@ __global__ void __launch_bounds__(kWarps * 32, 1) DecodeKv4Kernel(DecodeArgs a) 
     a.table.entries += static_cast<size_t>(known ? slot : 0) * a.table.length;
   }
   const int gqa = a.Hq / a.Hkv, G = gqa * a.T;
-  const Span span = Visible(a.positions, a.T, a.window, a.splits);
+  const Span span = Visible(a.positions, a.T, a.window, a.splits, kWarps);
   if (split >= span.active) return;
   const int per = (span.blocks + span.active - 1) / span.active;
   const int b0 = span.first + split * per + warp, b1 = min(span.first + span.blocks, span.first + (split + 1) * per);
   const int steps = b1 > b0 ? (b1 - b0 + kWarps - 1) / kWarps : 0;
 
-  unsigned char* ring = smem + warp * R::kStages * S::kRun;
-  uint64_t* full = bars + warp * R::kStages;
+  unsigned char* ring = smem + warp * kStages * S::kRun;
+  uint64_t* full = bars + warp * kStages;
   if (lane == 0) {
-    for (int i = 0; i < R::kStages; ++i) ptx::MbarInit(full + i, 1);
+    for (int i = 0; i < kStages; ++i) ptx::MbarInit(full + i, 1);
     ptx::MbarFenceInit();
   }
   if (threadIdx.x == 0) *abort_flag = 0;
-  __syncthreads();
+  if (threadIdx.x < kRows) nan_groups[threadIdx.x] = 0;
+  __syncwarp();
 
-  // ---- copies: block b0 + 8 i into slot i % kStages ----
+  // ---- copies: block b0 + i warps into slot i % kStages ----
   uint32_t missing = 0u, phases = 0u;          // by slot: no such block; parity of its next wait
   int entry = -1;
-  auto issue = [&](int i) {
+  auto issue = [&](int i, int slot) {
     if ((i & 31) == 0) entry = i + lane < steps && known ? a.table.BlockAt(b0 + (i + lane) * kWarps) : -1;
-    const int blk = __shfl_sync(0xffffffffu, entry, i & 31), slot = i % R::kStages;
+    const int blk = __shfl_sync(0xffffffffu, entry, i & 31);
     if (blk < 0) {
       missing |= 1u << slot;
       return;
@@ -150,196 +171,304 @@ __global__ void __launch_bounds__(kWarps * 32, 1) DecodeKv4Kernel(DecodeArgs a) 
       ptx::BulkLoad(ring + slot * S::kRun, a.cache + (static_cast<size_t>(blk) * a.Hkv + hkv) * S::kRun, S::kRun, full + slot);
     }
   };
-  for (int i = 0; i < min(steps, R::kStages); ++i) issue(i);
+  for (int i = 0; i < min(steps, kStages); ++i) issue(i, i);
 
-  // ---- query rows: operand B of the scores (row g; channels 32 j + 8 c .. as the pairs of CodePair), and their sums per group ----
+  // ---- query rows: a warp per row tile lays out operand B (row g; channels 32 j + 8 c .. in the order of the codes) and the sums ----
   const int my_pos = (lane < a.T) ? a.positions[lane] : -1;
   auto position = [&](int r) {
     const int p = __shfl_sync(0xffffffffu, my_pos, r < G ? r / gqa : 0);
     return r < G ? p : -1;
   };
-  uint32_t qb[NJ][4];
-  float qsum[NG][2];
-  {
-    const int r = row0 + g;
+  float qsum[NT][NG];                            // of row 8 nt + g, times 2^-28
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = row0 + 8 * nt + g;
     const __nv_bfloat16* src = a.q + (static_cast<size_t>(r / gqa) * a.Hq + hkv * gqa + r % gqa) * D + 8 * c;
-    float part[NG];
+#pragma unroll
+    for (int j = 0; j < NG; ++j) qsum[nt][j] = 0.f;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const uint4 v = r < G ? *reinterpret_cast<const uint4*>(src + 32 * j) : make_uint4(0u, 0u, 0u, 0u);
-      qb[j][0] = __byte_perm(v.x, v.z, 0x5410);
-      qb[j][1] = __byte_perm(v.x, v.z, 0x7632);
-      qb[j][2] = __byte_perm(v.y, v.w, 0x5410);
-      qb[j][3] = __byte_perm(v.y, v.w, 0x7632);
-      const float sum = ((BfLo(v.x) + BfHi(v.x)) + (BfLo(v.y) + BfHi(v.y))) + ((BfLo(v.z) + BfHi(v.z)) + (BfLo(v.w) + BfHi(v.w)));
-      part[j >> 1] = (j & 1) ? part[j >> 1] + sum : sum;
-    }
+      // channels i and i + 4 for i = 0 .. 3; every second pair meets codes that carry a factor 16
+      const float x[8] = {BfLo(v.x), BfHi(v.x), BfLo(v.y), BfHi(v.y), BfLo(v.z), BfHi(v.z), BfLo(v.w), BfHi(v.w)};
+      uint32_t b[4];
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      float s = part[i];
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      qsum[i][0] = __shfl_sync(0xffffffffu, s, 8 * c);
-      qsum[i][1] = __shfl_sync(0xffffffffu, s, 8 * c + 4);
-    }
-  }
-  const float scale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;
-  const int pos0 = position(row0 + 2 * c), pos1 = position(row0 + 2 * c + 1);
-  // positions among the rows that there are, for blocks that all of them see whole
-  const int row_pos = position(row0 + g);
-  const int p_min = __reduce_min_sync(0xffffffffu, row0 + g < G ? row_pos : 0x7fffffff), p_max = __reduce_max_sync(0xffffffffu, row_pos);
-
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;       // rows 2 c, 2 c + 1; l of this lane's tokens
-  float acc[NG][4][4], base[NG][2];
-#pragma unroll
-  for (int j = 0; j < NG; ++j) {
-    base[j][0] = base[j][1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[j][i][0] = acc[j][i][1] = acc[j][i][2] = acc[j][i][3] = 0.f;
-  }
-
-  bool ok = true;
-  int i = 0;
-  for (; i < steps; ++i) {
-    const int slot = i % R::kStages, kp0 = (b0 + i * kWarps) * kv4::kBlock;
-    if (missing >> slot & 1u) {
-      auto sees = [&](int pos) { return pos >= kp0 && (a.window == 0 || kp0 + kv4::kBlock - 1 > pos - a.window); };
-      if (sees(pos0)) l0 = __int_as_float(0x7fc00000);
-      if (sees(pos1)) l1 = __int_as_float(0x7fc00000);
-      if (i + R::kStages < steps) issue(i + R::kStages);
-      continue;
-    }
-    ok = ptx::WarpMbarWait(full + slot, phases >> slot & 1u, abort_flag, 1);
-    if (!ok) break;
-    phases ^= 1u << slot;
-    const uint32_t* kw = reinterpret_cast<const uint32_t*>(ring + slot * S::kRun);
-    const uint32_t* vw = kw + S::kPart / 4;
-
-    // ---- scores: tokens g (sc[0], sc[1]) and g + 8 (sc[2], sc[3]) of rows 2 c, 2 c + 1 ----
-    float sc[4] = {0.f, 0.f, 0.f, 0.f};
-    {
-      uint32_t pa[NG], pb[NG];
-      LoadWords<NG>(kw + 2 * D + g * NG, pa);
-      LoadWords<NG>(kw + 2 * D + (g + 8) * NG, pb);
-      uint32_t ca[NJ], cb[NJ];
-      if constexpr (D == 256) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int at = ((h ^ (g & 1)) * 16) + c * 4;
-          const uint4 x = *reinterpret_cast<const uint4*>(kw + g * 32 + at), y = *reinterpret_cast<const uint4*>(kw + (g + 8) * 32 + at);
-          ca[4 * h] = x.x; ca[4 * h + 1] = x.y; ca[4 * h + 2] = x.z; ca[4 * h + 3] = x.w;
-          cb[4 * h] = y.x; cb[4 * h + 1] = y.y; cb[4 * h + 2] = y.z; cb[4 * h + 3] = y.w;
-        }
-      } else {
-        LoadWords<NJ>(kw + g * (D / 8) + c * NJ, ca);
-        LoadWords<NJ>(kw + (g + 8) * (D / 8) + c * NJ, cb);
+      for (int i = 0; i < 4; ++i) {
+        const float f = i & 1 ? 0.00390625f : 0.0625f;
+        b[i] = PackHalf(x[i] * f, x[i + 4] * f);
+        qsum[nt][j >> 1] += (x[i] + x[i + 4]) * kUnit;
       }
-#pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        float s4[4] = {-136.f * qsum[j][0], -136.f * qsum[j][1], -136.f * qsum[j][0], -136.f * qsum[j][1]};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t x = ca[2 * j + h], y = cb[2 * j + h];
-          MmaBf16(s4, CodePair(x, 0), CodePair(y, 0), CodePair(x, 1), CodePair(y, 1), qb[2 * j + h][0], qb[2 * j + h][1]);
-          MmaBf16(s4, CodePair(x, 2), CodePair(y, 2), CodePair(x, 3), CodePair(y, 3), qb[2 * j + h][2], qb[2 * j + h][3]);
-        }
-        const float sa = BfLo(pa[j]), sb = BfLo(pb[j]), ta = fmaf(8.f, sa, BfHi(pa[j])), tb = fmaf(8.f, sb, BfHi(pb[j]));
-        sc[0] = fmaf(sa, s4[0], fmaf(ta, qsum[j][0], sc[0]));
-        sc[1] = fmaf(sa, s4[1], fmaf(ta, qsum[j][1], sc[1]));
-        sc[2] = fmaf(sb, s4[2], fmaf(tb, qsum[j][0], sc[2]));
-        sc[3] = fmaf(sb, s4[3], fmaf(tb, qsum[j][1], sc[3]));
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sc[e] *= scale;
-    const bool whole = kp0 + kv4::kBlock - 1 <= p_min && (a.window == 0 || kp0 > p_max - a.window);
-    bool seen[4] = {true, true, true, true};
-    if (!whole) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int kp = kp0 + g + (e >> 1) * 8, pos = e & 1 ? pos1 : pos0;
-        seen[e] = kp <= pos && (a.window == 0 || kp > pos - a.window);
-        if (!seen[e]) sc[e] = -INFINITY;
-      }
-    }
-
-    // ---- running maximum and probabilities ----
-    const float mx0 = fmaxf(sc[0], sc[2]), mx1 = fmaxf(sc[1], sc[3]);
-    if (__any_sync(0xffffffffu, mx0 > m0 + kRescaleStep || mx1 > m1 + kRescaleStep)) {
-      float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
-        n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
-      }
-      const float f0 = n0 == -INFINITY ? 1.f : Exp2(m0 - n0), f1 = n1 == -INFINITY ? 1.f : Exp2(m1 - n1);
-      m0 = n0;
-      m1 = n1;
-      l0 *= f0;
-      l1 *= f1;
-#pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        base[j][0] *= f0;
-        base[j][1] *= f1;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          acc[j][e][0] *= f0; acc[j][e][1] *= f1;
-          acc[j][e][2] *= f0; acc[j][e][3] *= f1;
-        }
-      }
-    }
-    const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
-    const float p[4] = {Exp2(sc[0] - r0), Exp2(sc[1] - r1), Exp2(sc[2] - r0), Exp2(sc[3] - r1)};
-    l0 += p[0] + p[2];
-    l1 += p[1] + p[3];
-
-    // ---- values: tokens 2 c, 2 c + 1 and 8 more; of every 64 channels 8 g .. ----
-    uint32_t va[NG], vb[NG], vc[NG], vd[NG], pa[NG], pb[NG];
-    LoadWords<NG>(vw + 2 * D + g * NG, pa);
-    LoadWords<NG>(vw + 2 * D + (g + 8) * NG, pb);
-    if constexpr (D == 256) {
-      const int at = (g ^ (2 * c)) * 4;
-      LoadWords<NG>(vw + (2 * c) * 32 + at, va);
-      LoadWords<NG>(vw + (2 * c + 1) * 32 + at, vb);
-      LoadWords<NG>(vw + (2 * c + 8) * 32 + at, vc);
-      LoadWords<NG>(vw + (2 * c + 9) * 32 + at, vd);
-    } else {
-      const int unit = 2 * NG, at = D == 128 ? (g ^ (2 * c)) * unit : (g ^ ((c & 2) << 1)) * unit;
-      uint32_t x[2 * NG], y[2 * NG];
-      LoadWords<2 * NG>(vw + c * (D / 4) + at, x);
-      LoadWords<2 * NG>(vw + (c + 4) * (D / 4) + at, y);
-#pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        va[j] = x[j]; vb[j] = x[NG + j];
-        vc[j] = y[j]; vd[j] = y[NG + j];
-      }
+      if (warp == nt % kWarps) query[(nt * NJ + j) * 32 + lane] = make_uint4(b[0], b[1], b[2], b[3]);
     }
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
-      const float sa = BfLo(pa[j]), sb = BfLo(pb[j]), ta = fmaf(8.f, sa, BfHi(pa[j])), tb = fmaf(8.f, sb, BfHi(pb[j]));
-      // (a token that a row does not see may hold anything: its pair is left out, not multiplied by zero)
-      const float w0 = seen[0] ? p[0] * sa : 0.f, w1 = seen[1] ? p[1] * sa : 0.f, w2 = seen[2] ? p[2] * sb : 0.f, w3 = seen[3] ? p[3] * sb : 0.f;
-      base[j][0] += (seen[0] ? p[0] * ta : 0.f) + (seen[2] ? p[2] * tb : 0.f);
-      base[j][1] += (seen[1] ? p[1] * ta : 0.f) + (seen[3] ? p[3] * tb : 0.f);
-      const uint32_t wb0 = Transpose8x8(PackBf16(w0, w1)), wb1 = Transpose8x8(PackBf16(w2, w3));
-      const uint32_t ab_lo = __byte_perm(va[j], vb[j], 0x5410), ab_hi = __byte_perm(va[j], vb[j], 0x7632);
-      const uint32_t cd_lo = __byte_perm(vc[j], vd[j], 0x5410), cd_hi = __byte_perm(vc[j], vd[j], 0x7632);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        MmaBf16(acc[j][e], Centred(CodePair(ab_lo, e)), Centred(CodePair(ab_hi, e)), Centred(CodePair(cd_lo, e)), Centred(CodePair(cd_hi, e)), wb0, wb1);
+      for (int o = 1; o < 4; o <<= 1) {
+        qsum[nt][j] += __shfl_xor_sync(0xffffffffu, qsum[nt][j], o);
+      }
     }
-    __syncwarp();                                // every lane has read the slot
-    if (i + R::kStages < steps) issue(i + R::kStages);
+  }
+  // operand B of sum_g lo sum(q): pairs (0, sum) in two (D = 256, 128) or four (64) parts of bf16
+  uint32_t qpair[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float rest = qsum[nt][0];
+#pragma unroll
+    for (int j = 1; j < NG; ++j) rest = c % NG == j ? qsum[nt][j] : rest;
+    float part = 0.f, next = 0.f;
+#pragma unroll
+    for (int k = 0; k <= 4 / NG; ++k) {
+      const float b = __bfloat162float(__float2bfloat16_rn(rest));
+      if (k == c / NG) part = b;
+      if (k == c / NG + 1) next = b;
+      rest -= b;
+    }
+    qpair[nt][0] = PackBf16(0.f, part);
+    qpair[nt][1] = NG == 4 ? PackBf16(0.f, next) : 0u;
+  }
+  __syncthreads();
+
+  const float scale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f / kUnit, step = kRescaleStep / scale;
+  int pos[NT][2], p_min = 0x7fffffff, p_max = -1;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    pos[nt][0] = position(row0 + 8 * nt + 2 * c);
+    pos[nt][1] = position(row0 + 8 * nt + 2 * c + 1);
+    // among the rows that there are, for blocks that all of them see whole
+    const int r = row0 + 8 * nt + g, p = position(r);
+    p_min = min(p_min, r < G ? p : 0x7fffffff);
+    p_max = max(p_max, p);
+  }
+  p_min = __reduce_min_sync(0xffffffffu, p_min);
+  p_max = __reduce_max_sync(0xffffffffu, p_max);
+  auto sees = [&](int at, int kp) { return kp <= at && (a.window == 0 || kp > at - a.window); };
+
+  float m[NT][2], l[NT][2];                      // rows 8 nt + 2 c, + 1; l of this lane's tokens
+  Frag acc[NT][NG][4];
+  float base[NT][NG][2];                         // sum p lo of this lane's tokens
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt][0] = m[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      base[nt][j][0] = base[nt][j][1] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[nt][j][e] = {{0.f, 0.f, 0.f, 0.f}};
+    }
+  }
+  uint32_t limit = 39u << 7;                     // scales (bf16 bits) from which the sums need a smaller power of two ..
+  float power = __uint_as_float((254u - 32u) << 23);      // .. than this: 2^-(exponent of the largest scale), at first 2^95
+
+  bool ok = true;
+  int i = 0, slot = 0;
+#pragma unroll 1
+  for (; i < steps; ++i) {
+    const int kp0 = (b0 + i * kWarps) * kv4::kBlock;
+    if (missing >> slot & 1u) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          if (pos[nt][r] >= kp0 && (a.window == 0 || kp0 + kv4::kBlock - 1 > pos[nt][r] - a.window)) l[nt][r] = __int_as_float(0x7fc00000);
+    } else {
+      if (!__all_sync(0xffffffffu, ptx::MbarTestWait(full + slot, phases >> slot & 1u))) ok = ptx::WarpMbarWait(full + slot, phases >> slot & 1u, abort_flag, 1);
+      if (!ok) break;
+      phases ^= 1u << slot;
+      uint32_t* kw = reinterpret_cast<uint32_t*>(ring + slot * S::kRun);
+      uint32_t* vw = kw + S::kPart / 4;
+      const bool whole = kp0 + kv4::kBlock - 1 <= p_min && (a.window == 0 || kp0 > p_max - a.window);
+      if (!whole) {
+        // Value pairs that are no numbers, or of tokens that no row here sees (whose bytes may be anything), are zeros from here on: what
+        // a row does not see has the weight 0, and 0 x NaN would reach it.  Rows that do see a NaN are noted.
+        bool used = false;
+        for (int t = row0 / gqa; t <= (min(G, row0 + kRows) - 1) / gqa; ++t) used |= sees(__shfl_sync(0xffffffffu, my_pos, t), kp0 + lane);
+        if (lane < kv4::kBlock) {
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            uint32_t& pair = vw[2 * D + lane * NG + j];
+            const bool number = (pair & 0x7f80u) != 0x7f80u && (pair & 0x7f800000u) != 0x7f800000u;
+            if (used && !number)
+              for (int r = row0; r < min(G, row0 + kRows); ++r)
+                if (sees(a.positions[r / gqa], kp0 + lane)) atomicOr(nan_groups + r - row0, 1 << j);
+            if (!used || !number) pair = 0u;
+          }
+        }
+        ptx::FenceProxyAsyncShared();            // (the next copy into the slot comes after these stores)
+        __syncwarp();
+      }
+
+      // ---- scores: tokens g (x[0], x[1]) and g + 8 (x[2], x[3]) of rows 2 c, 2 c + 1 ----
+      Frag sc[NT];
+      {
+        uint32_t pa[NG], pb[NG];
+        LoadWords<NG>(kw + 2 * D + g * NG, pa);
+        LoadWords<NG>(kw + 2 * D + (g + 8) * NG, pb);
+        const uint32_t mine_a = kw[2 * D + g * NG + c % NG], mine_b = kw[2 * D + (g + 8) * NG + c % NG];
+        uint32_t ca[NJ], cb[NJ];
+        if constexpr (D == 256) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int at = ((h ^ (g & 1)) * 16) + c * 4;
+            const uint4 x = *reinterpret_cast<const uint4*>(kw + g * 32 + at), y = *reinterpret_cast<const uint4*>(kw + (g + 8) * 32 + at);
+            ca[4 * h] = x.x; ca[4 * h + 1] = x.y; ca[4 * h + 2] = x.z; ca[4 * h + 3] = x.w;
+            cb[4 * h] = y.x; cb[4 * h + 1] = y.y; cb[4 * h + 2] = y.z; cb[4 * h + 3] = y.w;
+          }
+        } else {
+          LoadWords<NJ>(kw + g * (D / 8) + c * NJ, ca);
+          LoadWords<NJ>(kw + (g + 8) * (D / 8) + c * NJ, cb);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sc[nt] = MmaBf16(mine_a, mine_b, NG == 4 ? mine_a : 0u, NG == 4 ? mine_b : 0u, qpair[nt][0], qpair[nt][1], Frag{{0.f, 0.f, 0.f, 0.f}});
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          Frag s4[NT];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) s4[nt] = {{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t x = ca[2 * j + h], y = cb[2 * j + h], x8 = x >> 8, y8 = y >> 8;
+            const uint32_t a0 = Codes(x), a1 = Codes(y), a2 = Codes16(x), a3 = Codes16(y), a4 = Codes(x8), a5 = Codes(y8), a6 = Codes16(x8), a7 = Codes16(y8);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint4 b = query[(nt * NJ + 2 * j + h) * 32 + lane];
+              s4[nt] = MmaF16(a0, a1, a2, a3, b.x, b.y, s4[nt]);
+              s4[nt] = MmaF16(a4, a5, a6, a7, b.z, b.w, s4[nt]);
+            }
+          }
+          const float sa = BfLo(pa[j]), sb = BfLo(pb[j]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            sc[nt].x[0] = fmaf(sa, s4[nt].x[0], sc[nt].x[0]);
+            sc[nt].x[1] = fmaf(sa, s4[nt].x[1], sc[nt].x[1]);
+            sc[nt].x[2] = fmaf(sb, s4[nt].x[2], sc[nt].x[2]);
+            sc[nt].x[3] = fmaf(sb, s4[nt].x[3], sc[nt].x[3]);
+          }
+        }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!sees(pos[nt][e & 1], kp0 + g + (e >> 1) * 8)) sc[nt].x[e] = -INFINITY;
+      }
+
+      // ---- running maximum, power of two of the scales, probabilities ----
+      uint32_t pa[NG], pb[NG];
+      LoadWords<NG>(vw + 2 * D + g * NG, pa);
+      LoadWords<NG>(vw + 2 * D + (g + 8) * NG, pb);
+      uint32_t largest = 0u;                     // (of the lower halves)
+#pragma unroll
+      for (int j = 0; j < NG; ++j) largest = __vmaxu2(largest, __vmaxu2(pa[j], pb[j]));
+      largest &= 0xffffu;
+      bool move = largest >= limit;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) move = move || fmaxf(sc[nt].x[0], sc[nt].x[2]) > m[nt][0] + step || fmaxf(sc[nt].x[1], sc[nt].x[3]) > m[nt][1] + step;
+      if (__any_sync(0xffffffffu, move)) {
+        largest = __reduce_max_sync(0xffffffffu, largest >= 0x7f80u ? 0u : largest);
+        float shrink = 1.f;
+        if (largest >= limit) {
+          const uint32_t e = largest >> 7;
+          const float now = __uint_as_float((254u - e) << 23);
+          shrink = now / power;
+          power = now;
+          limit = (e + 7u) << 7;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float f[2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float n = fmaxf(m[nt][r], fmaxf(sc[nt].x[r], sc[nt].x[2 + r]));
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, o));
+            f[r] = n == -INFINITY ? 1.f : Exp2((m[nt][r] - n) * scale);
+            m[nt][r] = n;
+            l[nt][r] *= f[r];
+          }
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            base[nt][j][0] *= f[0];
+            base[nt][j][1] *= f[1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) acc[nt][j][e].x[x] *= f[x & 1] * shrink;
+          }
+        }
+      }
+      float p[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float r0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0] * scale, r1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1] * scale;
+        p[nt][0] = Exp2(fmaf(sc[nt].x[0], scale, -r0));
+        p[nt][1] = Exp2(fmaf(sc[nt].x[1], scale, -r1));
+        p[nt][2] = Exp2(fmaf(sc[nt].x[2], scale, -r0));
+        p[nt][3] = Exp2(fmaf(sc[nt].x[3], scale, -r1));
+        l[nt][0] += p[nt][0] + p[nt][2];
+        l[nt][1] += p[nt][1] + p[nt][3];
+      }
+
+      // ---- values: tokens 2 c, 2 c + 1 and 8 more; of every 64 channels 8 g .. ----
+      uint32_t va[NG], vb[NG], vc[NG], vd[NG];
+      if constexpr (D == 256) {
+        const int at = (g ^ (2 * c)) * 4;
+        LoadWords<NG>(vw + (2 * c) * 32 + at, va);
+        LoadWords<NG>(vw + (2 * c + 1) * 32 + at, vb);
+        LoadWords<NG>(vw + (2 * c + 8) * 32 + at, vc);
+        LoadWords<NG>(vw + (2 * c + 9) * 32 + at, vd);
+      } else {
+        const int unit = 2 * NG, at = D == 128 ? (g ^ (2 * c)) * unit : (g ^ ((c & 2) << 1)) * unit;
+        uint32_t x[2 * NG], y[2 * NG];
+        LoadWords<2 * NG>(vw + c * (D / 4) + at, x);
+        LoadWords<2 * NG>(vw + (c + 4) * (D / 4) + at, y);
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          va[j] = x[j]; vb[j] = x[NG + j];
+          vc[j] = y[j]; vd[j] = y[NG + j];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        const float sa = BfLo(pa[j]) * power, sb = BfLo(pb[j]) * power, la = BfHi(pa[j]), lb = BfHi(pb[j]);
+        uint32_t w0[NT], w1[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          w0[nt] = Transpose8x8(PackHalf(p[nt][0] * sa, p[nt][1] * sa));
+          w1[nt] = Transpose8x8(PackHalf(p[nt][2] * sb, p[nt][3] * sb));
+          base[nt][j][0] = fmaf(p[nt][0], la, fmaf(p[nt][2], lb, base[nt][j][0]));
+          base[nt][j][1] = fmaf(p[nt][1], la, fmaf(p[nt][3], lb, base[nt][j][1]));
+        }
+        uint32_t t[4] = {__byte_perm(va[j], vb[j], 0x5410), __byte_perm(va[j], vb[j], 0x7632), __byte_perm(vc[j], vd[j], 0x5410), __byte_perm(vc[j], vd[j], 0x7632)};
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const uint32_t a0 = Codes(t[0]), a1 = Codes(t[1]), a2 = Codes(t[2]), a3 = Codes(t[3]);
+          const uint32_t a4 = Codes16(t[0]), a5 = Codes16(t[1]), a6 = Codes16(t[2]), a7 = Codes16(t[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            acc[nt][j][e] = MmaF16(a0, a1, a2, a3, w0[nt], w1[nt], acc[nt][j][e]);
+            acc[nt][j][e + 1] = MmaF16(a4, a5, a6, a7, w0[nt], w1[nt], acc[nt][j][e + 1]);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) t[k] >>= 8;
+        }
+      }
+      __syncwarp();                              // every lane has read the slot
+    }
+    if (i + kStages < steps) issue(i + kStages, slot);
+    slot = slot + 1 == kStages ? 0 : slot + 1;
   }
   if (!ok) {
     // a copy did not arrive in time: the rows are NaN, the status word says so, and the copies still under way are waited for
-    l0 = l1 = __int_as_float(0x7fc00000);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) l[nt][0] = l[nt][1] = __int_as_float(0x7fc00000);
     if (lane == 0) {
       if (a.status != nullptr) atomicCAS(a.status, 0, 800 + *abort_flag);
       const long long t0 = clock64();
-      for (int k = i; k < min(steps, i + R::kStages); ++k) {
-        const int slot = k % R::kStages;
-        while (!(missing >> slot & 1u) && !ptx::MbarTryWait(full + slot, phases >> slot & 1u) && clock64() - t0 < ptx::kWaitClocks) {}
+      for (int k = i; k < min(steps, i + kStages); ++k) {
+        const int at = k % kStages;
+        while (!(missing >> at & 1u) && !ptx::MbarTryWait(full + at, phases >> at & 1u) && clock64() - t0 < ptx::kWaitClocks) {}
       }
     }
     __syncwarp();
@@ -347,67 +476,73 @@ __global__ void __launch_bounds__(kWarps * 32, 1) DecodeKv4Kernel(DecodeArgs a) 
 
   // ---- the lanes' sums of rows 2 c, 2 c + 1, then the warps' ----
 #pragma unroll
-  for (int o = 4; o < 32; o <<= 1) {
-    l0 += __shfl_xor_sync(0xffffffffu, l0, o);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int j = 0; j < NG; ++j) {
-      base[j][0] += __shfl_xor_sync(0xffffffffu, base[j][0], o);
-      base[j][1] += __shfl_xor_sync(0xffffffffu, base[j][1], o);
-    }
-  }
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        l[nt][r] += __shfl_xor_sync(0xffffffffu, l[nt][r], o);
+#pragma unroll
+        for (int j = 0; j < NG; ++j) base[nt][j][r] += __shfl_xor_sync(0xffffffffu, base[nt][j][r], o);
+      }
   __syncthreads();                               // the ring is read by no one any more
   float* merge = reinterpret_cast<float*>(smem);
-  {
-    float* dst = merge + (warp * kRows + 2 * c) * R::kStride + 8 * g;
+  const float back = 16777216.f / power, back16 = back * 0.0625f;      // codes n 2^-24, n 2^-20
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float* dst = merge + (warp * kRows + 8 * nt + 2 * c) * P::kStride + 8 * g;
 #pragma unroll
     for (int j = 0; j < NG; ++j)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float b = base[j][r];
-        *reinterpret_cast<float4*>(dst + r * R::kStride + 64 * j) = make_float4(acc[j][0][r] + b, acc[j][1][r] + b, acc[j][2][r] + b, acc[j][3][r] + b);
-        *reinterpret_cast<float4*>(dst + r * R::kStride + 64 * j + 4) =
-            make_float4(acc[j][0][2 + r] + b, acc[j][1][2 + r] + b, acc[j][2][2 + r] + b, acc[j][3][2 + r] + b);
+        const float b = base[nt][j][r];
+        const Frag(&o)[4] = acc[nt][j];
+        *reinterpret_cast<float4*>(dst + r * P::kStride + 64 * j) =
+            make_float4(fmaf(o[0].x[r], back, b), fmaf(o[1].x[r], back16, b), fmaf(o[2].x[r], back, b), fmaf(o[3].x[r], back16, b));
+        *reinterpret_cast<float4*>(dst + r * P::kStride + 64 * j + 4) =
+            make_float4(fmaf(o[0].x[2 + r], back, b), fmaf(o[1].x[2 + r], back16, b), fmaf(o[2].x[2 + r], back, b), fmaf(o[3].x[2 + r], back16, b));
       }
     if (g == 0) {
-      ml[warp * kRows + 2 * c] = make_float2(m0, l0);
-      ml[warp * kRows + 2 * c + 1] = make_float2(m1, l1);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) ml[warp * kRows + 8 * nt + 2 * c + r] = make_float2(m[nt][r] * scale, l[nt][r]);
     }
   }
   __syncthreads();
   // a warp per row
-  const int r = row0 + warp;
-  if (r >= G) return;
-  float m = -INFINITY, l = 0.f, weight[kWarps];
+  for (int rr = warp; rr < min(kRows, G - row0); rr += kWarps) {
+    const int r = row0 + rr;
+    float mx = -INFINITY, sum = 0.f, weight[kWarps];
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w * kRows + warp].x);
+    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ml[w * kRows + rr].x);
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    const float2 x = ml[w * kRows + warp];
-    weight[w] = x.x == -INFINITY ? 0.f : Exp2(x.x - m);
-    l += x.x == -INFINITY && x.y == 0.f ? 0.f : weight[w] * x.y;
-  }
-  float o[D / 32];
-#pragma unroll
-  for (int k = 0; k < D / 32; ++k) {
-    o[k] = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) o[k] = fmaf(weight[w], merge[(w * kRows + warp) * R::kStride + 32 * k + lane], o[k]);
-  }
-  if (span.active == 1) {
-    const size_t row = static_cast<size_t>(r / gqa) * a.Hq + hkv * gqa + r % gqa;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    for (int w = 0; w < kWarps; ++w) {
+      const float2 x = ml[w * kRows + rr];
+      weight[w] = x.x == -INFINITY ? 0.f : Exp2(x.x - mx);
+      sum += x.x == -INFINITY && x.y == 0.f ? 0.f : weight[w] * x.y;
+    }
+    const int nan = nan_groups[rr];
+    float o[D / 32];
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) {
-      float v = o[k] * inv;
-      if (a.qg != nullptr) v *= Sigmoid(__bfloat162float(a.qg[row * 2 * D + D + 32 * k + lane]));
-      a.out[row * D + 32 * k + lane] = __float2bfloat16_rn(v);
-    }
-  } else {
-    const size_t at = ((static_cast<size_t>(seq) * a.Hkv + hkv) * G + r) * a.splits + split;
+      o[k] = nan >> (k >> 1) & 1 ? __int_as_float(0x7fc00000) : 0.f;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) a.part_acc[at * D + 32 * k + lane] = o[k];
-    if (lane == 0) a.part_ml[at] = make_float2(m, l);
+      for (int w = 0; w < kWarps; ++w) o[k] = fmaf(weight[w], merge[(w * kRows + rr) * P::kStride + 32 * k + lane], o[k]);
+    }
+    if (span.active == 1) {
+      const size_t row = static_cast<size_t>(r / gqa) * a.Hq + hkv * gqa + r % gqa;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) {
+        float v = o[k] * inv;
+        if (a.qg != nullptr) v *= Sigmoid(__bfloat162float(a.qg[row * 2 * D + D + 32 * k + lane]));
+        a.out[row * D + 32 * k + lane] = __float2bfloat16_rn(v);
+      }
+    } else {
+      const size_t at = ((static_cast<size_t>(seq) * a.Hkv + hkv) * G + r) * a.splits + split;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) a.part_acc[at * D + 32 * k + lane] = o[k];
+      if (lane == 0) a.part_ml[at] = make_float2(mx, sum);
+    }
   }
 }
 
@@ -425,7 +560,7 @@ __global__ void __launch_bounds__(256) CombineKv4Kernel(DecodeArgs a) {
     a.positions += seq;
   }
   const int gqa = a.Hq / a.Hkv, G = gqa * a.T;
-  const int active = Visible(a.positions, a.T, a.window, a.splits).active;
+  const int active = Visible(a.positions, a.T, a.window, a.splits, a.warps).active;
   if (active == 1) return;                       // the first kernel has finished the rows
   __shared__ float wsm[kMaxSplits], red[8], lsum[8], osum[4][kCols];
   const size_t at = ((static_cast<size_t>(seq) * a.Hkv + hkv) * G + r) * a.splits;
@@ -466,14 +601,28 @@ __global__ void __launch_bounds__(256) CombineKv4Kernel(DecodeArgs a) {
   }
 }
 
-template <int D>
-int LaunchDecode(const DecodeArgs& a, int batch, cudaStream_t s) {
-  const cudaError_t e = AllowAllSharedMemory(DecodeKv4Kernel<D>);
+template <int D, int NT>
+int LaunchDecode(DecodeArgs a, int batch, cudaStream_t s) {
+  const cudaError_t e = AllowAllSharedMemory(DecodeKv4Kernel<D, NT>);
   if (e != cudaSuccess) return static_cast<int>(e);
-  const int G = a.Hq / a.Hkv * a.T, chunks = (G + kRows - 1) / kRows;
-  const int rc = LaunchPdl(DecodeKv4Kernel<D>, dim3(a.splits, a.Hkv * chunks, batch), dim3(kWarps * 32), Ring<D>::kSmem, s, a);
+  using P = Plan<D, NT>;
+  a.warps = P::kWarps;
+  const int G = a.Hq / a.Hkv * a.T, chunks = (G + P::kRows - 1) / P::kRows;
+  const int rc = LaunchPdl(DecodeKv4Kernel<D, NT>, dim3(a.splits, a.Hkv * chunks, batch), dim3(P::kWarps * 32), P::kSmem, s, a);
   if (rc || a.splits == 1) return rc;
   return LaunchPdl(CombineKv4Kernel<D>, dim3(G * (D / 64), a.Hkv, batch), dim3(256), 0, s, a);
+}
+
+// Row tiles of a CTA: as few CTAs as the registers allow read the same blocks.
+template <int D>
+int LaunchDecodeRows(const DecodeArgs& a, int batch, cudaStream_t s) {
+  const int G = a.Hq / a.Hkv * a.T;
+  if (G <= 8) return LaunchDecode<D, 1>(a, batch, s);
+  if constexpr (D == 256) {
+    return LaunchDecode<D, 2>(a, batch, s);
+  } else {
+    return G <= 16 ? LaunchDecode<D, 2>(a, batch, s) : LaunchDecode<D, 4>(a, batch, s);
+  }
 }
 
 }  // namespace
@@ -488,7 +637,7 @@ extern "C" int r4dxb_attn_decode_kv4(const void* q, const void* qg, const void* 
   if (T < 1 || T > 32 || batch < 1 || batch > 65535 || (row_slot == nullptr && batch != 1) || (row_slot != nullptr && T != 1) || Hkv < 1 || Hq < 1 ||
       Hq % Hkv || (D != 64 && D != 128 && D != 256) || splits < 1 || splits > kMaxSplits || slots < 1 || table_length < 1 || pool < 1 || window < 0)
     return R4DXB_BAD_ARG;
-  if ((static_cast<long long>(Hq / Hkv) * T + kRows - 1) / kRows * Hkv > 65535) return R4DXB_TOO_LARGE;
+  if ((static_cast<long long>(Hq / Hkv) * T + 7) / 8 * Hkv > 65535) return R4DXB_TOO_LARGE;
   if (q == nullptr || cache == nullptr || block_tables == nullptr || positions == nullptr || out == nullptr || (splits > 1 && scratch == nullptr))
     return R4DXB_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(scratch)) & 15) return R4DXB_BAD_ARG;
@@ -505,5 +654,5 @@ extern "C" int r4dxb_attn_decode_kv4(const void* q, const void* qg, const void* 
   a.status = status;
   a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.splits = splits; a.slots = slots; a.window = window;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return D == 256 ? LaunchDecode<256>(a, batch, s) : (D == 128 ? LaunchDecode<128>(a, batch, s) : LaunchDecode<64>(a, batch, s));
+  return D == 256 ? LaunchDecodeRows<256>(a, batch, s) : (D == 128 ? LaunchDecodeRows<128>(a, batch, s) : LaunchDecodeRows<64>(a, batch, s));
 }

@@ -1162,7 +1162,6 @@ register_cuda_sig("r4dxb_attn_decode_kv4", _I, [_P] * 5 + [_I] * 3 + [_P] * 3 + 
 register_cuda_sig("r4dxb_attn_prefill_kv4", _I, [_P] * 4 + [_I] * 2 + [_P] + [_I] * 6 + [_P] * 3)
 
 KV4_MAX_ROWS = 32           # rows of one sequence that attn_decode_kv4 takes
-_KV4_WARPS = 8              # of a CTA of it, each with blocks of its own
 
 
 def kv4_cache(blocks: int, Hkv: int, D: int, device="cuda") -> torch.Tensor:
@@ -1252,10 +1251,10 @@ def kv4_read(cache, block_table, positions, k: Optional[torch.Tensor] = None, v:
     return k, v
 
 
-def kv4_splits(rows: int, Hkv: int, batch: int, length: int) -> int:
-    """CTAs that share a sequence's blocks: those of a call fill the 148 SMs once, and each of a CTA's warps has a block of a full table."""
-    ctas = Hkv * batch * ((rows + 7) // 8)
-    return max(1, min(148 // ctas, (length + _KV4_WARPS - 1) // _KV4_WARPS))
+def kv4_splits(rows: int, Hkv: int, batch: int, length: int, D: int) -> int:
+    """CTAs that share a sequence's blocks: those of a call fill the 148 SMs once, and there are 128 tokens of a full table for each."""
+    tile = 8 if rows <= 8 else (16 if rows <= 16 or D == 256 else 32)
+    return max(1, min(148 // (Hkv * batch * -(-rows // tile)), (length + 7) // 8))
 
 
 def kv4_scratch_floats(T: int, batch: int, Hq: int, D: int, splits: int) -> int:
@@ -1278,7 +1277,7 @@ def attn_decode_kv4(q, qg, cache, block_table, positions, out, T: int, Hq: int, 
         _kv4_rows(qg, "qg", 2 * T * Hq * D, dev)
     rows, batch = (T, 1) if row_slot is None else (1, T)
     if splits is None:
-        splits = kv4_splits(rows * (Hq // Hkv), Hkv, batch, length)
+        splits = kv4_splits(rows * (Hq // Hkv), Hkv, batch, length, D)
     need = kv4_scratch_floats(rows, batch, Hq, D, splits)
     if need and scratch is None:
         scratch = torch.empty(need, dtype=torch.float32, device=dev)

@@ -81,5 +81,6 @@ def test_splits_fill_the_chip_once():
         for heads in (1, 2, 8):
             for batch in (1, 3, 64):
                 for length in (1, 8, 9, 5000):
-                    s = K.kv4_splits(rows, heads, batch, length)
-                    assert 1 <= s <= 148 and s <= max(1, (length + 7) // 8) and (s == 1 or s * heads * batch * -(-rows // 8) <= 148)
+                    for D, most in ((64, 32), (128, 32), (256, 16)):
+                        s = K.kv4_splits(rows, heads, batch, length, D)
+                        assert 1 <= s <= 148 and s <= max(1, (length + 7) // 8) and (s == 1 or s * heads * batch * -(-rows // most) <= 148)
