@@ -44,10 +44,13 @@ def host() -> ctypes.CDLL:
 
 def cuda() -> ctypes.CDLL:
     global _CUDA
+    if _CUDA is not None:              # (set once the signatures are: no lock on the way of every call)
+        return _CUDA
     with _LOCK:
         if _CUDA is None:
-            _CUDA = _load("libr4dxb_cuda.so", "cuda")
-            _declare_cuda(_CUDA)
+            lib = _load("libr4dxb_cuda.so", "cuda")
+            _declare_cuda(lib)
+            _CUDA = lib
         return _CUDA
 
 

@@ -13,6 +13,8 @@
 //            sum p lo per group in fp32.
 // The warps' results meet in shared memory, the splits' in a second kernel; a sequence short enough for one CTA is finished by it.
 // A row with no visible token (position -1) gives zeros; a block that the table or pool does not have gives NaN to the rows that see it.
+#include <atomic>
+
 #include "kv4.cuh"
 #include "sm100_ptx.cuh"
 
@@ -48,7 +50,8 @@ struct Plan {
   static constexpr int kMerge = kWarps * kRows * kStride * 4;
   static constexpr int kQuery = NT * (D / 32) * 512;             // operand B of the scores
   static constexpr int kBody = kRing > kMerge ? kRing : kMerge;
-  static constexpr size_t kSmem = kBody + kQuery + kWarps * kStages * 8 + kWarps * kRows * 8 + kRows * 4 + 16;
+  static constexpr int kSums = NT * (D / 32) * 8 * 4;            // of a row's query over 32 channels
+  static constexpr size_t kSmem = kBody + kQuery + kSums + kWarps * kStages * 8 + kWarps * kRows * 12 + kRows * 8 + 16;
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
@@ -114,6 +117,18 @@ __device__ __forceinline__ void LoadWords(const uint32_t* p, uint32_t (&w)[N]) {
   }
 }
 
+// Four columns of an output row, through its gate.
+__device__ __forceinline__ void StoreRow(const DecodeArgs& a, size_t row, int D, int col, float4 o) {
+  if (a.qg != nullptr) {
+    const uint2 gate = *reinterpret_cast<const uint2*>(a.qg + row * 2 * D + D + col);
+    o.x *= Sigmoid(BfLo(gate.x));
+    o.y *= Sigmoid(BfHi(gate.x));
+    o.z *= Sigmoid(BfLo(gate.y));
+    o.w *= Sigmoid(BfHi(gate.y));
+  }
+  *reinterpret_cast<uint2*>(a.out + row * D + col) = make_uint2(PackBf16(o.x, o.y), PackBf16(o.z, o.w));
+}
+
 template <int D, int NT>
 __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(DecodeArgs a) {
   PdlEnter();
@@ -122,9 +137,12 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
   constexpr int NG = S::kGroups, NJ = D / 32, kWarps = P::kWarps, kRows = P::kRows, kStages = P::kStages;
   extern __shared__ __align__(128) unsigned char smem[];
   uint4* query = reinterpret_cast<uint4*>(smem + P::kBody);                     // [row tile][32 channels][lane]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + P::kBody + P::kQuery);
+  float* sums = reinterpret_cast<float*>(smem + P::kBody + P::kQuery);          // [row tile][32 channels][row]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + P::kBody + P::kQuery + P::kSums);
   float2* ml = reinterpret_cast<float2*>(bars + kWarps * kStages);              // [warps][rows]
-  int* nan_groups = reinterpret_cast<int*>(ml + kWarps * kRows);                // [rows]: groups in which the row sees a NaN among the values
+  float* weights = reinterpret_cast<float*>(ml + kWarps * kRows);               // [warps][rows]
+  float* row_l = weights + kWarps * kRows;                                      // [rows]
+  int* nan_groups = reinterpret_cast<int*>(row_l + kRows);                      // [rows]: groups in which the row sees a NaN among the values
   volatile int* abort_flag = nan_groups + kRows;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x, hkv = blockIdx.y % a.Hkv, row0 = blockIdx.y / a.Hkv * kRows, seq = blockIdx.z;
@@ -156,65 +174,55 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
   __syncwarp();
 
   // ---- copies: block b0 + i warps into slot i % kStages ----
-  uint32_t missing = 0u, phases = 0u;          // by slot: no such block; parity of its next wait
+  uint32_t missing = 0u;                         // by slot: there is no such block
   int entry = -1;
   auto issue = [&](int i, int slot) {
     if ((i & 31) == 0) entry = i + lane < steps && known ? a.table.BlockAt(b0 + (i + lane) * kWarps) : -1;
     const int blk = __shfl_sync(0xffffffffu, entry, i & 31);
-    if (blk < 0) {
-      missing |= 1u << slot;
-      return;
-    }
-    missing &= ~(1u << slot);
+    missing = blk < 0 ? missing | 1u << slot : missing & ~(1u << slot);
     if (lane == 0) {
-      ptx::MbarArriveExpectTx(full + slot, S::kRun);
-      ptx::BulkLoad(ring + slot * S::kRun, a.cache + (static_cast<size_t>(blk) * a.Hkv + hkv) * S::kRun, S::kRun, full + slot);
+      if (blk < 0) {
+        ptx::MbarArrive(full + slot);
+      } else {
+        ptx::MbarArriveExpectTx(full + slot, S::kRun);
+        ptx::BulkLoad(ring + slot * S::kRun, a.cache + (static_cast<size_t>(blk) * a.Hkv + hkv) * S::kRun, S::kRun, full + slot);
+      }
     }
   };
   for (int i = 0; i < min(steps, kStages); ++i) issue(i, i);
 
-  // ---- query rows: a warp per row tile lays out operand B (row g; channels 32 j + 8 c .. in the order of the codes) and the sums ----
+  // ---- query rows: operand B (row g; channels 32 j + 8 c .. in the order of the codes) and its sums, a warp per 32 channels ----
   const int my_pos = (lane < a.T) ? a.positions[lane] : -1;
   auto position = [&](int r) {
     const int p = __shfl_sync(0xffffffffu, my_pos, r < G ? r / gqa : 0);
     return r < G ? p : -1;
   };
-  float qsum[NT][NG];                            // of row 8 nt + g, times 2^-28
+  for (int task = warp; task < NT * NJ; task += kWarps) {
+    const int r = row0 + task / NJ * 8 + g;
+    const uint4 v = r < G ? *reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(r / gqa) * a.Hq + hkv * gqa + r % gqa) * D + task % NJ * 32 + 8 * c)
+                          : make_uint4(0u, 0u, 0u, 0u);
+    // channels i and i + 4 for i = 0 .. 3; every second pair meets codes that carry a factor 16
+    const float x[8] = {BfLo(v.x), BfHi(v.x), BfLo(v.y), BfHi(v.y), BfLo(v.z), BfHi(v.z), BfLo(v.w), BfHi(v.w)};
+    uint32_t b[4];
+    float sum = 0.f;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = row0 + 8 * nt + g;
-    const __nv_bfloat16* src = a.q + (static_cast<size_t>(r / gqa) * a.Hq + hkv * gqa + r % gqa) * D + 8 * c;
-#pragma unroll
-    for (int j = 0; j < NG; ++j) qsum[nt][j] = 0.f;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const uint4 v = r < G ? *reinterpret_cast<const uint4*>(src + 32 * j) : make_uint4(0u, 0u, 0u, 0u);
-      // channels i and i + 4 for i = 0 .. 3; every second pair meets codes that carry a factor 16
-      const float x[8] = {BfLo(v.x), BfHi(v.x), BfLo(v.y), BfHi(v.y), BfLo(v.z), BfHi(v.z), BfLo(v.w), BfHi(v.w)};
-      uint32_t b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float f = i & 1 ? 0.00390625f : 0.0625f;
-        b[i] = PackHalf(x[i] * f, x[i + 4] * f);
-        qsum[nt][j >> 1] += (x[i] + x[i + 4]) * kUnit;
-      }
-      if (warp == nt % kWarps) query[(nt * NJ + j) * 32 + lane] = make_uint4(b[0], b[1], b[2], b[3]);
+    for (int i = 0; i < 4; ++i) {
+      const float f = i & 1 ? 0.00390625f : 0.0625f;
+      b[i] = PackHalf(x[i] * f, x[i + 4] * f);
+      sum += x[i] + x[i + 4];
     }
-#pragma unroll
-    for (int j = 0; j < NG; ++j) {
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        qsum[nt][j] += __shfl_xor_sync(0xffffffffu, qsum[nt][j], o);
-      }
-    }
+    query[task * 32 + lane] = make_uint4(b[0], b[1], b[2], b[3]);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    if (c == 0) sums[task * 8 + g] = sum * kUnit;
   }
+  __syncthreads();
   // operand B of sum_g lo sum(q): pairs (0, sum) in two (D = 256, 128) or four (64) parts of bf16
   uint32_t qpair[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    float rest = qsum[nt][0];
-#pragma unroll
-    for (int j = 1; j < NG; ++j) rest = c % NG == j ? qsum[nt][j] : rest;
+    const float* of = sums + (nt * NJ + 2 * (c % NG)) * 8 + g;
+    float rest = of[0] + of[8];
     float part = 0.f, next = 0.f;
 #pragma unroll
     for (int k = 0; k <= 4 / NG; ++k) {
@@ -226,7 +234,6 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
     qpair[nt][0] = PackBf16(0.f, part);
     qpair[nt][1] = NG == 4 ? PackBf16(0.f, next) : 0u;
   }
-  __syncthreads();
 
   const float scale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f / kUnit, step = kRescaleStep / scale;
   int pos[NT][2], p_min = 0x7fffffff, p_max = -1;
@@ -243,13 +250,18 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
   p_max = __reduce_max_sync(0xffffffffu, p_max);
   auto sees = [&](int at, int kp) { return kp <= at && (a.window == 0 || kp > at - a.window); };
 
-  float m[NT][2], l[NT][2];                      // rows 8 nt + 2 c, + 1; l of this lane's tokens
+  // steps whose blocks all rows see whole: [whole0, whole1)
+  const int stride = kWarps * kv4::kBlock, begin = b0 * kv4::kBlock;
+  const int whole1 = p_min >= begin + kv4::kBlock - 1 ? (p_min - (begin + kv4::kBlock - 1)) / stride + 1 : 0;
+  const int whole0 = a.window > 0 && p_max - a.window >= begin ? (p_max - a.window - begin) / stride + 1 : 0;
+
+  float m[NT][2], ms[NT][2], l[NT][2];           // rows 8 nt + 2 c, + 1: maximum, the same times the scale (0 for -inf), sum over this lane's tokens
   Frag acc[NT][NG][4];
   float base[NT][NG][2];                         // sum p lo of this lane's tokens
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     m[nt][0] = m[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = 0.f;
+    ms[nt][0] = ms[nt][1] = l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       base[nt][j][0] = base[nt][j][1] = 0.f;
@@ -261,10 +273,12 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
   float power = __uint_as_float((254u - 32u) << 23);      // .. than this: 2^-(exponent of the largest scale), at first 2^95
 
   bool ok = true;
-  int i = 0, slot = 0;
+  int i = 0, slot = 0, kp0 = begin;
+  uint32_t phase = 0u;
 #pragma unroll 1
-  for (; i < steps; ++i) {
-    const int kp0 = (b0 + i * kWarps) * kv4::kBlock;
+  for (; i < steps; ++i, kp0 += stride) {
+    if (!__all_sync(0xffffffffu, ptx::MbarTestWait(full + slot, phase))) ok = ptx::WarpMbarWait(full + slot, phase, abort_flag, 1);
+    if (!ok) break;
     if (missing >> slot & 1u) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -272,12 +286,9 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
         for (int r = 0; r < 2; ++r)
           if (pos[nt][r] >= kp0 && (a.window == 0 || kp0 + kv4::kBlock - 1 > pos[nt][r] - a.window)) l[nt][r] = __int_as_float(0x7fc00000);
     } else {
-      if (!__all_sync(0xffffffffu, ptx::MbarTestWait(full + slot, phases >> slot & 1u))) ok = ptx::WarpMbarWait(full + slot, phases >> slot & 1u, abort_flag, 1);
-      if (!ok) break;
-      phases ^= 1u << slot;
       uint32_t* kw = reinterpret_cast<uint32_t*>(ring + slot * S::kRun);
       uint32_t* vw = kw + S::kPart / 4;
-      const bool whole = kp0 + kv4::kBlock - 1 <= p_min && (a.window == 0 || kp0 > p_max - a.window);
+      const bool whole = i >= whole0 && i < whole1;
       if (!whole) {
         // Value pairs that are no numbers, or of tokens that no row here sees (whose bytes may be anything), are zeros from here on: what
         // a row does not see has the weight 0, and 0 x NaN would reach it.  Rows that do see a NaN are noted.
@@ -385,6 +396,7 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
             for (int o = 4; o < 32; o <<= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, o));
             f[r] = n == -INFINITY ? 1.f : Exp2((m[nt][r] - n) * scale);
             m[nt][r] = n;
+            ms[nt][r] = n == -INFINITY ? 0.f : n * scale;
             l[nt][r] *= f[r];
           }
 #pragma unroll
@@ -401,11 +413,10 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
       float p[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float r0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0] * scale, r1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1] * scale;
-        p[nt][0] = Exp2(fmaf(sc[nt].x[0], scale, -r0));
-        p[nt][1] = Exp2(fmaf(sc[nt].x[1], scale, -r1));
-        p[nt][2] = Exp2(fmaf(sc[nt].x[2], scale, -r0));
-        p[nt][3] = Exp2(fmaf(sc[nt].x[3], scale, -r1));
+        p[nt][0] = Exp2(fmaf(sc[nt].x[0], scale, -ms[nt][0]));
+        p[nt][1] = Exp2(fmaf(sc[nt].x[1], scale, -ms[nt][1]));
+        p[nt][2] = Exp2(fmaf(sc[nt].x[2], scale, -ms[nt][0]));
+        p[nt][3] = Exp2(fmaf(sc[nt].x[3], scale, -ms[nt][1]));
         l[nt][0] += p[nt][0] + p[nt][2];
         l[nt][1] += p[nt][1] + p[nt][3];
       }
@@ -457,7 +468,10 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
       __syncwarp();                              // every lane has read the slot
     }
     if (i + kStages < steps) issue(i + kStages, slot);
-    slot = slot + 1 == kStages ? 0 : slot + 1;
+    if (++slot == kStages) {
+      slot = 0;
+      phase ^= 1u;
+    }
   }
   if (!ok) {
     // a copy did not arrive in time: the rows are NaN, the status word says so, and the copies still under way are waited for
@@ -466,10 +480,8 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
     if (lane == 0) {
       if (a.status != nullptr) atomicCAS(a.status, 0, 800 + *abort_flag);
       const long long t0 = clock64();
-      for (int k = i; k < min(steps, i + kStages); ++k) {
-        const int at = k % kStages;
-        while (!(missing >> at & 1u) && !ptx::MbarTryWait(full + at, phases >> at & 1u) && clock64() - t0 < ptx::kWaitClocks) {}
-      }
+      for (int k = i; k < min(steps, i + kStages); ++k)
+        while (!ptx::MbarTryWait(full + k % kStages, static_cast<uint32_t>(k / kStages) & 1u) && clock64() - t0 < ptx::kWaitClocks) {}
     }
     __syncwarp();
   }
@@ -487,130 +499,168 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
       }
   __syncthreads();                               // the ring is read by no one any more
   float* merge = reinterpret_cast<float*>(smem);
+  // warps that had blocks (the first ones)
+  const int used = max(1, min(kWarps, min(per, span.blocks - split * per)));
   const float back = 16777216.f / power, back16 = back * 0.0625f;      // codes n 2^-24, n 2^-20
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
+    // (sixteen bytes of odd row pairs change places, so that the lanes of a store meet all banks)
     float* dst = merge + (warp * kRows + 8 * nt + 2 * c) * P::kStride + 8 * g;
+    const int h0 = (c & 1) * 4, h1 = 4 - h0;
+    if (warp < used) {
 #pragma unroll
-    for (int j = 0; j < NG; ++j)
+      for (int j = 0; j < NG; ++j)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float b = base[nt][j][r];
-        const Frag(&o)[4] = acc[nt][j];
-        *reinterpret_cast<float4*>(dst + r * P::kStride + 64 * j) =
-            make_float4(fmaf(o[0].x[r], back, b), fmaf(o[1].x[r], back16, b), fmaf(o[2].x[r], back, b), fmaf(o[3].x[r], back16, b));
-        *reinterpret_cast<float4*>(dst + r * P::kStride + 64 * j + 4) =
-            make_float4(fmaf(o[0].x[2 + r], back, b), fmaf(o[1].x[2 + r], back16, b), fmaf(o[2].x[2 + r], back, b), fmaf(o[3].x[2 + r], back16, b));
+        for (int r = 0; r < 2; ++r) {
+          const float b = base[nt][j][r];
+          const Frag(&o)[4] = acc[nt][j];
+          float* at = dst + r * P::kStride + 64 * j;
+          *reinterpret_cast<float4*>(at + h0) = make_float4(fmaf(o[0].x[r], back, b), fmaf(o[1].x[r], back16, b), fmaf(o[2].x[r], back, b), fmaf(o[3].x[r], back16, b));
+          *reinterpret_cast<float4*>(at + h1) =
+              make_float4(fmaf(o[0].x[2 + r], back, b), fmaf(o[1].x[2 + r], back16, b), fmaf(o[2].x[2 + r], back, b), fmaf(o[3].x[2 + r], back16, b));
+        }
+      if (g == 0) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) ml[warp * kRows + 8 * nt + 2 * c + r] = make_float2(m[nt][r] * scale, l[nt][r]);
       }
-    if (g == 0) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) ml[warp * kRows + 8 * nt + 2 * c + r] = make_float2(m[nt][r] * scale, l[nt][r]);
     }
   }
   __syncthreads();
-  // a warp per row
-  for (int rr = warp; rr < min(kRows, G - row0); rr += kWarps) {
-    const int r = row0 + rr;
-    float mx = -INFINITY, sum = 0.f, weight[kWarps];
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ml[w * kRows + rr].x);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float2 x = ml[w * kRows + rr];
-      weight[w] = x.x == -INFINITY ? 0.f : Exp2(x.x - mx);
-      sum += x.x == -INFINITY && x.y == 0.f ? 0.f : weight[w] * x.y;
+  const size_t part_row = ((static_cast<size_t>(seq) * a.Hkv + hkv) * G + row0) * a.splits + split;
+  if (threadIdx.x < kRows) {
+    const int r = threadIdx.x;
+    float mx = -INFINITY, sum = 0.f;
+    for (int w = 0; w < used; ++w) mx = fmaxf(mx, ml[w * kRows + r].x);
+    for (int w = 0; w < used; ++w) {
+      const float2 x = ml[w * kRows + r];
+      const float f = x.x == -INFINITY ? 0.f : Exp2(x.x - mx);
+      weights[w * kRows + r] = f;
+      sum += x.x == -INFINITY && x.y == 0.f ? 0.f : f * x.y;
     }
-    const int nan = nan_groups[rr];
-    float o[D / 32];
-#pragma unroll
-    for (int k = 0; k < D / 32; ++k) {
-      o[k] = nan >> (k >> 1) & 1 ? __int_as_float(0x7fc00000) : 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) o[k] = fmaf(weight[w], merge[(w * kRows + rr) * P::kStride + 32 * k + lane], o[k]);
+    row_l[r] = sum == 0.f ? 0.f : 1.f / sum;
+    if (span.active > 1 && row0 + r < G) a.part_ml[part_row + static_cast<size_t>(r) * a.splits] = make_float2(mx, sum);
+  }
+  __syncthreads();
+  for (int item = threadIdx.x; item < min(kRows, G - row0) * (D / 4); item += kWarps * 32) {
+    const int r = item / (D / 4), q4 = item % (D / 4);
+    const float none = nan_groups[r] >> (q4 >> 4) & 1 ? __int_as_float(0x7fc00000) : 0.f;
+    float4 o = make_float4(none, none, none, none);
+    const float* src = merge + r * P::kStride + (q4 ^ ((r >> 1) & 1)) * 4;
+    for (int w = 0; w < used; ++w) {
+      const float f = weights[w * kRows + r];
+      const float4 x = *reinterpret_cast<const float4*>(src + w * kRows * P::kStride);
+      o.x = fmaf(f, x.x, o.x);
+      o.y = fmaf(f, x.y, o.y);
+      o.z = fmaf(f, x.z, o.z);
+      o.w = fmaf(f, x.w, o.w);
     }
     if (span.active == 1) {
-      const size_t row = static_cast<size_t>(r / gqa) * a.Hq + hkv * gqa + r % gqa;
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-      for (int k = 0; k < D / 32; ++k) {
-        float v = o[k] * inv;
-        if (a.qg != nullptr) v *= Sigmoid(__bfloat162float(a.qg[row * 2 * D + D + 32 * k + lane]));
-        a.out[row * D + 32 * k + lane] = __float2bfloat16_rn(v);
-      }
+      const float inv = row_l[r];
+      const size_t row = static_cast<size_t>((row0 + r) / gqa) * a.Hq + hkv * gqa + (row0 + r) % gqa;
+      StoreRow(a, row, D, 4 * q4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     } else {
-      const size_t at = ((static_cast<size_t>(seq) * a.Hkv + hkv) * G + r) * a.splits + split;
-#pragma unroll
-      for (int k = 0; k < D / 32; ++k) a.part_acc[at * D + 32 * k + lane] = o[k];
-      if (lane == 0) a.part_ml[at] = make_float2(mx, sum);
+      *reinterpret_cast<float4*>(a.part_acc + (part_row + static_cast<size_t>(r) * a.splits) * D + 4 * q4) = o;
     }
   }
 }
 
-// grid (G D / 64, Hkv, batch), 256 threads: 64 columns x 4 groups of splits.
-constexpr int kMaxSplits = 256;
+// grid (G, Hkv, batch): a CTA per row, D / 4 columns of four times eight groups of splits.  Partial results are fetched before it is known how
+// many of them there are (the scratch has room for all), so the statistics, the results and the gate are one round trip to memory.
+constexpr int kMaxSplits = 256, kGroups = 8, kAhead = 5;
 template <int D>
-__global__ void __launch_bounds__(256) CombineKv4Kernel(DecodeArgs a) {
+__global__ void __launch_bounds__(kGroups * D / 4) CombineKv4Kernel(DecodeArgs a) {
   PdlEnter();
-  constexpr int kCols = 64;
-  const int seq = blockIdx.z, hkv = blockIdx.y, r = blockIdx.x / (D / kCols), col = blockIdx.x % (D / kCols) * kCols + (threadIdx.x & 63);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = threadIdx.x >> 6;
+  constexpr int kThreads = kGroups * D / 4;
+  const int seq = blockIdx.z, hkv = blockIdx.y, r = blockIdx.x, q4 = threadIdx.x % (D / 4), part = threadIdx.x / (D / 4);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (a.row_slot != nullptr) {
     a.out += static_cast<size_t>(seq) * a.Hq * D;
     if (a.qg != nullptr) a.qg += static_cast<size_t>(seq) * a.Hq * 2 * D;
     a.positions += seq;
   }
+  __shared__ float weight[kMaxSplits], red[kThreads / 32], lsum[kThreads / 32];
+  __shared__ float4 osum[kGroups][D / 4];
   const int gqa = a.Hq / a.Hkv, G = gqa * a.T;
+  const size_t at = ((static_cast<size_t>(seq) * a.Hkv + hkv) * G + r) * a.splits;
+  const float* src = a.part_acc + at * D + 4 * q4;
+  float4 v[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    v[i] = part + kGroups * i < a.splits ? __ldcs(reinterpret_cast<const float4*>(src + static_cast<size_t>(part + kGroups * i) * D)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  float2 x[(kMaxSplits + kThreads - 1) / kThreads];
+#pragma unroll
+  for (int k = 0; k < (kMaxSplits + kThreads - 1) / kThreads; ++k)
+    x[k] = static_cast<int>(threadIdx.x) + k * kThreads < a.splits ? a.part_ml[at + threadIdx.x + k * kThreads] : make_float2(0.f, 0.f);
   const int active = Visible(a.positions, a.T, a.window, a.splits, a.warps).active;
   if (active == 1) return;                       // the first kernel has finished the rows
-  __shared__ float wsm[kMaxSplits], red[8], lsum[8], osum[4][kCols];
-  const size_t at = ((static_cast<size_t>(seq) * a.Hkv + hkv) * G + r) * a.splits;
-  float2 x = make_float2(-INFINITY, 0.f);
-  if (static_cast<int>(threadIdx.x) < active) x = a.part_ml[at + threadIdx.x];
-  const float mx = WarpMax(x.x);
-  if (lane == 0) red[warp] = mx;
+  float m = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < (kMaxSplits + kThreads - 1) / kThreads; ++k)
+    if (static_cast<int>(threadIdx.x) + k * kThreads < active) m = fmaxf(m, x[k].x);
+  m = WarpMax(m);
+  if (lane == 0) red[warp] = m;
   __syncthreads();
-  float m = red[0];
+  m = red[0];
 #pragma unroll
-  for (int w = 1; w < 8; ++w) m = fmaxf(m, red[w]);
-  const float weight = x.x == -INFINITY ? 0.f : Exp2(x.x - m);
-  wsm[threadIdx.x] = weight;
-  const float ls = WarpSum(x.x == -INFINITY && x.y == 0.f ? 0.f : weight * x.y);
-  if (lane == 0) lsum[warp] = ls;
+  for (int w = 1; w < kThreads / 32; ++w) m = fmaxf(m, red[w]);
+  float l = 0.f;
+#pragma unroll
+  for (int k = 0; k < (kMaxSplits + kThreads - 1) / kThreads; ++k)
+    if (static_cast<int>(threadIdx.x) + k * kThreads < active) {
+      const float f = x[k].x == -INFINITY ? 0.f : Exp2(x[k].x - m);
+      weight[threadIdx.x + k * kThreads] = f;
+      l += x[k].x == -INFINITY && x[k].y == 0.f ? 0.f : f * x[k].y;
+    }
+  l = WarpSum(l);
+  if (lane == 0) lsum[warp] = l;
   __syncthreads();
-  float o = 0.f;
-  const float* src = a.part_acc + at * D + col;
-  for (int s0 = part; s0 < active; s0 += 32) {   // eight loads in flight
-    float v[8];
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](int s, const float4& p) {
+    if (s < active) {
+      const float f = weight[s];
+      o.x = fmaf(f, p.x, o.x);
+      o.y = fmaf(f, p.y, o.y);
+      o.z = fmaf(f, p.z, o.z);
+      o.w = fmaf(f, p.w, o.w);
+    }
+  };
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = s0 + 4 * i < active ? __ldcs(src + static_cast<size_t>(s0 + 4 * i) * D) : 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (s0 + 4 * i < active) o = fmaf(wsm[s0 + 4 * i], v[i], o);
-  }
-  osum[part][threadIdx.x & 63] = o;
+  for (int i = 0; i < kAhead; ++i) add(part + kGroups * i, v[i]);
+  for (int s = part + kGroups * kAhead; s < active; s += kGroups) add(s, __ldcs(reinterpret_cast<const float4*>(src + static_cast<size_t>(s) * D)));
+  osum[part][q4] = o;
   __syncthreads();
   if (part == 0) {
-    float l = 0.f;
+    l = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) l += lsum[w];
-    const int k = threadIdx.x;
-    float v = ((osum[0][k] + osum[1][k]) + (osum[2][k] + osum[3][k])) * (l == 0.f ? 0.f : 1.f / l);
-    const size_t row = static_cast<size_t>(r / gqa) * a.Hq + hkv * gqa + r % gqa;
-    if (a.qg != nullptr) v *= Sigmoid(__bfloat162float(a.qg[row * 2 * D + D + col]));
-    a.out[row * D + col] = __float2bfloat16_rn(v);
+    for (int w = 0; w < kThreads / 32; ++w) l += lsum[w];
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int k = 1; k < kGroups; ++k) {
+      const float4 p = osum[k][q4];
+      o.x += p.x; o.y += p.y; o.z += p.z; o.w += p.w;
+    }
+    StoreRow(a, static_cast<size_t>(r / gqa) * a.Hq + hkv * gqa + r % gqa, D, 4 * q4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
   }
 }
 
 template <int D, int NT>
 int LaunchDecode(DecodeArgs a, int batch, cudaStream_t s) {
-  const cudaError_t e = AllowAllSharedMemory(DecodeKv4Kernel<D, NT>);
+  // the kernel's limit of shared memory, once per device (a bit each; two threads may both set it)
+  static std::atomic<uint64_t> allowed{0};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return static_cast<int>(e);
+  if (device > 63 || !(allowed.load(std::memory_order_acquire) >> device & 1)) {
+    e = AllowAllSharedMemory(DecodeKv4Kernel<D, NT>);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    if (device < 64) allowed.fetch_or(uint64_t{1} << device, std::memory_order_release);
+  }
   using P = Plan<D, NT>;
   a.warps = P::kWarps;
   const int G = a.Hq / a.Hkv * a.T, chunks = (G + P::kRows - 1) / P::kRows;
   const int rc = LaunchPdl(DecodeKv4Kernel<D, NT>, dim3(a.splits, a.Hkv * chunks, batch), dim3(P::kWarps * 32), P::kSmem, s, a);
   if (rc || a.splits == 1) return rc;
-  return LaunchPdl(CombineKv4Kernel<D>, dim3(G * (D / 64), a.Hkv, batch), dim3(256), 0, s, a);
+  return LaunchPdl(CombineKv4Kernel<D>, dim3(G, a.Hkv, batch), dim3(kGroups * D / 4), 0, s, a);
 }
 
 // Row tiles of a CTA: as few CTAs as the registers allow read the same blocks.
@@ -640,7 +690,9 @@ extern "C" int r4dxb_attn_decode_kv4(const void* q, const void* qg, const void* 
   if ((static_cast<long long>(Hq / Hkv) * T + 7) / 8 * Hkv > 65535) return R4DXB_TOO_LARGE;
   if (q == nullptr || cache == nullptr || block_tables == nullptr || positions == nullptr || out == nullptr || (splits > 1 && scratch == nullptr))
     return R4DXB_BAD_ARG;
-  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(scratch)) & 15) return R4DXB_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(scratch)) & 15 ||
+      (reinterpret_cast<uintptr_t>(qg) | reinterpret_cast<uintptr_t>(out)) & 7)
+    return R4DXB_BAD_ARG;
   DecodeArgs a;
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.qg = static_cast<const __nv_bfloat16*>(qg);

@@ -56,6 +56,11 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def _raw_stream(index: int) -> int:
+    """Handle of the current stream of device ``index`` (`_stream` without a stream object: a tenth of its time)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _check(code: int, name: str) -> None:
     if code != 0:
         raise KernelError(f"{name} failed with code {code}")
@@ -1162,6 +1167,8 @@ register_cuda_sig("r4dxb_attn_decode_kv4", _I, [_P] * 5 + [_I] * 3 + [_P] * 3 + 
 register_cuda_sig("r4dxb_attn_prefill_kv4", _I, [_P] * 4 + [_I] * 2 + [_P] + [_I] * 6 + [_P] * 3)
 
 KV4_MAX_ROWS = 32           # rows of one sequence that attn_decode_kv4 takes
+_KV4_MAX_SPLITS = 256
+_KV4_WIDTHS = (576, 1152, 2304)      # 9 D
 
 
 def kv4_cache(blocks: int, Hkv: int, D: int, device="cuda") -> torch.Tensor:
@@ -1170,28 +1177,41 @@ def kv4_cache(blocks: int, Hkv: int, D: int, device="cuda") -> torch.Tensor:
     return torch.zeros(pool_shape(blocks, Hkv, D), dtype=torch.uint8, device=device)
 
 
-def _kv4_pool(cache: torch.Tensor, block_table: torch.Tensor, positions, row_slot, rows: int):
-    """Checks what all calls on a 4-bit cache share; (slots, table length, blocks of the pool, kv heads, head dimension)."""
-    if cache.dtype != torch.uint8 or cache.dim() != 4 or cache.shape[2] != 2 or cache.shape[3] not in (576, 1152, 2304) or not cache.is_cuda \
-            or not cache.is_contiguous() or not cache.numel():
-        raise KernelError("cache must be a contiguous CUDA uint8 pool [blocks, kv heads, 2, 9 D], D 64, 128 or 256")
-    dev = cache.device
-    if block_table.dtype != torch.int32 or block_table.device != dev or not block_table.is_contiguous() or not block_table.numel() \
-            or block_table.dim() != (1 if row_slot is None else 2):
+def _kv4_pool(cache: torch.Tensor, block_table: torch.Tensor, row_slot: Optional[torch.Tensor], rows: int):
+    """Checks what all calls on a 4-bit cache share; (device index, slots, table length, blocks of the pool, kv heads, head dimension).
+    (A decode call is a few microseconds on the device: checks ask a tensor for as little as they can.)"""
+    dev = cache.get_device()
+    shape = cache.shape
+    if cache.dtype is not torch.uint8 or len(shape) != 4 or shape[2] != 2 or shape[3] not in _KV4_WIDTHS or dev < 0 or not cache.is_contiguous() \
+            or not shape[0] or not shape[1] or cache.data_ptr() & 15:
+        raise KernelError("cache must be a contiguous, 16-byte aligned CUDA uint8 pool [blocks, kv heads, 2, 9 D], D 64, 128 or 256")
+    table = block_table.shape
+    if block_table.dtype is not torch.int32 or block_table.get_device() != dev or not block_table.is_contiguous() \
+            or len(table) != (1 if row_slot is None else 2) or 0 in table:
         raise KernelError("block_table must be a contiguous int32 tensor on the cache's device: [blocks], with row_slot [slots, blocks]")
-    for t, name in ((positions, "positions"), (row_slot, "row_slot")):
-        if t is not None and (t.dtype != torch.int32 or t.device != dev or not t.is_contiguous() or t.numel() < rows):
-            raise KernelError(f"{name} must be a contiguous int32 tensor of {rows} or more rows on the cache's device")
-    if dev.index != torch.cuda.current_device():
-        raise KernelError(f"the cache is on {dev}, which is not the current device")
-    slots = 1 if row_slot is None else block_table.shape[0]
-    return slots, block_table.shape[-1], cache.shape[0], cache.shape[1], cache.shape[3] // 9
+    if row_slot is not None:
+        _kv4_ints(row_slot, "row_slot", rows, dev)
+    if dev != torch._C._cuda_getDevice():
+        raise KernelError(f"the cache is on cuda:{dev}, which is not the current device")
+    return dev, 1 if row_slot is None else table[0], table[-1], shape[0], shape[1], shape[3] // 9
 
 
-def _kv4_rows(t: torch.Tensor, name: str, numel: int, dev) -> torch.Tensor:
-    if t.dtype != BF or t.device != dev or not t.is_contiguous() or t.numel() < numel or t.data_ptr() & 15:
-        raise KernelError(f"{name} must be a contiguous, 16-byte aligned bf16 tensor of {numel} or more elements on {dev}")
-    return t
+def _status_word(dev: int) -> int:
+    word = _STATUS.get(dev)
+    return (gemm_status(torch.device("cuda", dev)) if word is None else word).data_ptr()
+
+
+def _kv4_ints(t: torch.Tensor, name: str, n: int, dev: int) -> int:
+    if t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous() or t.numel() < n:
+        raise KernelError(f"{name} must be a contiguous int32 tensor of {n} or more elements on cuda:{dev}")
+    return t.data_ptr()
+
+
+def _kv4_rows(t: torch.Tensor, name: str, n: int, dev: int) -> int:
+    p = t.data_ptr()
+    if t.dtype is not BF or p & 15 or t.get_device() != dev or not t.is_contiguous() or t.numel() < n:
+        raise KernelError(f"{name} must be a contiguous, 16-byte aligned bf16 tensor of {n} or more elements on cuda:{dev}")
+    return p
 
 
 def attn_precore_kv4(qg, k, v, q_norm, k_norm, positions, block_table, q_out, cache, T: int, Hq: int, Hkv: int, D: int, rotary_dim: int,
@@ -1200,21 +1220,16 @@ def attn_precore_kv4(qg, k, v, q_norm, k_norm, positions, block_table, q_out, ca
     ``positions``.  q_norm / k_norm None: no per-head normalisation; q_stride 0: qg rows are q|gate pairs (2D per head).  With
     ``row_slot`` row t belongs to the sequence of table ``block_table[row_slot[t]]``.  A row whose position (-1: padding), slot or table
     entry is out of range is not written; positions of one sequence must differ within a call."""
-    slots, length, pool, heads, dim = _kv4_pool(cache, block_table, positions, row_slot, T)
+    dev, slots, length, pool, heads, dim = _kv4_pool(cache, block_table, row_slot, T)
     q_stride = q_stride or 2 * D
-    if T < 1 or Hq < 1 or (Hkv, D) != (heads, dim) or q_stride < D or q_stride % 8 or not 0 <= rotary_dim <= D or rotary_dim % 2:
+    if T < 1 or Hq < 1 or Hkv != heads or D != dim or q_stride < D or q_stride % 8 or not 0 <= rotary_dim <= D or rotary_dim % 2:
         raise KernelError(f"attn_precore_kv4: unsupported shape T={T}, Hq={Hq}, Hkv={Hkv}, D={D}, rotary_dim={rotary_dim}, q_stride={q_stride}")
-    dev = cache.device
-    _kv4_rows(qg, "qg", (T * Hq - 1) * q_stride + D, dev)
-    _kv4_rows(k, "k", T * Hkv * D, dev)
-    _kv4_rows(v, "v", T * Hkv * D, dev)
-    _kv4_rows(q_out, "q_out", T * Hq * D, dev)
-    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if w is not None:
-            _kv4_rows(w, name, D, dev)
-    _check(_lib().r4dxb_attn_precore_kv4(_p(qg), _p(k), _p(v), _p(q_norm), _p(k_norm), _p(positions), _p(block_table), _p(row_slot), slots, length,
-                                         pool, _p(q_out), _p(cache), T, Hq, Hkv, D, rotary_dim, theta, eps, q_stride, _stream()),
-           "attn_precore_kv4")
+    _check(_lib().r4dxb_attn_precore_kv4(
+        _kv4_rows(qg, "qg", (T * Hq - 1) * q_stride + D, dev), _kv4_rows(k, "k", T * Hkv * D, dev), _kv4_rows(v, "v", T * Hkv * D, dev),
+        None if q_norm is None else _kv4_rows(q_norm, "q_norm", D, dev), None if k_norm is None else _kv4_rows(k_norm, "k_norm", D, dev),
+        _kv4_ints(positions, "positions", T, dev), block_table.data_ptr(), _p(row_slot), slots, length, pool,
+        _kv4_rows(q_out, "q_out", T * Hq * D, dev), cache.data_ptr(), T, Hq, Hkv, D, rotary_dim, theta, eps, q_stride, _raw_stream(dev)),
+        "attn_precore_kv4")
     return q_out
 
 
@@ -1222,15 +1237,15 @@ def kv4_write(k, v, positions, block_table, cache, row_slot: Optional[torch.Tens
     """Quantises rows k, v [T, Hkv, D] as they are (keys already rotated) into the 4-bit cache at ``positions``; returns the cache.
     Rows and positions as in ``attn_precore_kv4``."""
     T = positions.numel()
-    slots, length, pool, Hkv, D = _kv4_pool(cache, block_table, positions, row_slot, T)
-    if not T:
-        return cache
-    for t, name in ((k, "k"), (v, "v")):
-        _kv4_rows(t, name, T * Hkv * D, cache.device)
-        if t.numel() != T * Hkv * D:
-            raise KernelError(f"{name} must hold one row of {Hkv} x {D} per position")
-    _check(_lib().r4dxb_attn_precore_kv4(None, _p(k), _p(v), None, None, _p(positions), _p(block_table), _p(row_slot), slots, length, pool, None,
-                                         _p(cache), T, 0, Hkv, D, 0, 1.0, 0.0, D, _stream()), "kv4_write")
+    dev, slots, length, pool, Hkv, D = _kv4_pool(cache, block_table, row_slot, T)
+    n = T * Hkv * D
+    if k.numel() != n or v.numel() != n:
+        raise KernelError(f"k and v must hold one row of {Hkv} x {D} per position")
+    if T:
+        _check(_lib().r4dxb_attn_precore_kv4(
+            None, _kv4_rows(k, "k", n, dev), _kv4_rows(v, "v", n, dev), None, None, _kv4_ints(positions, "positions", T, dev),
+            block_table.data_ptr(), _p(row_slot), slots, length, pool, None, cache.data_ptr(), T, 0, Hkv, D, 0, 1.0, 0.0, D, _raw_stream(dev)),
+            "kv4_write")
     return cache
 
 
@@ -1239,22 +1254,24 @@ def kv4_read(cache, block_table, positions, k: Optional[torch.Tensor] = None, v:
     """(k, v) bf16 [T, Hkv, D]: what the 4-bit cache holds at ``positions`` (any order, repeats allowed; NaN rows where a position, slot
     or table entry is out of range)."""
     T = positions.numel()
-    slots, length, pool, Hkv, D = _kv4_pool(cache, block_table, positions, row_slot, T)
+    dev, slots, length, pool, Hkv, D = _kv4_pool(cache, block_table, row_slot, T)
+    n = T * Hkv * D
     k = k if k is not None else torch.empty(T, Hkv, D, dtype=BF, device=cache.device)
     v = v if v is not None else torch.empty(T, Hkv, D, dtype=BF, device=cache.device)
-    if not T:
-        return k, v
-    for t, name in ((k, "k"), (v, "v")):
-        _kv4_rows(t, name, T * Hkv * D, cache.device)
-    _check(_lib().r4dxb_kv4_read(_p(cache), _p(block_table), _p(row_slot), slots, length, pool, _p(positions), _p(k), _p(v), T, Hkv, D, _stream()),
-           "kv4_read")
+    if T:
+        _check(_lib().r4dxb_kv4_read(
+            cache.data_ptr(), block_table.data_ptr(), _p(row_slot), slots, length, pool, _kv4_ints(positions, "positions", T, dev),
+            _kv4_rows(k, "k", n, dev), _kv4_rows(v, "v", n, dev), T, Hkv, D, _raw_stream(dev)), "kv4_read")
     return k, v
 
 
+@functools.lru_cache(maxsize=4096)
 def kv4_splits(rows: int, Hkv: int, batch: int, length: int, D: int) -> int:
-    """CTAs that share a sequence's blocks: those of a call fill the 148 SMs once, and there are 128 tokens of a full table for each."""
+    """CTAs that share a sequence's blocks: those of a call fill the 148 SMs once, and there are 128 tokens of a full table for each.  Never
+    so few that a warp adds up more than 4096 tokens: tensor-core sums round towards zero, by up to 2^-24 of the sum of codes (7.5 a
+    token) at each of its blocks, which stays below 0.1 % of a mean over equal weights there."""
     tile = 8 if rows <= 8 else (16 if rows <= 16 or D == 256 else 32)
-    return max(1, min(148 // (Hkv * batch * -(-rows // tile)), (length + 7) // 8))
+    return min(_KV4_MAX_SPLITS, max(1, min(148 // (Hkv * batch * -(-rows // tile)), (length + 7) // 8), -(-length // 2048)))
 
 
 def kv4_scratch_floats(T: int, batch: int, Hq: int, D: int, splits: int) -> int:
@@ -1267,25 +1284,26 @@ def attn_decode_kv4(q, qg, cache, block_table, positions, out, T: int, Hq: int, 
     T sequences (tables ``block_table[row_slot[t]]``).  ``gated``: times the sigmoid of the upper half of qg's heads.  ``window`` > 0: only
     the last ``window`` keys.  A position of -1 sees nothing and gives zeros; a row that sees a block which the table or pool does not have
     gives NaN.  ``scratch``: fp32, ``kv4_scratch_floats`` of it, not shared with a call that may run at the same time."""
-    slots, length, pool, heads, dim = _kv4_pool(cache, block_table, positions, row_slot, T)
-    if not 1 <= T <= (65535 if row_slot is not None else KV4_MAX_ROWS) or (Hkv, D) != (heads, dim) or Hq < 1 or Hq % Hkv or window < 0:
-        raise KernelError(f"attn_decode_kv4: unsupported shape T={T}, Hq={Hq}, Hkv={Hkv}, D={D}, window={window}")
-    dev = cache.device
-    _kv4_rows(q, "q", T * Hq * D, dev)
-    _kv4_rows(out, "out", T * Hq * D, dev)
-    if gated:
-        _kv4_rows(qg, "qg", 2 * T * Hq * D, dev)
+    dev, slots, length, pool, heads, dim = _kv4_pool(cache, block_table, row_slot, T)
     rows, batch = (T, 1) if row_slot is None else (1, T)
+    if T < 1 or rows > KV4_MAX_ROWS or batch > 65535 or Hkv != heads or D != dim or Hq < 1 or Hq % Hkv or window < 0:
+        raise KernelError(f"attn_decode_kv4: unsupported shape T={T}, Hq={Hq}, Hkv={Hkv}, D={D}, window={window}")
+    n = T * Hq * D
     if splits is None:
         splits = kv4_splits(rows * (Hq // Hkv), Hkv, batch, length, D)
-    need = kv4_scratch_floats(rows, batch, Hq, D, splits)
-    if need and scratch is None:
-        scratch = torch.empty(need, dtype=torch.float32, device=dev)
-    elif need and (scratch.dtype != torch.float32 or scratch.device != dev or not scratch.is_contiguous() or scratch.numel() < need):
-        raise KernelError(f"scratch must be a contiguous fp32 tensor of {need} or more elements on {dev}")
-    _check(_lib().r4dxb_attn_decode_kv4(_p(q), _p(qg) if gated else None, _p(cache), _p(block_table), _p(row_slot), slots, length, pool,
-                                        _p(positions), _p(scratch) if need else None, _p(out), rows, batch, Hq, Hkv, D, splits, window,
-                                        _p(gemm_status(dev)), _stream()), "attn_decode_kv4")
+    elif not 1 <= splits <= _KV4_MAX_SPLITS:
+        raise KernelError(f"attn_decode_kv4: splits={splits} not in 1 .. {_KV4_MAX_SPLITS}")
+    need = 0 if splits == 1 else n * splits // D * (D + 2)
+    if need:
+        if scratch is None:
+            scratch = torch.empty(need, dtype=torch.float32, device=cache.device)
+        elif scratch.dtype is not torch.float32 or scratch.get_device() != dev or not scratch.is_contiguous() or scratch.numel() < need \
+                or scratch.data_ptr() & 15:
+            raise KernelError(f"scratch must be a contiguous, 16-byte aligned fp32 tensor of {need} or more elements on cuda:{dev}")
+    _check(_lib().r4dxb_attn_decode_kv4(
+        _kv4_rows(q, "q", n, dev), _kv4_rows(qg, "qg", 2 * n, dev) if gated else None, cache.data_ptr(), block_table.data_ptr(), _p(row_slot),
+        slots, length, pool, _kv4_ints(positions, "positions", T, dev), scratch.data_ptr() if need else None, _kv4_rows(out, "out", n, dev),
+        rows, batch, Hq, Hkv, D, splits, window, _status_word(dev), _raw_stream(dev)), "attn_decode_kv4")
     return out
 
 
@@ -1294,16 +1312,12 @@ def attn_prefill_kv4(q, qg, cache, block_table, out, T: int, Hq: int, Hkv: int, 
     """Causal attention of T rows at positions pos0 .. over a 4-bit cache that already holds them (``attn_prefill`` for that cache, on
     tcgen05 for every head dimension, key limits included).  Keys and values are widened to fp16 values, in which magnitudes below 6e-5
     lose bits."""
-    slots, length, pool, heads, dim = _kv4_pool(cache, block_table, None, None, T)
-    if T < 1 or (Hkv, D) != (heads, dim) or Hq < 1 or Hq % Hkv or window < 0 or pos0 < 0 or pos0 + T > 1 << 30:
+    dev, slots, length, pool, heads, dim = _kv4_pool(cache, block_table, None, T)
+    if T < 1 or Hkv != heads or D != dim or Hq < 1 or Hq % Hkv or window < 0 or pos0 < 0 or pos0 + T > 1 << 30:
         raise KernelError(f"attn_prefill_kv4: unsupported shape T={T}, Hq={Hq}, Hkv={Hkv}, D={D}, pos0={pos0}, window={window}")
-    dev = cache.device
-    _kv4_rows(q, "q", T * Hq * D, dev)
-    _kv4_rows(out, "out", T * Hq * D, dev)
-    if gated:
-        _kv4_rows(qg, "qg", 2 * T * Hq * D, dev)
-    if key_limit is not None and (key_limit.dtype != torch.int32 or key_limit.device != dev or not key_limit.is_contiguous() or key_limit.numel() < T):
-        raise KernelError(f"key_limit must be a contiguous int32 tensor of {T} or more rows on {dev}")
-    _check(_lib().r4dxb_attn_prefill_kv4(_p(q), _p(qg) if gated else None, _p(cache), _p(block_table), length, pool, _p(out), T, Hq, Hkv, D, pos0,
-                                         window, _p(key_limit), _p(gemm_status(dev)), _stream()), "attn_prefill_kv4")
+    n = T * Hq * D
+    _check(_lib().r4dxb_attn_prefill_kv4(
+        _kv4_rows(q, "q", n, dev), _kv4_rows(qg, "qg", 2 * n, dev) if gated else None, cache.data_ptr(), block_table.data_ptr(), length, pool,
+        _kv4_rows(out, "out", n, dev), T, Hq, Hkv, D, pos0, window, None if key_limit is None else _kv4_ints(key_limit, "key_limit", T, dev),
+        _status_word(dev), _raw_stream(dev)), "attn_prefill_kv4")
     return out

@@ -83,4 +83,5 @@ def test_splits_fill_the_chip_once():
                 for length in (1, 8, 9, 5000):
                     for D, most in ((64, 32), (128, 32), (256, 16)):
                         s = K.kv4_splits(rows, heads, batch, length, D)
-                        assert 1 <= s <= 148 and s <= max(1, (length + 7) // 8) and (s == 1 or s * heads * batch * -(-rows // most) <= 148)
+                        least = -(-length // 2048)          # 4096 tokens a warp
+                        assert least <= s <= max(least, min(148, (length + 7) // 8)) and (s == least or s * heads * batch * -(-rows // most) <= 148)
