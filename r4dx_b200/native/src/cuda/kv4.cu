@@ -9,6 +9,8 @@
 // bf16 values brought into +-32768.  The minimum of bf16 values is one of them, so lo loses nothing; the codes are taken against
 // the rounded s, so its rounding (2^-9) only clips the top code.  Divisions are IEEE ones: the codes are those of any other
 // program that follows the definition.  A group that holds a NaN gets s = NaN and reads back as NaN throughout.
+#include <cmath>
+
 #include "kv4.cuh"
 
 namespace r4dxb {
@@ -26,48 +28,42 @@ struct PrecoreArgs {
   __nv_bfloat16* q_out;
   uint32_t* cache;
   int T, Hq, Hkv, slots, rotary_dim, q_stride;
-  float theta, eps;
+  int steps, groups;           // rounds of heads that a warp takes, warps to a token
+  float eps;
+  double turn_exponent, turn_step;      // angle of channel pair i, in turns per position: 2^(turn_exponent + i turn_step)
 };
 
-// N bf16 values from 2 N bytes at once
-template <int N>
-__device__ __forceinline__ void LoadRow(const __nv_bfloat16* p, float (&x)[N]) {
-  uint32_t w[N / 2];
-  if constexpr (N == 8) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  } else if constexpr (N == 4) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-    w[0] = v.x; w[1] = v.y;
-  } else {
-    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-  }
+__device__ __forceinline__ void Unpack8(const uint4& v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int i = 0; i < N / 2; ++i) {
+  for (int i = 0; i < 4; ++i) {
     x[2 * i] = BfLo(w[i]);
     x[2 * i + 1] = BfHi(w[i]);
   }
 }
-
-// grid (T, head groups), 8 warps: a warp per head, lane l channels l D / 32 ..  A CTA's angles are one table: for few rows they cost
-// each CTA one round of fp64 sincos, for many the table serves all heads of a token.
+__device__ __forceinline__ uint4 Load8(const __nv_bfloat16* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+// A warp has one token and some of its heads (q, then k, then v): eight channels a lane, D / 8 lanes a head, so 1, 2 or 4 heads at a time, the
+// next ones' rows on their way meanwhile.  A channel pair's angle is position x frequency in turns, in 64 bits; what its whole turns
+// leave fits 32 bits for the sine and cosine (64-bit ones took as long as all the rest).  Rotated channels change lanes by shuffle
+// where their distance is a power of two of lanes, else through shared memory.
 template <int D>
 __global__ void __launch_bounds__(256) PrecoreKv4Kernel(PrecoreArgs a) {
   PdlEnter();
-  constexpr int PER = D / 32, LANES = kv4::kGroup / PER;         // channels of a lane, lanes of a group
+  constexpr int LPH = D / 8, HPW = 32 / LPH;
   extern __shared__ float smem[];
-  const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int half = a.rotary_dim / 2, pos = a.positions[t];
-  float* cs = smem;                                              // [half] cosines, [half] sines
-  float* hrow = smem + a.rotary_dim + warp * D;
-  for (int i = threadIdx.x; i < half; i += 256) {
-    const double inv = exp2(-log2(static_cast<double>(a.theta)) * (2.0 * i / a.rotary_dim));
-    double s, c;
-    sincos(static_cast<double>(pos) * inv, &s, &c);
-    cs[i] = static_cast<float>(c);
-    cs[half + i] = static_cast<float>(s);
-  }
-  __syncthreads();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, li = lane % LPH;
+  const int task = blockIdx.x * 8 + warp, t = task / a.groups;
+  if (t >= a.T) return;
+  const int half = a.rotary_dim / 2, pos = a.positions[t], heads = a.Hq + 2 * a.Hkv;
+  float* cs = smem + warp * (a.rotary_dim + 32 * 8);             // [half] cosines, [half] sines
+  float* rows = cs + a.rotary_dim;                               // [32 lanes][8]
+  const int first = (task % a.groups) * a.steps * HPW + lane / LPH, last = min(heads, first - lane / LPH + a.steps * HPW);
+
+  auto source = [&](int hh) {
+    return hh < a.Hq ? a.qg + (static_cast<size_t>(t) * a.Hq + hh) * a.q_stride
+                     : (hh < a.Hq + a.Hkv ? a.k + (static_cast<size_t>(t) * a.Hkv + hh - a.Hq) * D : a.v + (static_cast<size_t>(t) * a.Hkv + hh - a.Hq - a.Hkv) * D);
+  };
+  uint4 next = first < last ? Load8(source(first) + 8 * li) : make_uint4(0u, 0u, 0u, 0u);
   const int slot = a.row_slot != nullptr ? a.row_slot[t] : 0;
   int blk = -1;
   if (pos >= 0 && slot >= 0 && slot < a.slots) {
@@ -76,142 +72,180 @@ __global__ void __launch_bounds__(256) PrecoreKv4Kernel(PrecoreArgs a) {
     blk = table.BlockAt(pos / kv4::kBlock);
   }
   const int tok = pos & (kv4::kBlock - 1);
-  for (int hh = blockIdx.y * 8 + warp; hh < a.Hq + 2 * a.Hkv; hh += 8 * gridDim.y) {
-    const int kind = hh < a.Hq ? 0 : (hh < a.Hq + a.Hkv ? 1 : 2);       // 0 = q, 1 = k, 2 = v
+  for (int i = lane; i < half; i += 32) {
+    const double turns = static_cast<double>(pos) * exp2(a.turn_exponent + i * a.turn_step);
+    float s, c;
+    sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
+    cs[i] = c;
+    cs[half + i] = s;
+  }
+  __syncwarp();
+  // this lane's rotated channels: d < half with the one half further on, or the other way round
+  const int hop = half / 8;                      // lanes
+  const bool shuffle = half % 8 == 0 && (hop & (hop - 1)) == 0;
+  float fc[8], fs[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int d = 8 * li + i, j = d < half ? d : d - half;
+    fc[i] = d < a.rotary_dim ? cs[j] : 1.f;
+    fs[i] = d < a.rotary_dim ? (d < half ? -cs[half + j] : cs[half + j]) : 0.f;
+  }
+  uint4 norm = make_uint4(0u, 0u, 0u, 0u);       // the weights of the kind at hand
+  int norm_kind = -1;
+
+  for (int step = 0; step < a.steps; ++step) {
+    const int hh = first + step * HPW;
+    const uint4 raw = next;
+    if (step + 1 < a.steps && hh + HPW < last) next = Load8(source(hh + HPW) + 8 * li);
+    if (hh - lane / LPH >= last) break;          // (the warp's heads are done)
+    const int kind = hh >= last ? 3 : (hh < a.Hq ? 0 : (hh < a.Hq + a.Hkv ? 1 : 2));       // 0 = q, 1 = k, 2 = v, 3 = none
     const int head = kind == 0 ? hh : (kind == 1 ? hh - a.Hq : hh - a.Hq - a.Hkv);
-    if (kind != 0 && blk < 0) continue;
-    const __nv_bfloat16* src = kind == 0 ? a.qg + (static_cast<size_t>(t) * a.Hq + head) * a.q_stride
-                                         : (kind == 1 ? a.k : a.v) + (static_cast<size_t>(t) * a.Hkv + head) * D;
-    float x[PER];
-    LoadRow<PER>(src + lane * PER, x);
-    if (kind != 2) {
-      const __nv_bfloat16* nw = kind == 0 ? a.q_norm : a.k_norm;
+    float x[8];
+    Unpack8(raw, x);
+    const __nv_bfloat16* nw = kind == 0 ? a.q_norm : (kind == 1 ? a.k_norm : nullptr);
+    if (nw != nullptr && kind != norm_kind) {
+      norm = Load8(nw + 8 * li);
+      norm_kind = kind;
+    }
+    if (a.q_norm != nullptr || a.k_norm != nullptr) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+#pragma unroll
+      for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
       if (nw != nullptr) {
-        float ss = 0.f;
+        const float r = rsqrtf(ss / D + a.eps);
+        float w[8];
+        Unpack8(norm, w);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) ss += x[i] * x[i];
-        const float r = rsqrtf(WarpSum(ss) / D + a.eps);
-        float w[PER];
-        LoadRow<PER>(nw + lane * PER, w);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) x[i] = x[i] * r * (1.0f + w[i]);
+        for (int i = 0; i < 8; ++i) x[i] = x[i] * r * (1.0f + w[i]);
       }
-      if (half > 0) {
+    }
+    if (half > 0) {
+      float y[8];
+      if (shuffle) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __shfl_xor_sync(0xffffffffu, x[i], hop);
+      } else {
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < PER; ++i) hrow[lane * PER + i] = x[i];
+        for (int i = 0; i < 8; ++i) rows[lane * 8 + i] = x[i];
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int d = lane * PER + i;
-          if (d < a.rotary_dim) {
-            const int j = d < half ? d : d - half;
-            const float fc = cs[j], fs = cs[half + j];
-            x[i] = d < half ? hrow[d] * fc - hrow[d + half] * fs : hrow[d] * fc + hrow[d - half] * fs;
-          }
+        for (int i = 0; i < 8; ++i) {
+          const int d = 8 * li + i;
+          y[i] = d < a.rotary_dim ? rows[(lane - li) * 8 + (d < half ? d + half : d - half)] : 0.f;
         }
       }
-    }
-    uint32_t packed[PER / 2];
+      if (kind < 2) {
 #pragma unroll
-    for (int i = 0; i < PER / 2; ++i) packed[i] = PackBf16(x[2 * i], x[2 * i + 1]);
-    if (kind == 0) {
-      __nv_bfloat16* dst = a.q_out + (static_cast<size_t>(t) * a.Hq + head) * D + lane * PER;
-      if constexpr (PER == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-      else if constexpr (PER == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[1]);
-      else *reinterpret_cast<uint32_t*>(dst) = packed[0];
-      continue;
+        for (int i = 0; i < 8; ++i)
+          if (8 * li + i < a.rotary_dim) x[i] = x[i] * fc[i] + y[i] * fs[i];
+      }
     }
+    const uint4 packed = make_uint4(PackBf16(x[0], x[1]), PackBf16(x[2], x[3]), PackBf16(x[4], x[5]), PackBf16(x[6], x[7]));
+    if (kind == 0) *reinterpret_cast<uint4*>(a.q_out + (static_cast<size_t>(t) * a.Hq + head) * D + 8 * li) = packed;
+    if (__all_sync(0xffffffffu, kind == 0)) continue;
+    Unpack8(packed, x);
     bool nan = false;
     float lo = kv4::kLimit, hi = -kv4::kLimit;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      x[i] = (i & 1) ? BfHi(packed[i / 2]) : BfLo(packed[i / 2]);
+    for (int i = 0; i < 8; ++i) {
       nan |= x[i] != x[i];
       x[i] = fminf(fmaxf(x[i], -kv4::kLimit), kv4::kLimit);
       lo = fminf(lo, x[i]);
       hi = fmaxf(hi, x[i]);
     }
 #pragma unroll
-    for (int o = 1; o < LANES; o <<= 1) {
+    for (int o = 1; o < 8; o <<= 1) {            // the eight lanes of a group
       lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
       hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
-    const uint32_t nans = __ballot_sync(0xffffffffu, nan);
-    constexpr uint32_t kOne = LANES == 32 ? 0xffffffffu : (1u << (LANES & 31)) - 1u;
-    const bool bad = (nans >> (lane / LANES * LANES) & kOne) != 0u;
+    const bool bad = (__ballot_sync(0xffffffffu, nan) >> (lane & ~7) & 0xffu) != 0u;
     const __nv_bfloat16 sb = __float2bfloat16_rn(bad ? __int_as_float(0x7fc00000) : __fdiv_rn(hi - lo, 15.f));
     const float s = __bfloat162float(sb);
     uint32_t codes = 0u;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const float n = s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x[i] - lo, s)), 0.f), 15.f) : 0.f;
       codes |= static_cast<uint32_t>(n) << (4 * i);
     }
-    // the lanes of a word: D = 256 one, 128 two, 64 four
-#pragma unroll
-    for (int o = 1; o < 8 / PER; o <<= 1) {
-      const uint32_t other = __shfl_xor_sync(0xffffffffu, codes, o);
-      codes = lane & o ? other | codes << (4 * PER * o) : codes | other << (4 * PER * o);
+    if (kind >= 1 && kind <= 2 && blk >= 0) {
+      uint32_t* part = a.cache + ((static_cast<size_t>(blk) * a.Hkv + head) * 2 + (kind - 1)) * (kv4::Shape<D>::kPart / 4);
+      part[kind == 1 ? kv4::Word<D, false>(tok, li) : kv4::Word<D, true>(tok, li)] = codes;
+      if (li % 8 == 0)
+        part[2 * D + tok * kv4::Shape<D>::kGroups + li / 8] =
+            static_cast<uint32_t>(__bfloat16_as_ushort(sb)) | static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(lo))) << 16;
     }
-    uint32_t* part = a.cache + ((static_cast<size_t>(blk) * a.Hkv + head) * 2 + (kind - 1)) * (kv4::Shape<D>::kPart / 4);
-    const int w = lane * PER / 8;
-    if (lane % (8 / PER) == 0) part[kind == 1 ? kv4::Word<D, false>(tok, w) : kv4::Word<D, true>(tok, w)] = codes;
-    if (lane % LANES == 0)
-      part[2 * D + tok * kv4::Shape<D>::kGroups + lane / LANES] =
-          static_cast<uint32_t>(__bfloat16_as_ushort(sb)) | static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(lo))) << 16;
   }
 }
 
-// A thread per word of eight channels: [row][head][keys, values][word].
-template <int D>
+// Rows read back: a thread has one word (eight channels) of a row and up to ITEMS of its 2 Hkv heads' keys and values, whose codes and pairs it
+// asks for at once.  (A thread per value word, each with the row's position and table entry to find first, took 62 us for 32517 rows of
+// 8 heads of 128 where the bytes take 26.)
+template <int D, int ITEMS>
 __global__ void __launch_bounds__(256) ReadKv4Kernel(const uint32_t* __restrict__ cache, kv4::Table table, const int* __restrict__ positions,
                                                      const int* __restrict__ row_slot, int slots, __nv_bfloat16* __restrict__ k,
-                                                     __nv_bfloat16* __restrict__ v, long long words, int Hkv) {
+                                                     __nv_bfloat16* __restrict__ v, int T, int Hkv) {
   PdlEnter();
   using S = kv4::Shape<D>;
-  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= words) return;
-  const int w = static_cast<int>(i % S::kWords), part = static_cast<int>(i / S::kWords) & 1;
-  const long long rh = i / (2 * S::kWords);                     // row * Hkv + head
-  const int head = static_cast<int>(rh % Hkv), t = static_cast<int>(rh / Hkv);
+  const int w = threadIdx.x % S::kWords, t = blockIdx.x * (256 / S::kWords) + threadIdx.x / S::kWords;
+  if (t >= T) return;
   const int pos = positions[t], slot = row_slot != nullptr ? row_slot[t] : 0;
   int blk = -1;
   if (pos >= 0 && slot >= 0 && slot < slots) {
     table.entries += static_cast<size_t>(slot) * table.length;
     blk = table.BlockAt(pos / kv4::kBlock);
   }
-  uint4 o = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
-  if (blk >= 0) {
-    const int tok = pos & (kv4::kBlock - 1);
-    const uint32_t* at = cache + ((static_cast<size_t>(blk) * Hkv + head) * 2 + part) * (S::kPart / 4);
-    const uint32_t codes = __ldg(at + (part == 0 ? kv4::Word<D, false>(tok, w) : kv4::Word<D, true>(tok, w)));
-    const uint32_t pair = __ldg(at + 2 * D + tok * S::kGroups + w / 8);
-    const float s = BfLo(pair), lo = BfHi(pair);
+  const int tok = pos & (kv4::kBlock - 1), first = blockIdx.y * ITEMS;
+  const int at_k = kv4::Word<D, false>(tok, w), at_v = kv4::Word<D, true>(tok, w), at_pair = 2 * D + tok * S::kGroups + w / 8;
+  uint32_t codes[ITEMS], pair[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {              // item: head, then keys or values - the order of the pool
+    codes[i] = 0u;
+    pair[i] = 0x7fc07fc0u;
+    if (blk >= 0 && first + i < 2 * Hkv) {
+      const uint32_t* part = cache + (static_cast<size_t>(blk) * 2 * Hkv + first + i) * (S::kPart / 4);
+      codes[i] = __ldg(part + ((first + i) & 1 ? at_v : at_k));
+      pair[i] = __ldg(part + at_pair);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    if (first + i >= 2 * Hkv) break;
+    const float s = BfLo(pair[i]), lo = BfHi(pair[i]);
     uint32_t p[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      p[c] = PackBf16(fmaf(static_cast<float>(codes >> (8 * c) & 15u), s, lo), fmaf(static_cast<float>(codes >> (8 * c + 4) & 15u), s, lo));
-    o = make_uint4(p[0], p[1], p[2], p[3]);
+      p[c] = PackBf16(fmaf(static_cast<float>(codes[i] >> (8 * c) & 15u), s, lo), fmaf(static_cast<float>(codes[i] >> (8 * c + 4) & 15u), s, lo));
+    *reinterpret_cast<uint4*>(((first + i) & 1 ? v : k) + (static_cast<size_t>(t) * Hkv + (first + i) / 2) * D + 8 * w) = make_uint4(p[0], p[1], p[2], p[3]);
   }
-  *reinterpret_cast<uint4*>((part == 0 ? k : v) + rh * D + 8 * w) = o;
 }
 
 template <int D>
-int LaunchPrecore(const PrecoreArgs& a, cudaStream_t s) {
-  // enough CTAs for eight to an SM where there are few rows, one CTA (and one table of angles) a row where there are many
-  const int groups = (a.Hq + 2 * a.Hkv + 7) / 8, most = (8 * 148 + a.T - 1) / a.T;
-  const size_t smem = (a.rotary_dim + 8 * D) * sizeof(float);
-  return LaunchPdl(PrecoreKv4Kernel<D>, dim3(a.T, groups < most ? groups : most), dim3(256), smem, s, a);
+int LaunchPrecore(PrecoreArgs a, cudaStream_t s) {
+  // warps for every SM four times over where there are rows enough; up to eight rounds of heads to a warp, which share its angles
+  const int per_round = 256 / D, rounds = (a.Hq + 2 * a.Hkv + per_round - 1) / per_round;
+  const long long most = static_cast<long long>(a.T) * rounds / (4 * 148 * 32);
+  a.steps = static_cast<int>(most < 1 ? 1 : (most > 8 ? 8 : most));
+  a.groups = (rounds + a.steps - 1) / a.steps;
+  const long long tasks = static_cast<long long>(a.T) * a.groups;
+  if (tasks > 0x7fffffffll - 8) return R4DXB_TOO_LARGE;
+  const size_t smem = 8 * (a.rotary_dim + 32 * 8) * sizeof(float);
+  return LaunchPdl(PrecoreKv4Kernel<D>, dim3(static_cast<unsigned>((tasks + 7) / 8)), dim3(256), smem, s, a);
 }
 
 template <int D>
 int LaunchRead(const void* cache, const kv4::Table& table, const int* positions, const int* row_slot, int slots, void* k, void* v, int T, int Hkv,
                cudaStream_t s) {
-  const long long words = static_cast<long long>(T) * Hkv * 2 * kv4::Shape<D>::kWords;
-  if ((words + 255) / 256 > 0x7fffffffll) return R4DXB_TOO_LARGE;
-  return LaunchPdl(ReadKv4Kernel<D>, dim3(static_cast<unsigned>((words + 255) / 256)), dim3(256), 0, s, static_cast<const uint32_t*>(cache), table,
-                   positions, row_slot, slots, static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v), words, Hkv);
+  constexpr int kRows = 256 / kv4::Shape<D>::kWords;
+  if (Hkv > 32767) return R4DXB_TOO_LARGE;
+  const unsigned rows = (static_cast<unsigned>(T) + kRows - 1) / kRows, items = 2 * Hkv;
+  auto launch = [&](auto kern, unsigned per) {
+    return LaunchPdl(kern, dim3(rows, (items + per - 1) / per), dim3(256), 0, s, static_cast<const uint32_t*>(cache), table, positions, row_slot, slots,
+                     static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v), T, Hkv);
+  };
+  return static_cast<unsigned long long>(rows) * items >= 8 * 8 * 148 ? launch(ReadKv4Kernel<D, 8>, 8) : launch(ReadKv4Kernel<D, 1>, 1);
 }
 
 bool Misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
@@ -226,7 +260,7 @@ extern "C" {
 int r4dxb_attn_precore_kv4(const void* qg, const void* k, const void* v, const void* q_norm, const void* k_norm, const int* positions,
                            const int* block_tables, const int* row_slot, int slots, int table_length, int pool, void* q_out, void* cache, int T,
                            int Hq, int Hkv, int D, int rotary_dim, float theta, float eps, int q_stride, void* stream) {
-  if (T < 1 || Hq < 0 || Hkv < 1 || (D != 64 && D != 128 && D != 256) || rotary_dim < 0 || rotary_dim > D || rotary_dim % 2 || slots < 1 ||
+  if (T < 1 || Hq < 0 || Hkv < 1 || (D != 64 && D != 128 && D != 256) || rotary_dim < 0 || rotary_dim > D || rotary_dim % 2 || (rotary_dim > 0 && !(theta > 0.f)) || slots < 1 ||
       table_length < 1 || pool < 1 || q_stride < D || q_stride % 8 || k == nullptr || v == nullptr || positions == nullptr ||
       block_tables == nullptr || cache == nullptr || (Hq > 0 && (qg == nullptr || q_out == nullptr)))
     return R4DXB_BAD_ARG;
@@ -243,7 +277,9 @@ int r4dxb_attn_precore_kv4(const void* qg, const void* k, const void* v, const v
   a.table = {block_tables, table_length, pool};
   a.q_out = static_cast<__nv_bfloat16*>(q_out);
   a.cache = static_cast<uint32_t*>(cache);
-  a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.slots = slots; a.rotary_dim = rotary_dim; a.q_stride = q_stride; a.theta = theta; a.eps = eps;
+  a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.slots = slots; a.rotary_dim = rotary_dim; a.q_stride = q_stride; a.eps = eps;
+  a.turn_step = rotary_dim > 0 ? -2.0 / rotary_dim * std::log2(static_cast<double>(theta)) : 0.0;
+  a.turn_exponent = -2.651496129472319;          // -log2(2 pi)
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return D == 256 ? LaunchPrecore<256>(a, s) : (D == 128 ? LaunchPrecore<128>(a, s) : LaunchPrecore<64>(a, s));
 }
