@@ -7,11 +7,12 @@
 //
 // Codes of a group of 64 channels:  lo = min x,  s = bf16((max x - lo) / 15),  n = clamp(rint((x - lo) / s), 0, 15), with x the row's
 // bf16 values brought into +-32768.  The minimum of bf16 values is one of them, so lo loses nothing; the codes are taken against
-// the rounded s, so its rounding (2^-9) only clips the top code.  Divisions are IEEE ones: the codes are those of any other
+// the rounded s, so its rounding (2^-8) only clips the top code.  Quotients are those of IEEE divisions: the codes are those of any other
 // program that follows the definition.  A group that holds a NaN gets s = NaN and reads back as NaN throughout.
 #include <cmath>
 
 #include "kv4.cuh"
+#include "sm100_ptx.cuh"
 
 namespace r4dxb {
 namespace {
@@ -28,24 +29,179 @@ struct PrecoreArgs {
   __nv_bfloat16* q_out;
   uint32_t* cache;
   int T, Hq, Hkv, slots, rotary_dim, q_stride;
-  int steps, groups;           // rounds of heads that a warp takes, warps to a token
+  int steps, groups;           // rounds of heads that a warp takes at most, warps to a token
   float eps;
   double turn_exponent, turn_step;      // angle of channel pair i, in turns per position: 2^(turn_exponent + i turn_step)
 };
 
-__device__ __forceinline__ void Unpack8(const uint4& v, float (&x)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = BfLo(w[i]);
-    x[2 * i + 1] = BfHi(w[i]);
-  }
+// eight bf16 values as pairs, and back
+__device__ __forceinline__ void Unpack8(const uint4& v, float2 (&x)[4]) {
+  x[0] = make_float2(BfLo(v.x), BfHi(v.x));
+  x[1] = make_float2(BfLo(v.y), BfHi(v.y));
+  x[2] = make_float2(BfLo(v.z), BfHi(v.z));
+  x[3] = make_float2(BfLo(v.w), BfHi(v.w));
+}
+__device__ __forceinline__ uint4 Pack8(const float2 (&x)[4]) {
+  return make_uint4(PackBf16(x[0].x, x[0].y), PackBf16(x[1].x, x[1].y), PackBf16(x[2].x, x[2].y), PackBf16(x[3].x, x[3].y));
 }
 __device__ __forceinline__ uint4 Load8(const __nv_bfloat16* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
-// A warp has one token and some of its heads (q, then k, then v): eight channels a lane, D / 8 lanes a head, so 1, 2 or 4 heads at a time, the
-// next ones' rows on their way meanwhile.  A channel pair's angle is position x frequency in turns, in 64 bits; what its whole turns
-// leave fits 32 bits for the sine and cosine (64-bit ones took as long as all the rest).  Rotated channels change lanes by shuffle
-// where their distance is a power of two of lanes, else through shared memory.
+__device__ __forceinline__ float2 Mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// What a warp knows of its token.
+struct Token {
+  int t, tok, blk, lane, li;
+  float2 fc[4], fs[4];         // this lane's rotated channels: own value x fc + the partner channel's x fs
+  float* rows;                 // [32 lanes][8] of shared memory
+};
+
+// Rounds of heads `first` .. (one, two or four at a time, lane / (D / 8)) of one kind: q (KIND 0), k (1) or v (2); two rounds in flight.
+template <int D, int KIND>
+__device__ __forceinline__ void Heads(const PrecoreArgs& a, const Token& tk, int first, int rounds) {
+  constexpr int LPH = D / 8, HPW = 32 / LPH, AHEAD = 2;
+  const int heads = KIND == 0 ? a.Hq : a.Hkv, li = tk.li, lane = tk.lane;
+  const __nv_bfloat16* src = KIND == 0 ? a.qg + static_cast<size_t>(tk.t) * a.Hq * a.q_stride : (KIND == 1 ? a.k : a.v) + static_cast<size_t>(tk.t) * a.Hkv * D;
+  const int step = KIND == 0 ? a.q_stride : D;
+  const __nv_bfloat16* norm = KIND == 0 ? a.q_norm : (KIND == 1 ? a.k_norm : nullptr);
+  float2 w[4];
+  if (norm != nullptr) {
+    Unpack8(Load8(norm + 8 * li), w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = make_float2(1.0f + w[i].x, 1.0f + w[i].y);
+  }
+  // partner channels: by shuffle where they are a power of two of lanes away
+  const int half = a.rotary_dim / 2, hop = half / 8;
+  const bool shuffle = half % 8 == 0 && (hop & (hop - 1)) == 0;
+
+  auto load = [&](int round) {
+    const int head = first + round * HPW;
+    return round < rounds && head < heads ? Load8(src + static_cast<size_t>(head) * step + 8 * li) : make_uint4(0u, 0u, 0u, 0u);
+  };
+  uint4 next[AHEAD];
+#pragma unroll
+  for (int u = 0; u < AHEAD; ++u) next[u] = load(u);
+#pragma unroll 1
+  for (int round = 0; round < rounds; round += AHEAD) {
+    float2 x[AHEAD][4];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      Unpack8(next[u], x[u]);
+      next[u] = load(round + AHEAD + u);
+    }
+    if (KIND < 2 && norm != nullptr) {
+      float ss[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        float2 p = Mul2(x[u][0], x[u][0]);
+#pragma unroll
+        for (int i = 1; i < 4; ++i) p = ptx::Fma2(x[u][i], x[u][i], p);
+        ss[u] = p.x + p.y;
+      }
+#pragma unroll
+      for (int o = 1; o < LPH; o <<= 1)
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) ss[u] += __shfl_xor_sync(0xffffffffu, ss[u], o);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const float r = rsqrtf(ss[u] * (1.0f / D) + a.eps);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[u][i] = Mul2(Mul2(x[u][i], make_float2(r, r)), w[i]);
+      }
+    }
+    if (KIND < 2 && half > 0) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        float2 y[4];
+        if (shuffle) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = make_float2(__shfl_xor_sync(0xffffffffu, x[u][i].x, hop), __shfl_xor_sync(0xffffffffu, x[u][i].y, hop));
+          if (8 * li < a.rotary_dim) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[u][i] = ptx::Fma2(x[u][i], tk.fc[i], Mul2(y[i], tk.fs[i]));
+          }
+        } else {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *reinterpret_cast<float2*>(tk.rows + lane * 8 + 2 * i) = x[u][i];
+          __syncwarp();
+          auto turn = [&](float& v, int d, float c, float s) {
+            if (d < a.rotary_dim) v = fmaf(v, c, tk.rows[(lane - li) * 8 + (d < half ? d + half : d - half)] * s);
+          };
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            turn(x[u][i].x, 8 * li + 2 * i, tk.fc[i].x, tk.fs[i].x);
+            turn(x[u][i].y, 8 * li + 2 * i + 1, tk.fc[i].y, tk.fs[i].y);
+          }
+        }
+      }
+    }
+    if constexpr (KIND == 0) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int head = first + (round + u) * HPW;
+        if (round + u < rounds && head < heads) *reinterpret_cast<uint4*>(a.q_out + (static_cast<size_t>(tk.t) * a.Hq + head) * D + 8 * li) = Pack8(x[u]);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const uint4 bits = Pack8(x[u]);
+        Unpack8(bits, x[u]);
+        // the largest magnitudes of the two halves of the words: beyond the limit or no number at all?
+        const uint32_t mag = __vmaxu2(__vmaxu2(bits.x & 0x7fff7fffu, bits.y & 0x7fff7fffu), __vmaxu2(bits.z & 0x7fff7fffu, bits.w & 0x7fff7fffu));
+        const uint32_t top = max(mag >> 16, mag & 0xffffu);
+        if (__any_sync(0xffffffffu, top > 0x4700u)) {           // 32768
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[u][i].x = fminf(fmaxf(x[u][i].x, -kv4::kLimit), kv4::kLimit);
+            x[u][i].y = fminf(fmaxf(x[u][i].y, -kv4::kLimit), kv4::kLimit);
+          }
+        }
+        float lo = fminf(fminf(fminf(x[u][0].x, x[u][0].y), fminf(x[u][1].x, x[u][1].y)), fminf(fminf(x[u][2].x, x[u][2].y), fminf(x[u][3].x, x[u][3].y)));
+        float hi = fmaxf(fmaxf(fmaxf(x[u][0].x, x[u][0].y), fmaxf(x[u][1].x, x[u][1].y)), fmaxf(fmaxf(x[u][2].x, x[u][2].y), fmaxf(x[u][3].x, x[u][3].y)));
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {        // the eight lanes of a group
+          lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+          hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        const bool bad = (__ballot_sync(0xffffffffu, top > 0x7f80u) >> (lane & ~7) & 0xffu) != 0u;
+        const __nv_bfloat16 sb = __float2bfloat16_rn(bad ? __int_as_float(0x7fc00000) : __fdiv_rn(hi - lo, 15.f));
+        const float s = __bfloat162float(sb);
+        // (x - lo) / s as the IEEE division gives it, without its branches: from the rounded reciprocal two steps of remainder and correction
+        // (Markstein); scales near the bottom of the range are lifted first, which changes no quotient
+        const float lift = s < 1e-18f ? 18446744073709551616.f : 1.f, sl = s * lift, inv = s > 0.f ? __frcp_rn(sl) : 0.f;
+        uint32_t codes = 0u;
+        auto code = [&](float v, int at) {
+          const float d = (v - lo) * lift;
+          float n = d * inv;
+          n = fmaf(fmaf(-n, sl, d), inv, n);
+          n = fmaf(fmaf(-n, sl, d), inv, n);
+          n = fminf(fmaxf(n, 0.f), 15.f) + 12582912.f;          // 1.5 x 2^23: the integer, rounded to even at halves, in the lowest bits
+          codes |= (__float_as_uint(n) & 15u) << (4 * at);
+        };
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          code(x[u][i].x, 2 * i);
+          code(x[u][i].y, 2 * i + 1);
+        }
+        const int head = first + (round + u) * HPW;
+        if (round + u < rounds && head < heads) {
+          uint32_t* part = a.cache + ((static_cast<size_t>(tk.blk) * a.Hkv + head) * 2 + (KIND - 1)) * (kv4::Shape<D>::kPart / 4);
+          part[kv4::Word<D, KIND == 2>(tk.tok, li)] = codes;
+          if (li % 8 == 0)
+            part[2 * D + tk.tok * kv4::Shape<D>::kGroups + li / 8] =
+                static_cast<uint32_t>(__bfloat16_as_ushort(sb)) | static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(lo))) << 16;
+        }
+      }
+    }
+  }
+}
+
+// A warp has one token and some of its q, its k or its v heads: eight channels a lane, D / 8 lanes a head.  A channel pair's angle is position x
+// frequency in turns, in 64 bits; what its whole turns leave fits 32 bits for the sine and cosine.
 template <int D>
 __global__ void __launch_bounds__(256) PrecoreKv4Kernel(PrecoreArgs a) {
   PdlEnter();
@@ -54,130 +210,53 @@ __global__ void __launch_bounds__(256) PrecoreKv4Kernel(PrecoreArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, li = lane % LPH;
   const int task = blockIdx.x * 8 + warp, t = task / a.groups;
   if (t >= a.T) return;
-  const int half = a.rotary_dim / 2, pos = a.positions[t], heads = a.Hq + 2 * a.Hkv;
+  int part = task % a.groups;
+  const int rounds_q = (a.Hq + HPW - 1) / HPW, rounds_kv = (a.Hkv + HPW - 1) / HPW;
+  const int parts_q = (rounds_q + a.steps - 1) / a.steps, parts_kv = (rounds_kv + a.steps - 1) / a.steps;
+  const int kind = part < parts_q ? 0 : (part < parts_q + parts_kv ? 1 : 2);
+  part -= kind == 0 ? 0 : (kind == 1 ? parts_q : parts_q + parts_kv);
+  const int pos = a.positions[t], half = a.rotary_dim / 2;
+  Token tk;
+  tk.t = t;
+  tk.lane = lane;
+  tk.li = li;
+  tk.tok = pos & (kv4::kBlock - 1);
+  tk.blk = -1;
+  if (kind != 0) {
+    const int slot = a.row_slot != nullptr ? a.row_slot[t] : 0;
+    if (pos >= 0 && slot >= 0 && slot < a.slots) {
+      kv4::Table table = a.table;
+      table.entries += static_cast<size_t>(slot) * table.length;
+      tk.blk = table.BlockAt(pos / kv4::kBlock);
+    }
+    if (tk.blk < 0) return;
+  }
   float* cs = smem + warp * (a.rotary_dim + 32 * 8);             // [half] cosines, [half] sines
-  float* rows = cs + a.rotary_dim;                               // [32 lanes][8]
-  const int first = (task % a.groups) * a.steps * HPW + lane / LPH, last = min(heads, first - lane / LPH + a.steps * HPW);
-
-  auto source = [&](int hh) {
-    return hh < a.Hq ? a.qg + (static_cast<size_t>(t) * a.Hq + hh) * a.q_stride
-                     : (hh < a.Hq + a.Hkv ? a.k + (static_cast<size_t>(t) * a.Hkv + hh - a.Hq) * D : a.v + (static_cast<size_t>(t) * a.Hkv + hh - a.Hq - a.Hkv) * D);
-  };
-  uint4 next = first < last ? Load8(source(first) + 8 * li) : make_uint4(0u, 0u, 0u, 0u);
-  const int slot = a.row_slot != nullptr ? a.row_slot[t] : 0;
-  int blk = -1;
-  if (pos >= 0 && slot >= 0 && slot < a.slots) {
-    kv4::Table table = a.table;
-    table.entries += static_cast<size_t>(slot) * table.length;
-    blk = table.BlockAt(pos / kv4::kBlock);
-  }
-  const int tok = pos & (kv4::kBlock - 1);
-  for (int i = lane; i < half; i += 32) {
-    const double turns = static_cast<double>(pos) * exp2(a.turn_exponent + i * a.turn_step);
-    float s, c;
-    sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
-    cs[i] = c;
-    cs[half + i] = s;
-  }
-  __syncwarp();
-  // this lane's rotated channels: d < half with the one half further on, or the other way round
-  const int hop = half / 8;                      // lanes
-  const bool shuffle = half % 8 == 0 && (hop & (hop - 1)) == 0;
-  float fc[8], fs[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int d = 8 * li + i, j = d < half ? d : d - half;
-    fc[i] = d < a.rotary_dim ? cs[j] : 1.f;
-    fs[i] = d < a.rotary_dim ? (d < half ? -cs[half + j] : cs[half + j]) : 0.f;
-  }
-  uint4 norm = make_uint4(0u, 0u, 0u, 0u);       // the weights of the kind at hand
-  int norm_kind = -1;
-
-  for (int step = 0; step < a.steps; ++step) {
-    const int hh = first + step * HPW;
-    const uint4 raw = next;
-    if (step + 1 < a.steps && hh + HPW < last) next = Load8(source(hh + HPW) + 8 * li);
-    if (hh - lane / LPH >= last) break;          // (the warp's heads are done)
-    const int kind = hh >= last ? 3 : (hh < a.Hq ? 0 : (hh < a.Hq + a.Hkv ? 1 : 2));       // 0 = q, 1 = k, 2 = v, 3 = none
-    const int head = kind == 0 ? hh : (kind == 1 ? hh - a.Hq : hh - a.Hq - a.Hkv);
-    float x[8];
-    Unpack8(raw, x);
-    const __nv_bfloat16* nw = kind == 0 ? a.q_norm : (kind == 1 ? a.k_norm : nullptr);
-    if (nw != nullptr && kind != norm_kind) {
-      norm = Load8(nw + 8 * li);
-      norm_kind = kind;
+  tk.rows = cs + a.rotary_dim;
+  if (kind != 2) {
+    for (int i = lane; i < half; i += 32) {
+      const double turns = static_cast<double>(pos) * exp2(a.turn_exponent + i * a.turn_step);
+      float s, c;
+      sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
+      cs[i] = c;
+      cs[half + i] = s;
     }
-    if (a.q_norm != nullptr || a.k_norm != nullptr) {
-      float ss = 0.f;
+    __syncwarp();
+    auto turn = [&](int d, float& c, float& s) {
+      const int j = d < half ? d : d - half;
+      c = d < a.rotary_dim ? cs[j] : 1.f;
+      s = d < a.rotary_dim ? (d < half ? -cs[half + j] : cs[half + j]) : 0.f;
+    };
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
-#pragma unroll
-      for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (nw != nullptr) {
-        const float r = rsqrtf(ss / D + a.eps);
-        float w[8];
-        Unpack8(norm, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * r * (1.0f + w[i]);
-      }
-    }
-    if (half > 0) {
-      float y[8];
-      if (shuffle) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = __shfl_xor_sync(0xffffffffu, x[i], hop);
-      } else {
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) rows[lane * 8 + i] = x[i];
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int d = 8 * li + i;
-          y[i] = d < a.rotary_dim ? rows[(lane - li) * 8 + (d < half ? d + half : d - half)] : 0.f;
-        }
-      }
-      if (kind < 2) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (8 * li + i < a.rotary_dim) x[i] = x[i] * fc[i] + y[i] * fs[i];
-      }
-    }
-    const uint4 packed = make_uint4(PackBf16(x[0], x[1]), PackBf16(x[2], x[3]), PackBf16(x[4], x[5]), PackBf16(x[6], x[7]));
-    if (kind == 0) *reinterpret_cast<uint4*>(a.q_out + (static_cast<size_t>(t) * a.Hq + head) * D + 8 * li) = packed;
-    if (__all_sync(0xffffffffu, kind == 0)) continue;
-    Unpack8(packed, x);
-    bool nan = false;
-    float lo = kv4::kLimit, hi = -kv4::kLimit;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      nan |= x[i] != x[i];
-      x[i] = fminf(fmaxf(x[i], -kv4::kLimit), kv4::kLimit);
-      lo = fminf(lo, x[i]);
-      hi = fmaxf(hi, x[i]);
-    }
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {            // the eight lanes of a group
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    const bool bad = (__ballot_sync(0xffffffffu, nan) >> (lane & ~7) & 0xffu) != 0u;
-    const __nv_bfloat16 sb = __float2bfloat16_rn(bad ? __int_as_float(0x7fc00000) : __fdiv_rn(hi - lo, 15.f));
-    const float s = __bfloat162float(sb);
-    uint32_t codes = 0u;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float n = s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x[i] - lo, s)), 0.f), 15.f) : 0.f;
-      codes |= static_cast<uint32_t>(n) << (4 * i);
-    }
-    if (kind >= 1 && kind <= 2 && blk >= 0) {
-      uint32_t* part = a.cache + ((static_cast<size_t>(blk) * a.Hkv + head) * 2 + (kind - 1)) * (kv4::Shape<D>::kPart / 4);
-      part[kind == 1 ? kv4::Word<D, false>(tok, li) : kv4::Word<D, true>(tok, li)] = codes;
-      if (li % 8 == 0)
-        part[2 * D + tok * kv4::Shape<D>::kGroups + li / 8] =
-            static_cast<uint32_t>(__bfloat16_as_ushort(sb)) | static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(lo))) << 16;
+    for (int i = 0; i < 4; ++i) {
+      turn(8 * li + 2 * i, tk.fc[i].x, tk.fs[i].x);
+      turn(8 * li + 2 * i + 1, tk.fc[i].y, tk.fs[i].y);
     }
   }
+  const int first = part * a.steps * HPW + lane / LPH, rounds = min(a.steps, (kind == 0 ? rounds_q : rounds_kv) - part * a.steps);
+  if (kind == 0) Heads<D, 0>(a, tk, first, rounds);
+  else if (kind == 1) Heads<D, 1>(a, tk, first, rounds);
+  else Heads<D, 2>(a, tk, first, rounds);
 }
 
 // Rows read back: a thread has one word (eight channels) of a row and up to ITEMS of its 2 Hkv heads' keys and values, whose codes and pairs it
@@ -225,10 +304,10 @@ __global__ void __launch_bounds__(256) ReadKv4Kernel(const uint32_t* __restrict_
 template <int D>
 int LaunchPrecore(PrecoreArgs a, cudaStream_t s) {
   // warps for every SM four times over where there are rows enough; up to eight rounds of heads to a warp, which share its angles
-  const int per_round = 256 / D, rounds = (a.Hq + 2 * a.Hkv + per_round - 1) / per_round;
-  const long long most = static_cast<long long>(a.T) * rounds / (4 * 148 * 32);
+  const int per_round = 256 / D, rounds_q = (a.Hq + per_round - 1) / per_round, rounds_kv = (a.Hkv + per_round - 1) / per_round;
+  const long long most = static_cast<long long>(a.T) * (rounds_q + 2 * rounds_kv) / (4 * 148 * 32);
   a.steps = static_cast<int>(most < 1 ? 1 : (most > 8 ? 8 : most));
-  a.groups = (rounds + a.steps - 1) / a.steps;
+  a.groups = (rounds_q + a.steps - 1) / a.steps + 2 * ((rounds_kv + a.steps - 1) / a.steps);
   const long long tasks = static_cast<long long>(a.T) * a.groups;
   if (tasks > 0x7fffffffll - 8) return R4DXB_TOO_LARGE;
   const size_t smem = 8 * (a.rotary_dim + 32 * 8) * sizeof(float);
