@@ -109,12 +109,17 @@ __device__ __forceinline__ void OrRemote(uint32_t addr, uint32_t bits) {
 // 1024 (or, where they lie four bits higher, as 1024 + 16 n), come back out exactly, and one fma rounds to fp16.
 __device__ __forceinline__ __half2 AsHalf2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
 __device__ __forceinline__ uint32_t Bits(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
+__device__ __forceinline__ uint32_t AndOr(uint32_t a, uint32_t b, uint32_t c) {        // (one instruction: two where the compiler folds constants)
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
 __device__ __forceinline__ void Kv4ToHalf(uint32_t w, __half2 s, __half2 lo, uint32_t (&h)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; i += 2) {
     const uint32_t x = w >> (4 * i);
-    const __half2 n0 = __hsub2(AsHalf2((x & 0x000f000fu) | 0x64006400u), AsHalf2(0x64006400u));
-    const __half2 n1 = __hfma2(AsHalf2((x & 0x00f000f0u) | 0x64006400u), AsHalf2(0x2c002c00u), AsHalf2(0xd400d400u));     // / 16 - 64
+    const __half2 n0 = __hsub2(AsHalf2(AndOr(x, 0x000f000fu, 0x64006400u)), AsHalf2(0x64006400u));
+    const __half2 n1 = __hfma2(AsHalf2(AndOr(x, 0x00f000f0u, 0x64006400u)), AsHalf2(0x2c002c00u), AsHalf2(0xd400d400u));     // / 16 - 64
     h[i] = Bits(__hfma2(n0, s, lo));
     h[i + 1] = Bits(__hfma2(n1, s, lo));
   }
@@ -201,11 +206,14 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
     uint4 kraw[KI];
     uint32_t vraw[8][VW];
     // 4-bit cache.  K: a thread owns the words of channels 8 kc .. of every 32 of one key (the keys of eight lanes are 4 apart, for the
-    // banks of its stores).  V: word vw (of this CTA's half) of VT tokens, turned into eight rows of VT fp16 values; the row that it
-    // starts with depends on its word.
+    // banks of its stores).  V: word vword (of this CTA's half) of VT consecutive tokens, turned into eight rows of VT fp16 values; the
+    // lanes of a store have the tokens of half a tile (all banks), the words of a warp lie in the same 32 bytes of the cache.
     constexpr int NJ = D / 32, NG = kv4::Shape<D>::kGroups, VT = D / 32, VWords = D / 16;
     const int kc = tid & 3, kkey = (tid >> 5) * 8 + ((tid >> 3) & 3) + (tid & 4);
-    const int vword = tid % VWords, vtok = tid / VWords * VT, vgroup = (rank * VWords + vword) >> 3;
+    constexpr int VUnits = kHalfTile / VT;       // groups of tokens in half a tile: 8, 16 or 32 lanes
+    const int vsub = lane / VUnits;         // warps 0 .. 3: the first half of the tile
+    const int vword = D == 256 ? (cw & 3) * 2 + (vsub & 1) + (vsub >> 1) * 8 : (cw & 3) * (VWords / 4) + vsub;
+    const int vtok = (cw >> 2) * kHalfTile + lane % VUnits * VT, vgroup = (rank * VWords + vword) >> 3;
     uint32_t kcodes[NJ], kpairs[NG], vcodes[VT], vpairs[VT];
     const uint32_t* cache4 = reinterpret_cast<const uint32_t*>(a.cache) + static_cast<size_t>(hkv) * (kv4::Shape<D>::kRun / 4);
     const size_t page_words = static_cast<size_t>(a.Hkv) * (kv4::Shape<D>::kRun / 4);
@@ -357,27 +365,23 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
           asm volatile("fence.acq_rel.cluster;" ::: "memory");
         }
         __half2 s2[VT / 2], lo2[VT / 2];
-        uint32_t lo_codes[VT / 2], hi_codes[VT / 2];          // channels 0 .. 3 and 4 .. 7 of two tokens
 #pragma unroll
         for (int t = 0; t < VT / 2; ++t) {
           s2[t] = __floats2half2_rn(BfLo(vpairs[2 * t]), BfLo(vpairs[2 * t + 1]));
           lo2[t] = __floats2half2_rn(BfHi(vpairs[2 * t]), BfHi(vpairs[2 * t + 1]));
-          lo_codes[t] = __byte_perm(vcodes[2 * t], vcodes[2 * t + 1], 0x5410);
-          hi_codes[t] = __byte_perm(vcodes[2 * t], vcodes[2 * t + 1], 0x7632);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int d = (i + vword) & 7;
-          uint32_t h[VT / 2];
+        for (int q = 0; q < 2; ++q) {            // channels 0 .. 3 and 4 .. 7: a half of each token's word
+          uint32_t h[VT / 2][4];
 #pragma unroll
-          for (int t = 0; t < VT / 2; ++t) {
-            const uint32_t x = (d & 4 ? hi_codes[t] : lo_codes[t]) >> (4 * (d & 3));
-            h[t] = Bits(__hfma2(__hsub2(AsHalf2((x & 0x000f000fu) | 0x64006400u), AsHalf2(0x64006400u)), s2[t], lo2[t]));
+          for (int t = 0; t < VT / 2; ++t) Kv4ToHalf(__byte_perm(vcodes[2 * t], vcodes[2 * t + 1], q == 0 ? 0x5410 : 0x7632), s2[t], lo2[t], h[t]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            unsigned char* dst = at + Sw128(vword * 8 + 4 * q + i, (vtok >> 3) & 7) + (vtok & 7) * 2;
+            if constexpr (VT == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(h[0][i], h[1][i], h[2][i], h[3][i]);
+            else if constexpr (VT == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(h[0][i], h[1][i]);
+            else *reinterpret_cast<uint32_t*>(dst) = h[0][i];
           }
-          unsigned char* dst = at + Sw128(vword * 8 + d, (vtok >> 3) & 7) + (vtok & 7) * 2;
-          if constexpr (VT == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
-          else if constexpr (VT == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(h[0], h[1]);
-          else *reinterpret_cast<uint32_t*>(dst) = h[0];
         }
         ptx::FenceProxyAsyncShared();
         __syncwarp();
