@@ -12,6 +12,9 @@ def add_model_flags(ap: argparse.ArgumentParser) -> None:
     g.add_argument("--layout", default="trellis", choices=["bf16", "w4a16", "trellis", "w8a16"])
     g.add_argument("--tokenizer-dir", default=None)
     g.add_argument("--max-ctx", type=int, default=8192)
+    g.add_argument("--kv-cache", default="fp8", choices=["fp8", "int4"],
+                   help="format of the paged KV cache: e4m3 with a descale per head, or 4-bit codes with a scale and low end per 64 "
+                        "channels (9/16 of the bytes; head dimensions 64, 128 and 256; not qwen4_exp)")
     g.add_argument("--layers", type=int, default=0, help="load only the first N layers (debug)")
     g.add_argument("--prefill-chunk", type=int, default=int(os.environ.get("R4DXB_PREFILL_CHUNK", "0")),
                    help="rows per prefill chunk (0: chosen from the prompt length)")

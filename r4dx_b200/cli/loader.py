@@ -9,6 +9,10 @@ import torch
 from ..config import ModelConfig, qwen_hybrid_27b_config, small_hybrid_config, tiny_hybrid_config
 
 
+def _kv_cache(args) -> str:
+    return getattr(args, "kv_cache", "fp8")
+
+
 def load_text_model(args, device: Optional[str] = None):
     """Returns (TextModel, tokenizer, chat_template)."""
     from ..models.hybrid import HybridModel
@@ -71,7 +75,7 @@ def load_text_model(args, device: Optional[str] = None):
         from ..parallel.tp_comm import make_comm, spin_limit_for_ms
         comm = make_comm(args.tp, rank, device, mode=args.tp_mode, hidden=gcfg.hidden_size,
                          spin_limit=spin_limit_for_ms(getattr(args, "tp_ar_timeout_ms", 500)))
-    model = HybridModel(cfg, weights, max_ctx=args.max_ctx, device=device, comm=comm)
+    model = HybridModel(cfg, weights, max_ctx=args.max_ctx, device=device, comm=comm, kv_cache=_kv_cache(args))
     drafter = None
     if args.mtp > 0 and any(k.startswith("mtp.") for k in weights):
         from ..models.mtp import MtpDrafter
@@ -107,7 +111,7 @@ def _load_qwen4_exp(args, gcfg, weights, model_arg: str, model_id: str, device):
     from ..runtime.tokenizer import load_tokenizer
     bad = [f for f, on in (("--tp", args.tp > 1), ("--pp", getattr(args, "pp", 1) > 1), ("--ep", getattr(args, "ep", 1) > 1),
                            ("--mtp", getattr(args, "mtp", 0) > 0), ("--dflash", bool(getattr(args, "dflash", None))),
-                           ("--ngram", getattr(args, "ngram", 0) > 0), ("--vision on", getattr(args, "vision", "off") == "on")) if on]
+                           ("--ngram", getattr(args, "ngram", 0) > 0), ("--kv-cache int4", _kv_cache(args) != "fp8"), ("--vision on", getattr(args, "vision", "off") == "on")) if on]
     if bad:
         raise SystemExit("qwen4_exp does not support: " + ", ".join(bad))
     table = None
@@ -169,7 +173,7 @@ def _load_pipeline(args, gcfg, cfg, weights, full, model_id, device, rank, world
     # the pipeline stages keep state for prompts only: with --hybrid-ctx they hold fewer positions than the decode model, and
     # longer prompts take the tensor-parallel prefill (reference: docs/usage.md "--hybrid-ctx N": the stage-KV capacity)
     stage_ctx = min(args.max_ctx, getattr(args, "hybrid_ctx", 0) or args.max_ctx) if hybrid else args.max_ctx
-    stage = HybridModel(gcfg, stage_w, max_ctx=stage_ctx, device=device, layer_range=rng)
+    stage = HybridModel(gcfg, stage_w, max_ctx=stage_ctx, device=device, layer_range=rng, kv_cache=_kv_cache(args))
     chunk = getattr(args, "prefill_chunk", 0) or 1024
     tk, tpl = load_tokenizer(args.tokenizer_dir, gcfg.vocab_size)
     if not hybrid:
@@ -178,7 +182,7 @@ def _load_pipeline(args, gcfg, cfg, weights, full, model_id, device, rank, world
     from ..parallel.tp_comm import make_comm, spin_limit_for_ms
     comm = make_comm(args.tp, rank, device, mode=args.tp_mode, hidden=gcfg.hidden_size,
                      spin_limit=spin_limit_for_ms(getattr(args, "tp_ar_timeout_ms", 500)))
-    tp_model = HybridModel(cfg, weights, max_ctx=args.max_ctx, device=device, comm=comm)
+    tp_model = HybridModel(cfg, weights, max_ctx=args.max_ctx, device=device, comm=comm, kv_cache=_kv_cache(args))
     local = HybridPpTextModel(tp_model, stage, rank, world, split, gcfg, model_id=model_id, chunk=chunk,
                               min_rows=getattr(args, "pp_min_rows", 512), prefill_chunk=getattr(args, "prefill_chunk", 0))
     return _facade(local, rank, world, args, comm=comm), tk, tpl
@@ -199,7 +203,7 @@ def _load_expert_parallel(args, gcfg, weights, model_id, device, rank, world):
         raise SystemExit(f"--ep {world} must divide the {gcfg.num_experts} experts")
     from ..models.hybrid import MAX_ROWS
     comm = EpComm(world, rank, device, gcfg, max_rows=MAX_ROWS, spin_limit=spin_limit_for_ms(getattr(args, "tp_ar_timeout_ms", 500)))
-    model = HybridModel(gcfg, weights, max_ctx=args.max_ctx, device=device, comm=comm)
+    model = HybridModel(gcfg, weights, max_ctx=args.max_ctx, device=device, comm=comm, kv_cache=_kv_cache(args))
     tk, tpl = load_tokenizer(args.tokenizer_dir, gcfg.vocab_size)
     local = LocalTextModel(model, model_id=model_id, global_config=gcfg, prefill_chunk=getattr(args, "prefill_chunk", 0))
     return _facade(local, rank, world, args), tk, tpl

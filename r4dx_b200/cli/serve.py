@@ -24,7 +24,8 @@ def main(argv=None) -> int:
         from ..models.batch import BatchModel
         from ..server.batch_executor import BatchEngine
         m = tm.m
-        bm = BatchModel(m.cfg, m.w, slots=args.batch, slot_ctx=args.batch_ctx, device=str(m.device), comm=m.comm)
+        bm = BatchModel(m.cfg, m.w, slots=args.batch, slot_ctx=args.batch_ctx, device=str(m.device), comm=m.comm,
+                        kv_cache=m.kv_cache)
         eng = BatchEngine(bm, tk, max_queue=max(args.max_queue, 2 * args.batch),
                           request_log=RequestLog(args.request_log, args.request_log_tokens))
     else:

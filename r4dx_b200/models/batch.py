@@ -55,10 +55,10 @@ class PagedKvAllocator:
 
 class BatchModel:
     def __init__(self, cfg: ModelConfig, weights: Dict[str, object], slots: int, slot_ctx: int, device: str = "cuda",
-                 comm=None, pool_blocks: Optional[int] = None):
+                 comm=None, pool_blocks: Optional[int] = None, kv_cache: str = "fp8"):
         self.cfg, self.slots, self.device = cfg, slots, torch.device(device)
         self.slot_ctx = ((slot_ctx + KV_BLOCK - 1) // KV_BLOCK) * KV_BLOCK
-        self.base = HybridModel(cfg, weights, max_ctx=self.slot_ctx, device=device, comm=comm)
+        self.base = HybridModel(cfg, weights, max_ctx=self.slot_ctx, device=device, comm=comm, kv_cache=kv_cache)
         b = self.base
         nblk = self.slot_ctx // KV_BLOCK
         self.alloc = PagedKvAllocator(pool_blocks or slots * nblk, slots, nblk + 1, self.device)
@@ -66,7 +66,7 @@ class BatchModel:
         Hv, Dg = cfg.linear_num_value_heads, cfg.linear_key_head_dim
         z = lambda *s, dtype=torch.float32: torch.zeros(*s, dtype=dtype, device=self.device)
         pool = (pool_blocks or slots * nblk) + 1
-        self.kv = {i: z(pool, Hkv, 2, KV_BLOCK, D, dtype=torch.uint8) for i in b.kv}
+        self.kv = {i: b.new_pool(pool) for i in b.kv}
         self.gdn_state = {i: z(slots, Hv, Dg, Dg) for i in b.gdn_state}
         self.ring = {i: z(slots, CONV_RING, cfg.conv_dim, dtype=BF) for i in b.ring}
         self.log_u = {i: z(slots, MAX_ROWS, Hv, Dg) for i in b.gdn_state}
@@ -126,6 +126,36 @@ class BatchModel:
         self.alloc.release(slot)
         self.active[slot] = False
 
+    def _attn_fp8(self, i: int, qg, kk, vv, q, core, B: int, positions, row_slot, splits: int, part_acc, part_ml) -> None:
+        """One layer's cache write and attention of B rows over the fp8 cache."""
+        from .. import native
+        L = self._L = self._L or native.cuda()
+        cfg, w, pa = self.cfg, self.base.w, f"text.layers.{i}.attn."
+        Hq, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
+        qn, kn = w.get(pa + "q_norm"), w.get(pa + "k_norm")
+        st = torch.cuda.current_stream().cuda_stream
+        rc = L.r4dxb_attn_precore_batch(qg.data_ptr(), kk.data_ptr(), vv.data_ptr(), qn.data_ptr() if qn is not None else None,
+                                        kn.data_ptr() if kn is not None else None, w[pa + "k_descale"].data_ptr(), w[pa + "v_descale"].data_ptr(),
+                                        positions.data_ptr(), self.alloc.tables.data_ptr(), row_slot.data_ptr(),
+                                        self.alloc.tables.shape[1], q.data_ptr(), self.kv[i].data_ptr(), B, Hq, Hkv, D,
+                                        cfg.rotary_dim, cfg.rope_theta, cfg.rms_norm_eps, cfg.q_proj_dim // Hq, st)
+        assert rc == 0, rc
+        rc = L.r4dxb_attn_decode_batch(q.data_ptr(), qg.data_ptr(), self.kv[i].data_ptr(), self.alloc.tables.data_ptr(),
+                                       row_slot.data_ptr(), self.alloc.tables.shape[1], positions.data_ptr(),
+                                       w[pa + "k_descale"].data_ptr(), w[pa + "v_descale"].data_ptr(), part_acc.data_ptr(),
+                                       part_ml.data_ptr(), core.data_ptr(), B, Hq, Hkv, D, splits,
+                                       1 if cfg.attn_output_gate else 0, st)
+        assert rc == 0, rc
+
+    def _attn_int4(self, i: int, qg, kk, vv, q, core, B: int, positions, row_slot) -> None:
+        """The same over the 4-bit cache."""
+        cfg, w, pa = self.cfg, self.base.w, f"text.layers.{i}.attn."
+        Hq, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
+        K.attn_precore_kv4(qg, kk, vv, w.get(pa + "q_norm"), w.get(pa + "k_norm"), positions, self.alloc.tables, q, self.kv[i], B, Hq, Hkv, D,
+                           cfg.rotary_dim, cfg.layer_theta(i), cfg.rms_norm_eps, q_stride=cfg.q_proj_dim // Hq, row_slot=row_slot)
+        K.attn_decode_kv4(q, qg, self.kv[i], self.alloc.tables, positions, core, B, Hq, Hkv, D, cfg.attn_output_gate, cfg.layer_window(i),
+                          row_slot=row_slot)
+
     # ---- one token for B slots ---------------------------------------------------------------------------
     def decode_batch(self, slots: Sequence[int], tokens: Sequence[int]) -> List[int]:
         from .. import native
@@ -145,8 +175,9 @@ class BatchModel:
         Hv, Hk, Dg = cfg.linear_num_value_heads, cfg.linear_num_key_heads, cfg.linear_key_head_dim
         G = Hq // max(1, Hkv)
         splits = max(1, min(16, 592 // max(1, Hkv * B)))        # about four CTAs per SM
-        part_acc = torch.empty(B * splits * Hkv * G * D, dtype=torch.float32, device=dev)
-        part_ml = torch.empty(B * splits * Hkv * G * 2, dtype=torch.float32, device=dev)
+        fp8 = b.kv_cache == "fp8"
+        part_acc = torch.empty(B * splits * Hkv * G * D, dtype=torch.float32, device=dev) if fp8 else None
+        part_ml = torch.empty(B * splits * Hkv * G * 2, dtype=torch.float32, device=dev) if fp8 else None
 
         def lin(name, inp, out, residual=None, fused=False):
             l = b.lin[name]
@@ -162,20 +193,11 @@ class BatchModel:
                 pa = p + "attn."
                 qg, kk, vv, q = cb["qg"][:B], cb["k"][:B], cb["v"][:B], cb["q"][:B]
                 lin(pa + "qg", h, qg); lin(pa + "k", h, kk); lin(pa + "v", h, vv)
-                qn, kn = w.get(pa + "q_norm"), w.get(pa + "k_norm")
-                rc = L.r4dxb_attn_precore_batch(qg.data_ptr(), kk.data_ptr(), vv.data_ptr(), qn.data_ptr() if qn is not None else None,
-                                                kn.data_ptr() if kn is not None else None, w[pa + "k_descale"].data_ptr(), w[pa + "v_descale"].data_ptr(),
-                                                positions.data_ptr(), self.alloc.tables.data_ptr(), row_slot.data_ptr(),
-                                                self.alloc.tables.shape[1], q.data_ptr(), self.kv[i].data_ptr(), B, Hq, Hkv, D,
-                                                cfg.rotary_dim, cfg.rope_theta, cfg.rms_norm_eps, cfg.q_proj_dim // Hq, st)
-                assert rc == 0, rc
                 core = cb["core"][:B * cfg.q_dim].view(B, cfg.q_dim)
-                rc = L.r4dxb_attn_decode_batch(q.data_ptr(), qg.data_ptr(), self.kv[i].data_ptr(), self.alloc.tables.data_ptr(),
-                                               row_slot.data_ptr(), self.alloc.tables.shape[1], positions.data_ptr(),
-                                               w[pa + "k_descale"].data_ptr(), w[pa + "v_descale"].data_ptr(), part_acc.data_ptr(),
-                                               part_ml.data_ptr(), core.data_ptr(), B, Hq, Hkv, D, splits,
-                                               1 if cfg.attn_output_gate else 0, st)
-                assert rc == 0, rc
+                if b.kv_cache == "int4":
+                    self._attn_int4(i, qg, kk, vv, q, core, B, positions, row_slot)
+                else:
+                    self._attn_fp8(i, qg, kk, vv, q, core, B, positions, row_slot, splits, part_acc, part_ml)
                 lin(pa + "o", core, x, residual=x)
             else:
                 pg = p + "gdn."

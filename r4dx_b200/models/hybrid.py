@@ -1,6 +1,6 @@
 """GPU model graph of the Qwen-style hybrid decoder (dense), single rank or one TP rank.
 
-PyTorch is the framework layer here: module wiring, state allocation (paged fp8 KV, GDN state,
+PyTorch is the framework layer here: module wiring, state allocation (paged fp8 or 4-bit KV, GDN state,
 conv ring), workspaces and CUDA-graph capture.  Every op on the token path is a kernel of
 ``libr4dxb_cuda.so``.  The forward follows the reference's chunk pipeline -- prologue (ids ->
 embedding), layer range, epilogue (final norm, LM head, argmax)
@@ -19,6 +19,7 @@ import torch
 
 from ..config import ModelConfig
 from ..ops import kernels as K
+from ..quant.kv4 import HEAD_DIMS
 from ..quant.trellis import TrellisWeight
 from ..quant.w4a16 import W4Weight, W8Weight
 
@@ -150,10 +151,16 @@ class StepBuffers:
 
 class HybridModel:
     def __init__(self, cfg: ModelConfig, weights: Dict[str, object], max_ctx: int = 8192 + 1024,
-                 device: str = "cuda", attn_splits: Optional[int] = None, comm=None, layer_range=None):
+                 device: str = "cuda", attn_splits: Optional[int] = None, comm=None, layer_range=None, kv_cache: str = "fp8"):
         """``layer_range`` = (first, end): a pipeline stage that runs only those layers (embedding with the
-        first stage, head with the last)."""
+        first stage, head with the last).  ``kv_cache``: "fp8" (e4m3, a static descale per head) or "int4" (4-bit codes with a
+        bf16 scale and low end per 64 channels, quant/kv4.py: 9/16 of the bytes, no descales)."""
         cfg.validate() if cfg.tp_world == 1 else None
+        if kv_cache not in ("fp8", "int4"):
+            raise ValueError(f"kv_cache {kv_cache!r}: fp8 or int4")
+        if kv_cache == "int4" and cfg.head_dim not in HEAD_DIMS:
+            raise ValueError(f"the 4-bit KV cache has head dimensions {HEAD_DIMS}, not {cfg.head_dim}")
+        self.kv_cache = kv_cache
         if cfg.has_conv_layers and comm is not None and comm.world > 1 and os.environ.get("R4DXB_UNVALIDATED_TP") != "1":
             # the sharding of this family is checked on the CPU (shards add up to the unsharded block); its only two-GPU run
             # did not finish within its time limit and the cause has not been found, so the path stays closed by default
@@ -210,7 +217,7 @@ class HybridModel:
         self.log_eg: Dict[int, torch.Tensor] = {}
         for i in range(self.layer_begin, self.layer_end):
             if cfg.is_attention_layer(i):
-                self.kv[i] = torch.zeros(nblk, Hkv, 2, KV_BLOCK, D, dtype=torch.uint8, device=dev)
+                self.kv[i] = self.new_pool(nblk)
             elif cfg.is_conv_layer(i):
                 self.ring[i] = torch.zeros(32, cfg.conv_channels, dtype=BF, device=dev)   # B * x rows keyed by position & 31
             else:
@@ -237,6 +244,53 @@ class HybridModel:
             logits=e(R, V, dtype=torch.float32), argmax_scratch=e(2 * R * 256, dtype=torch.float32),
             part_acc=e(attn_splits * Hkv * G * D, dtype=torch.float32),
             part_ml=e(attn_splits * Hkv * G * 2, dtype=torch.float32))
+        if self.kv_cache == "int4":
+            # splits by row count, and a scratch for the largest call
+            self.kv4_splits = {T: K.kv4_splits(T * (Hq // max(1, Hkv)), max(1, Hkv), 1, nblk, D) for T in range(1, R + 1)}
+            self.kv4_scratch = e(max(1, *(K.kv4_scratch_floats(T, 1, Hq, D, s) for T, s in self.kv4_splits.items())), dtype=torch.float32)
+
+    def new_pool(self, blocks: int) -> torch.Tensor:
+        """An empty pool of KV blocks of one layer."""
+        Hkv, D = self.cfg.num_key_value_heads, self.cfg.head_dim
+        if self.kv_cache == "int4":
+            return K.kv4_cache(blocks, Hkv, D, self.device)
+        return torch.zeros(blocks, Hkv, 2, KV_BLOCK, D, dtype=torch.uint8, device=self.device)
+
+    # ---- attention over the cache (either format) --------------------------------------------------
+    def _attn_write(self, i: int, qg, k, v, positions, q, T: int) -> None:
+        """Norms and rope of the rows' queries and keys; keys and values enter layer i's cache."""
+        cfg, w, p = self.cfg, self.w, f"text.layers.{i}.attn."
+        Hq, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
+        if self.kv_cache == "int4":
+            K.attn_precore_kv4(qg, k, v, w.get(p + "q_norm"), w.get(p + "k_norm"), positions, self.block_table, q, self.kv[i], T, Hq, Hkv, D,
+                               cfg.rotary_dim, cfg.layer_theta(i), cfg.rms_norm_eps, q_stride=cfg.q_proj_dim // Hq)
+        else:
+            K.attn_precore(qg, k, v, w.get(p + "q_norm"), w.get(p + "k_norm"), w[p + "k_descale"], w[p + "v_descale"], positions,
+                           self.block_table, q, self.kv[i], T, Hq, Hkv, D, cfg.rotary_dim, cfg.layer_theta(i), cfg.rms_norm_eps,
+                           q_stride=cfg.q_proj_dim // Hq)
+
+    def _attn_rows(self, i: int, T: int, core: torch.Tensor) -> None:
+        """Attention of the T staged rows."""
+        cfg, b, w, p = self.cfg, self.buf, self.w, f"text.layers.{i}.attn."
+        Hq, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
+        if self.kv_cache == "int4":
+            K.attn_decode_kv4(b.q, b.qg, self.kv[i], self.block_table, b.positions, core, T, Hq, Hkv, D, cfg.attn_output_gate,
+                              cfg.layer_window(i), splits=self.kv4_splits[T], scratch=self.kv4_scratch)
+        else:
+            K.attn_decode(b.q, b.qg, self.kv[i], self.block_table, b.positions, w[p + "k_descale"], w[p + "v_descale"],
+                          b.part_acc, b.part_ml, core, T, Hq, Hkv, D, self.attn_splits, cfg.attn_output_gate,
+                          window=cfg.layer_window(i))
+
+    def _attn_chunk(self, i: int, q, qg, core, T: int, pos0: int) -> None:
+        """Attention of a prompt chunk's T rows at positions pos0 .."""
+        cfg, w, p = self.cfg, self.w, f"text.layers.{i}.attn."
+        Hq, Hkv, D, win = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, cfg.layer_window(i)
+        limit = self._key_limit if win > 0 else None
+        if self.kv_cache == "int4":
+            K.attn_prefill_kv4(q, qg, self.kv[i], self.block_table, core, T, Hq, Hkv, D, pos0, cfg.attn_output_gate, win, limit)
+        else:
+            K.attn_prefill(q, qg, self.kv[i], self.block_table, w[p + "k_descale"], w[p + "v_descale"], core, T, Hq, Hkv, D, pos0,
+                           cfg.attn_output_gate, window=win, key_limit=limit)
 
     def state_bytes(self) -> int:
         n = 0
@@ -337,7 +391,6 @@ class HybridModel:
     def _attn_layer(self, i: int, T: int) -> None:
         cfg, b, w = self.cfg, self.buf, self.w
         p = f"text.layers.{i}.attn."
-        Hq, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         x, nw, eps = b.x[:T], w[f"text.layers.{i}.input_layernorm"], cfg.rms_norm_eps
         grp = self._siblings((p + "qg", p + "k", p + "v"))
         if grp is not None:
@@ -349,13 +402,9 @@ class HybridModel:
                 self.lin[p + "k"](x, out=b.k[:T], prologue=K.PRO_RMSNORM, norm_w=nw, eps=eps)
                 self.lin[p + "v"](x, out=b.v[:T], prologue=K.PRO_RMSNORM, norm_w=nw, eps=eps)
             self._join(side)
-        K.attn_precore(b.qg, b.k, b.v, w.get(p + "q_norm"), w.get(p + "k_norm"), w[p + "k_descale"], w[p + "v_descale"],
-                       b.positions, self.block_table, b.q, self.kv[i], T, Hq, Hkv, D, cfg.rotary_dim,
-                       cfg.layer_theta(i), cfg.rms_norm_eps, q_stride=cfg.q_proj_dim // Hq)
+        self._attn_write(i, b.qg, b.k, b.v, b.positions, b.q, T)
         core = b.core.view(-1)[:T * cfg.q_dim].view(T, cfg.q_dim)
-        K.attn_decode(b.q, b.qg, self.kv[i], self.block_table, b.positions, w[p + "k_descale"], w[p + "v_descale"],
-                      b.part_acc, b.part_ml, core, T, Hq, Hkv, D, self.attn_splits, cfg.attn_output_gate,
-                      window=cfg.layer_window(i))
+        self._attn_rows(i, T, core)
         self._row_parallel(self.lin[p + "o"], core, T, post_norm=w.get(f"text.layers.{i}.post_attn_out_norm"))
 
     def _mlp(self, i: int, T: int) -> None:
@@ -423,7 +472,11 @@ class HybridModel:
         for i, t in self.gdn_state.items():
             d[f"gdn.{i}"] = float(t.double().sum())
             d[f"ring.{i}"] = float(self.ring[i].double().sum())
-        if blocks:
+        if blocks and self.kv_cache == "int4":         # what the written rows stand for
+            rows = torch.arange(self.pos, dtype=torch.int32, device=self.device)
+            for i, kv in self.kv.items():
+                d[f"kv.{i}"] = float(sum(x.double().sum() for x in K.kv4_read(kv, self.block_table, rows)))
+        elif blocks:
             tab = self.block_table[:blocks].long()
             live = (torch.arange(blocks * KV_BLOCK, device=self.device) < self.pos).view(blocks, 1, 1, KV_BLOCK, 1)
             for i, kv in self.kv.items():          # only rows below the position count: later rows of the last block are stale
@@ -589,7 +642,6 @@ class HybridModel:
         """Runs T (> MAX_ROWS) rows staged in the chunk buffers at positions self.pos .. ; commits them."""
         cfg, w, cb = self.cfg, self.w, self._cb
         H = cfg.hidden_size
-        Hq, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         Hv, Hk, Dg = cfg.linear_num_value_heads, cfg.linear_num_key_heads, cfg.linear_key_head_dim
         x, h = cb["x"][:T], cb["h"][:T]
         pos0 = self.pos
@@ -608,14 +660,9 @@ class HybridModel:
                 self.lin[pa + "qg"].chunk(h, cb["xh"], qg)
                 self.lin[pa + "k"].chunk(h, cb["xh"], kk)
                 self.lin[pa + "v"].chunk(h, cb["xh"], vv)
-                K.attn_precore(qg, kk, vv, w.get(pa + "q_norm"), w.get(pa + "k_norm"), w[pa + "k_descale"], w[pa + "v_descale"],
-                               cb["positions"], self.block_table, q, self.kv[i], T, Hq, Hkv, D, cfg.rotary_dim,
-                               cfg.layer_theta(i), cfg.rms_norm_eps, q_stride=cfg.q_proj_dim // Hq)
+                self._attn_write(i, qg, kk, vv, cb["positions"], q, T)
                 core = cb["core"][:T * cfg.q_dim].view(T, cfg.q_dim)
-                win = cfg.layer_window(i)
-                K.attn_prefill(q, qg, self.kv[i], self.block_table, w[pa + "k_descale"], w[pa + "v_descale"], core, T,
-                               Hq, Hkv, D, pos0, cfg.attn_output_gate, window=win,
-                               key_limit=self._key_limit if win > 0 else None)
+                self._attn_chunk(i, q, qg, core, T, pos0)
                 self._row_parallel_chunk(self.lin[pa + "o"], core, x, cb, post_norm=w.get(p + "post_attn_out_norm"))
             elif cfg.is_conv_layer(i):
                 pc = p + "conv."

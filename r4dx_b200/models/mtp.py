@@ -53,7 +53,8 @@ class MtpDrafter:
             if k.startswith("mtp.") and not k.startswith("mtp.draft_head.") and \
                     k not in ("mtp.fc", "mtp.norm", "mtp.pre_fc_norm_embedding", "mtp.pre_fc_norm_hidden"):
                 w["text.layers.0." + k[4:]] = v
-        self.head = HybridModel(mtp_config(cfg, vocab), w, max_ctx=main.max_ctx, device=str(main.device), comm=main.comm)
+        self.head = HybridModel(mtp_config(cfg, vocab), w, max_ctx=main.max_ctx, device=str(main.device), comm=main.comm,
+                                kv_cache=main.kv_cache)
         self.fc = Linear(weights["mtp.fc"], "mtp.fc")
         self.norm_e, self.norm_h = weights["mtp.pre_fc_norm_embedding"], weights["mtp.pre_fc_norm_hidden"]
         H = cfg.hidden_size

@@ -20,6 +20,7 @@ import torch
 
 from ..config import ModelConfig
 from ..ops import reference as R
+from ..quant import kv4
 
 
 def linear_names(cfg: ModelConfig) -> List[str]:
@@ -135,11 +136,12 @@ class OracleState:
 
 
 class OracleModel:
-    """fp32 forward over explicit state. ``fp8_kv=True`` rounds K/V through e4m3 like the cache."""
+    """fp32 forward over explicit state. ``fp8_kv=True`` rounds K/V through e4m3 like the cache, ``int4_kv=True`` through the 4-bit one."""
 
     def __init__(self, cfg: ModelConfig, weights: Dict[str, torch.Tensor], fp8_kv: bool = False,
-                 chunked_gdn: bool = False, act_dtype: Optional[torch.dtype] = None):
+                 chunked_gdn: bool = False, act_dtype: Optional[torch.dtype] = None, int4_kv: bool = False):
         cfg.validate()
+        self.int4_kv = int4_kv
         self.cfg = cfg
         self.w = {k: v.float() for k, v in weights.items()}
         self.fp8_kv = fp8_kv
@@ -184,6 +186,8 @@ class OracleModel:
         if self.fp8_kv:
             k = R.fp8_e4m3_roundtrip(k, w[p + "attn.k_descale"][None, :, None])
             v = R.fp8_e4m3_roundtrip(v, w[p + "attn.v_descale"][None, :, None])
+        if self.int4_kv:
+            k, v = kv4.round_trip(k.to(torch.bfloat16)), kv4.round_trip(v.to(torch.bfloat16))
         K = torch.cat([st.k[li], k], 0) if li in st.k else k
         V = torch.cat([st.v[li], v], 0) if li in st.v else v
         if store:

@@ -17,7 +17,7 @@ from ..ops import kernels as K
 _GEMM = {"trellis_gemv", "trellis_gemm", "w4a16_gemv", "bf16_gemv", "bf16_gemv_norm", "trellis_input"}
 _OPS = ["embed_gather", "rmsnorm", "add_rmsnorm", "silu_mul", "residual_add", "trellis_gemv", "trellis_gemm", "trellis_input",
         "w4a16_gemv", "bf16_gemv", "bf16_gemv_norm", "argmax_rows", "gdn_decode", "gdn_prefill", "attn_precore", "attn_decode",
-        "attn_prefill", "spec_accept"]
+        "attn_prefill", "attn_precore_kv4", "attn_decode_kv4", "attn_prefill_kv4", "spec_accept"]
 
 
 class SpanAccumulator:

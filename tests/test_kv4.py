@@ -85,3 +85,19 @@ def test_splits_fill_the_chip_once():
                         s = K.kv4_splits(rows, heads, batch, length, D)
                         least = -(-length // 2048)          # 4096 tokens a warp
                         assert least <= s <= max(least, min(148, (length + 7) // 8)) and (s == least or s * heads * batch * -(-rows // most) <= 148)
+
+
+def test_flag_of_the_commands():
+    from r4dx_b200.cli.args import cli_parser, server_parser
+    for parser in (cli_parser(), server_parser()):
+        assert parser.parse_args(["--model", "m"]).kv_cache == "fp8"
+        assert parser.parse_args(["--model", "m", "--kv-cache", "int4"]).kv_cache == "int4"
+        with pytest.raises(SystemExit):
+            parser.parse_args(["--model", "m", "--kv-cache", "int3"])
+
+
+def test_four_stream_family_keeps_its_fp8_cache():
+    from types import SimpleNamespace
+    from r4dx_b200.cli.loader import _load_qwen4_exp
+    with pytest.raises(SystemExit, match="--kv-cache int4"):
+        _load_qwen4_exp(SimpleNamespace(tp=1, kv_cache="int4"), None, {}, "m", "m", "cpu")
