@@ -244,10 +244,9 @@ class HybridModel:
             logits=e(R, V, dtype=torch.float32), argmax_scratch=e(2 * R * 256, dtype=torch.float32),
             part_acc=e(attn_splits * Hkv * G * D, dtype=torch.float32),
             part_ml=e(attn_splits * Hkv * G * 2, dtype=torch.float32))
-        if self.kv_cache == "int4":
-            # splits by row count, and a scratch for the largest call
-            self.kv4_splits = {T: K.kv4_splits(T * (Hq // max(1, Hkv)), max(1, Hkv), 1, nblk, D) for T in range(1, R + 1)}
-            self.kv4_scratch = e(max(1, *(K.kv4_scratch_floats(T, 1, Hq, D, s) for T, s in self.kv4_splits.items())), dtype=torch.float32)
+        self.kv4_scratch = None                  # for the rows of a call, whatever their number
+        if self.kv_cache == "int4" and self.kv:
+            self.kv4_scratch = e(max(1, *(K.kv4_scratch_floats(T, 1, Hq, Hkv, D, nblk) for T in range(1, R + 1))), dtype=torch.float32)
 
     def new_pool(self, blocks: int) -> torch.Tensor:
         """An empty pool of KV blocks of one layer."""
@@ -275,7 +274,7 @@ class HybridModel:
         Hq, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         if self.kv_cache == "int4":
             K.attn_decode_kv4(b.q, b.qg, self.kv[i], self.block_table, b.positions, core, T, Hq, Hkv, D, cfg.attn_output_gate,
-                              cfg.layer_window(i), splits=self.kv4_splits[T], scratch=self.kv4_scratch)
+                              cfg.layer_window(i), scratch=self.kv4_scratch)
         else:
             K.attn_decode(b.q, b.qg, self.kv[i], self.block_table, b.positions, w[p + "k_descale"], w[p + "v_descale"],
                           b.part_acc, b.part_ml, core, T, Hq, Hkv, D, self.attn_splits, cfg.attn_output_gate,

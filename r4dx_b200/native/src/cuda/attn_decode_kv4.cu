@@ -11,7 +11,8 @@
 //   values   O^T[D x 8 rows] += n (p s):  A = codes of token pairs, again as subnormals; B = p s times a power of two that brings the largest
 //            scale met so far to 1 .. 2, rounded to fp16 (2^-11 of 15 steps at most), turned from scores' to operand order with movmatrix.
 //            sum p lo per group in fp32.
-// The warps' results meet in shared memory, the splits' in a second kernel; a sequence short enough for one CTA is finished by it.
+// The warps' results meet in shared memory; the splits' in the shared memory of a cluster of up to 16 CTAs, or, for long tables, in a second
+// kernel.  A sequence short enough for one CTA is finished by it.
 // A row with no visible token (position -1) gives zeros; a block that the table or pool does not have gives NaN to the rows that see it.
 #include <atomic>
 
@@ -21,6 +22,7 @@
 namespace r4dxb {
 namespace {
 
+constexpr int kMaxCluster = 16;
 constexpr float kRescaleStep = 8.f;
 constexpr float kUnit = 1.f / (1 << 28);       // of the scores before the softmax: 2^-4 from q, 2^-24 from the codes
 
@@ -37,6 +39,9 @@ struct DecodeArgs {
   int* status;
   int T, Hq, Hkv, splits, slots, window;
   int warps;                   // of a CTA
+  uint32_t per_token;          // 2^32 / (query heads per kv head), rounded up; 0: one query head
+  // row r of a kv head's G = T Hq / Hkv belongs to token Row(r)
+  __device__ __forceinline__ int Row(int r) const { return per_token != 0u ? static_cast<int>(__umulhi(static_cast<uint32_t>(r), per_token)) : r; }
 };
 
 // Warps of a CTA and blocks in flight per warp, by head dimension and row tiles.
@@ -49,20 +54,24 @@ struct Plan {
   static constexpr int kStride = D + 4;                          // floats between rows of the merge
   static constexpr int kMerge = kWarps * kRows * kStride * 4;
   static constexpr int kQuery = NT * (D / 32) * 512;             // operand B of the scores
-  static constexpr int kBody = kRing > kMerge ? kRing : kMerge;
+  static constexpr int kBase = kWarps * kRows * (D / 64) * 4;    // sum p lo of each warp, row and group
+  static constexpr int kOut = kRows * D * 4;                     // a CTA's rows, for the other CTAs of its cluster
+  static constexpr int kBody = kRing > kMerge + kBase + kOut ? kRing : kMerge + kBase + kOut;
   static constexpr int kSums = NT * (D / 32) * 8 * 4;            // of a row's query over 32 channels
-  static constexpr size_t kSmem = kBody + kQuery + kSums + kWarps * kStages * 8 + kWarps * kRows * 12 + kRows * 8 + 16;
+  static constexpr size_t kSmem = kBody + kQuery + kSums + kWarps * kStages * 8 + kWarps * kRows * 8 + kRows * 20 + 16;
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
 // The blocks that the rows of a call may see and the number of CTAs that share them: a block per warp at least.
 struct Span {
   int first, blocks, active;
+  int position;                // of token `lane`, -1 beyond the last
 };
 __device__ __forceinline__ Span Visible(const int* positions, int T, int window, int splits, int warps) {
   const int lane = threadIdx.x & 31;
   const int p = lane < T ? positions[lane] : -1;
   Span s;
+  s.position = p;
   const int high = __reduce_max_sync(0xffffffffu, p), low = __reduce_min_sync(0xffffffffu, p < 0 ? 0x7fffffff : p);
   s.first = window > 0 && high >= 0 ? max(0, low - window + 1) / kv4::kBlock : 0;
   s.blocks = high >= 0 ? high / kv4::kBlock + 1 - s.first : 0;
@@ -129,7 +138,7 @@ __device__ __forceinline__ void StoreRow(const DecodeArgs& a, size_t row, int D,
   *reinterpret_cast<uint2*>(a.out + row * D + col) = make_uint2(PackBf16(o.x, o.y), PackBf16(o.z, o.w));
 }
 
-template <int D, int NT>
+template <int D, int NT, bool CLUSTER>
 __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(DecodeArgs a) {
   PdlEnter();
   using S = kv4::Shape<D>;
@@ -139,10 +148,9 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
   uint4* query = reinterpret_cast<uint4*>(smem + P::kBody);                     // [row tile][32 channels][lane]
   float* sums = reinterpret_cast<float*>(smem + P::kBody + P::kQuery);          // [row tile][32 channels][row]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + P::kBody + P::kQuery + P::kSums);
-  float2* ml = reinterpret_cast<float2*>(bars + kWarps * kStages);              // [warps][rows]
-  float* weights = reinterpret_cast<float*>(ml + kWarps * kRows);               // [warps][rows]
-  float* row_l = weights + kWarps * kRows;                                      // [rows]
-  int* nan_groups = reinterpret_cast<int*>(row_l + kRows);                      // [rows]: groups in which the row sees a NaN among the values
+  float4* shared_ml = reinterpret_cast<float4*>(bars + kWarps * kStages);       // [rows]: maximum and sum of this CTA
+  float2* ml = reinterpret_cast<float2*>(shared_ml + kRows);                    // [warps][rows]
+  int* nan_groups = reinterpret_cast<int*>(ml + kWarps * kRows);                // [rows]: groups in which the row sees a NaN among the values
   volatile int* abort_flag = nan_groups + kRows;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x, hkv = blockIdx.y % a.Hkv, row0 = blockIdx.y / a.Hkv * kRows, seq = blockIdx.z;
@@ -157,8 +165,15 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
     a.table.entries += static_cast<size_t>(known ? slot : 0) * a.table.length;
   }
   const int gqa = a.Hq / a.Hkv, G = gqa * a.T;
+  // A warp lays out 32 channels of a row tile's queries; the first of its tasks is on its way while positions and table are.
+  auto load_query = [&](int task) {
+    const int r = row0 + task / NJ * 8 + g, t = a.Row(r);
+    return r < G ? *reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(t) * a.Hq + hkv * gqa + r - t * gqa) * D + task % NJ * 32 + 8 * c)
+                 : make_uint4(0u, 0u, 0u, 0u);
+  };
+  uint4 query_next = warp < NT * NJ ? load_query(warp) : make_uint4(0u, 0u, 0u, 0u);
   const Span span = Visible(a.positions, a.T, a.window, a.splits, kWarps);
-  if (split >= span.active) return;
+  if (split >= (CLUSTER && span.active > 1 ? a.splits : span.active)) return;       // (a cluster stays together, its CTAs without blocks merge too)
   const int per = (span.blocks + span.active - 1) / span.active;
   const int b0 = span.first + split * per + warp, b1 = min(span.first + span.blocks, span.first + (split + 1) * per);
   const int steps = b1 > b0 ? (b1 - b0 + kWarps - 1) / kWarps : 0;
@@ -191,16 +206,14 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
   };
   for (int i = 0; i < min(steps, kStages); ++i) issue(i, i);
 
-  // ---- query rows: operand B (row g; channels 32 j + 8 c .. in the order of the codes) and its sums, a warp per 32 channels ----
-  const int my_pos = (lane < a.T) ? a.positions[lane] : -1;
+  // ---- query rows: operand B (row g; channels 32 j + 8 c .. in the order of the codes) and its sums ----
   auto position = [&](int r) {
-    const int p = __shfl_sync(0xffffffffu, my_pos, r < G ? r / gqa : 0);
+    const int p = __shfl_sync(0xffffffffu, span.position, r < G ? a.Row(r) : 0);
     return r < G ? p : -1;
   };
   for (int task = warp; task < NT * NJ; task += kWarps) {
-    const int r = row0 + task / NJ * 8 + g;
-    const uint4 v = r < G ? *reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(r / gqa) * a.Hq + hkv * gqa + r % gqa) * D + task % NJ * 32 + 8 * c)
-                          : make_uint4(0u, 0u, 0u, 0u);
+    const uint4 v = query_next;
+    if (task + kWarps < NT * NJ) query_next = load_query(task + kWarps);
     // channels i and i + 4 for i = 0 .. 3; every second pair meets codes that carry a factor 16
     const float x[8] = {BfLo(v.x), BfHi(v.x), BfLo(v.y), BfHi(v.y), BfLo(v.z), BfHi(v.z), BfLo(v.w), BfHi(v.w)};
     uint32_t b[4];
@@ -293,7 +306,7 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
         // Value pairs that are no numbers, or of tokens that no row here sees (whose bytes may be anything), are zeros from here on: what
         // a row does not see has the weight 0, and 0 x NaN would reach it.  Rows that do see a NaN are noted.
         bool used = false;
-        for (int t = row0 / gqa; t <= (min(G, row0 + kRows) - 1) / gqa; ++t) used |= sees(__shfl_sync(0xffffffffu, my_pos, t), kp0 + lane);
+        for (int t = a.Row(row0); t <= a.Row(min(G, row0 + kRows) - 1); ++t) used |= sees(__shfl_sync(0xffffffffu, span.position, t), kp0 + lane);
         if (lane < kv4::kBlock) {
 #pragma unroll
           for (int j = 0; j < NG; ++j) {
@@ -301,7 +314,7 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
             const bool number = (pair & 0x7f80u) != 0x7f80u && (pair & 0x7f800000u) != 0x7f800000u;
             if (used && !number)
               for (int r = row0; r < min(G, row0 + kRows); ++r)
-                if (sees(a.positions[r / gqa], kp0 + lane)) atomicOr(nan_groups + r - row0, 1 << j);
+                if (sees(a.positions[a.Row(r)], kp0 + lane)) atomicOr(nan_groups + r - row0, 1 << j);
             if (!used || !number) pair = 0u;
           }
         }
@@ -492,32 +505,45 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        l[nt][r] += __shfl_xor_sync(0xffffffffu, l[nt][r], o);
-#pragma unroll
-        for (int j = 0; j < NG; ++j) base[nt][j][r] += __shfl_xor_sync(0xffffffffu, base[nt][j][r], o);
-      }
+      for (int o = 4; o < 32; o <<= 1) l[nt][r] += __shfl_xor_sync(0xffffffffu, l[nt][r], o);
   __syncthreads();                               // the ring is read by no one any more
   float* merge = reinterpret_cast<float*>(smem);
+  float* sums_lo = reinterpret_cast<float*>(smem + P::kMerge);                  // [warps][rows][groups]
   // warps that had blocks (the first ones)
   const int used = max(1, min(kWarps, min(per, span.blocks - split * per)));
-  const float back = 16777216.f / power, back16 = back * 0.0625f;      // codes n 2^-24, n 2^-20
+  if (warp < used) {
+    const float back = 16777216.f / power, back16 = back * 0.0625f;             // codes n 2^-24, n 2^-20
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    // (sixteen bytes of odd row pairs change places, so that the lanes of a store meet all banks)
-    float* dst = merge + (warp * kRows + 8 * nt + 2 * c) * P::kStride + 8 * g;
-    const int h0 = (c & 1) * 4, h1 = 4 - h0;
-    if (warp < used) {
+    for (int nt = 0; nt < NT; ++nt) {
+      // sum p lo over the lanes g: each round halves the values that a lane still adds up, until lane g has the sum of its own one
+      float v[2 * NG];
+#pragma unroll
+      for (int k = 0; k < 2 * NG; ++k) v[k] = base[nt][k >> 1][k & 1];
+      int width = 16;
+#pragma unroll
+      for (int n = NG; n >= 1; n >>= 1, width >>= 1) {
+#pragma unroll
+        for (int k = 0; k < n; ++k) {
+          const bool upper = lane & width;
+          const float give = upper ? v[k] : v[k + n];
+          v[k] = (upper ? v[k + n] : v[k]) + __shfl_xor_sync(0xffffffffu, give, width);
+        }
+      }
+#pragma unroll
+      for (; width >= 4; width >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], width);
+      const int k = g / (4 / NG);
+      sums_lo[(warp * kRows + 8 * nt + 2 * c + (k & 1)) * NG + (k >> 1)] = v[0];
+      // (sixteen bytes of odd row pairs change places, so that the lanes of a store meet all banks)
+      float* dst = merge + (warp * kRows + 8 * nt + 2 * c) * P::kStride + 8 * g;
+      const int h0 = (c & 1) * 4, h1 = 4 - h0;
 #pragma unroll
       for (int j = 0; j < NG; ++j)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float b = base[nt][j][r];
           const Frag(&o)[4] = acc[nt][j];
           float* at = dst + r * P::kStride + 64 * j;
-          *reinterpret_cast<float4*>(at + h0) = make_float4(fmaf(o[0].x[r], back, b), fmaf(o[1].x[r], back16, b), fmaf(o[2].x[r], back, b), fmaf(o[3].x[r], back16, b));
-          *reinterpret_cast<float4*>(at + h1) =
-              make_float4(fmaf(o[0].x[2 + r], back, b), fmaf(o[1].x[2 + r], back16, b), fmaf(o[2].x[2 + r], back, b), fmaf(o[3].x[2 + r], back16, b));
+          *reinterpret_cast<float4*>(at + h0) = make_float4(o[0].x[r] * back, o[1].x[r] * back16, o[2].x[r] * back, o[3].x[r] * back16);
+          *reinterpret_cast<float4*>(at + h1) = make_float4(o[0].x[2 + r] * back, o[1].x[2 + r] * back16, o[2].x[2 + r] * back, o[3].x[2 + r] * back16);
         }
       if (g == 0) {
 #pragma unroll
@@ -527,40 +553,79 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
   }
   __syncthreads();
   const size_t part_row = ((static_cast<size_t>(seq) * a.Hkv + hkv) * G + row0) * a.splits + split;
-  if (threadIdx.x < kRows) {
-    const int r = threadIdx.x;
-    float mx = -INFINITY, sum = 0.f;
-    for (int w = 0; w < used; ++w) mx = fmaxf(mx, ml[w * kRows + r].x);
-    for (int w = 0; w < used; ++w) {
-      const float2 x = ml[w * kRows + r];
-      const float f = x.x == -INFINITY ? 0.f : Exp2(x.x - mx);
-      weights[w * kRows + r] = f;
-      sum += x.x == -INFINITY && x.y == 0.f ? 0.f : f * x.y;
-    }
-    row_l[r] = sum == 0.f ? 0.f : 1.f / sum;
-    if (span.active > 1 && row0 + r < G) a.part_ml[part_row + static_cast<size_t>(r) * a.splits] = make_float2(mx, sum);
-  }
-  __syncthreads();
   for (int item = threadIdx.x; item < min(kRows, G - row0) * (D / 4); item += kWarps * 32) {
     const int r = item / (D / 4), q4 = item % (D / 4);
+    float weight[kWarps], mx = -INFINITY, sum = 0.f;
+    float2 x[kWarps];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      x[w] = w < used ? ml[w * kRows + r] : make_float2(-INFINITY, 0.f);
+      mx = fmaxf(mx, x[w].x);
+    }
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      weight[w] = x[w].x == -INFINITY ? 0.f : Exp2(x[w].x - mx);
+      sum += x[w].x == -INFINITY && x[w].y == 0.f ? 0.f : weight[w] * x[w].y;
+    }
     const float none = nan_groups[r] >> (q4 >> 4) & 1 ? __int_as_float(0x7fc00000) : 0.f;
     float4 o = make_float4(none, none, none, none);
     const float* src = merge + r * P::kStride + (q4 ^ ((r >> 1) & 1)) * 4;
-    for (int w = 0; w < used; ++w) {
-      const float f = weights[w * kRows + r];
-      const float4 x = *reinterpret_cast<const float4*>(src + w * kRows * P::kStride);
-      o.x = fmaf(f, x.x, o.x);
-      o.y = fmaf(f, x.y, o.y);
-      o.z = fmaf(f, x.z, o.z);
-      o.w = fmaf(f, x.w, o.w);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < used) {
+        const float f = weight[w], b = sums_lo[(w * kRows + r) * NG + (q4 >> 4)];
+        const float4 v = *reinterpret_cast<const float4*>(src + w * kRows * P::kStride);
+        o.x = fmaf(f, v.x + b, o.x);
+        o.y = fmaf(f, v.y + b, o.y);
+        o.z = fmaf(f, v.z + b, o.z);
+        o.w = fmaf(f, v.w + b, o.w);
+      }
     }
     if (span.active == 1) {
-      const float inv = row_l[r];
-      const size_t row = static_cast<size_t>((row0 + r) / gqa) * a.Hq + hkv * gqa + (row0 + r) % gqa;
-      StoreRow(a, row, D, 4 * q4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int t = a.Row(row0 + r);
+      StoreRow(a, static_cast<size_t>(t) * a.Hq + hkv * gqa + row0 + r - t * gqa, D, 4 * q4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    } else if constexpr (CLUSTER) {
+      *reinterpret_cast<float4*>(smem + P::kMerge + P::kBase + item * 16) = o;
+      if (q4 == 0) shared_ml[r] = make_float4(mx, sum, 0.f, 0.f);
     } else {
-      *reinterpret_cast<float4*>(a.part_acc + (part_row + static_cast<size_t>(r) * a.splits) * D + 4 * q4) = o;
+      const size_t row = part_row + static_cast<size_t>(r) * a.splits;
+      *reinterpret_cast<float4*>(a.part_acc + row * D + 4 * q4) = o;
+      if (q4 == 0) a.part_ml[row] = make_float2(mx, sum);
     }
+  }
+  if constexpr (CLUSTER) {
+    if (span.active == 1) return;
+    ptx::ClusterSync();
+    // each CTA finishes its share of the columns from all CTAs' shared memory: statistics first, then the sums, each in flight together
+    const uint32_t ml_at = ptx::SmemAddr(shared_ml), o_at = ptx::SmemAddr(smem + P::kMerge + P::kBase);
+    for (int item = split * kWarps * 32 + threadIdx.x; item < min(kRows, G - row0) * (D / 4); item += a.splits * kWarps * 32) {
+      const int r = item / (D / 4), q4 = item % (D / 4);
+      float weight[kMaxCluster], mx = -INFINITY, sum = 0.f;
+      float4 part[kMaxCluster], o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kMaxCluster; ++k) part[k] = k < span.active ? ptx::LoadRemote4(ml_at + r * 16, k) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kMaxCluster; ++k) mx = fmaxf(mx, part[k].x);
+#pragma unroll
+      for (int k = 0; k < kMaxCluster; ++k) {
+        weight[k] = part[k].x == -INFINITY ? 0.f : Exp2(part[k].x - mx);
+        sum += part[k].x == -INFINITY && part[k].y == 0.f ? 0.f : weight[k] * part[k].y;
+      }
+#pragma unroll
+      for (int k = 0; k < kMaxCluster; ++k) part[k] = k < span.active ? ptx::LoadRemote4(o_at + item * 16, k) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kMaxCluster; ++k) {
+        o.x = fmaf(weight[k], part[k].x, o.x);
+        o.y = fmaf(weight[k], part[k].y, o.y);
+        o.z = fmaf(weight[k], part[k].z, o.z);
+        o.w = fmaf(weight[k], part[k].w, o.w);
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int t = a.Row(row0 + r);
+      StoreRow(a, static_cast<size_t>(t) * a.Hq + hkv * gqa + row0 + r - t * gqa, D, 4 * q4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    }
+    ptx::ClusterSync();                          // nobody leaves while its results are read
   }
 }
 
@@ -639,40 +704,69 @@ __global__ void __launch_bounds__(kGroups * D / 4) CombineKv4Kernel(DecodeArgs a
       const float4 p = osum[k][q4];
       o.x += p.x; o.y += p.y; o.z += p.z; o.w += p.w;
     }
-    StoreRow(a, static_cast<size_t>(r / gqa) * a.Hq + hkv * gqa + r % gqa, D, 4 * q4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    const int t = a.Row(r);
+    StoreRow(a, static_cast<size_t>(t) * a.Hq + hkv * gqa + r - t * gqa, D, 4 * q4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
   }
 }
 
-template <int D, int NT>
+template <int D, int NT, bool CLUSTER>
 int LaunchDecode(DecodeArgs a, int batch, cudaStream_t s) {
-  // the kernel's limit of shared memory, once per device (a bit each; two threads may both set it)
+  // the kernel's limits of shared memory and cluster size, once per device (a bit each; two threads may both set them)
   static std::atomic<uint64_t> allowed{0};
+  const auto kern = DecodeKv4Kernel<D, NT, CLUSTER>;
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return static_cast<int>(e);
   if (device > 63 || !(allowed.load(std::memory_order_acquire) >> device & 1)) {
-    e = AllowAllSharedMemory(DecodeKv4Kernel<D, NT>);
+    e = AllowAllSharedMemory(kern);
+    if (e == cudaSuccess && CLUSTER) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return static_cast<int>(e);
     if (device < 64) allowed.fetch_or(uint64_t{1} << device, std::memory_order_release);
   }
   using P = Plan<D, NT>;
   a.warps = P::kWarps;
+  a.per_token = a.Hq == a.Hkv ? 0u : static_cast<uint32_t>((0x100000000ull + a.Hq / a.Hkv - 1) / (a.Hq / a.Hkv));
   const int G = a.Hq / a.Hkv * a.T, chunks = (G + P::kRows - 1) / P::kRows;
-  const int rc = LaunchPdl(DecodeKv4Kernel<D, NT>, dim3(a.splits, a.Hkv * chunks, batch), dim3(P::kWarps * 32), P::kSmem, s, a);
-  if (rc || a.splits == 1) return rc;
-  return LaunchPdl(CombineKv4Kernel<D>, dim3(G, a.Hkv, batch), dim3(kGroups * D / 4), 0, s, a);
+  const dim3 grid(a.splits, a.Hkv * chunks, batch);
+  if constexpr (CLUSTER) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(P::kWarps * 32);
+    cfg.dynamicSmemBytes = P::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = a.splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = g_use_pdl ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, kern, a);
+    ++g_launch_count;
+    return static_cast<int>(e);
+  } else {
+    const int rc = LaunchPdl(kern, grid, dim3(P::kWarps * 32), P::kSmem, s, a);
+    if (rc || a.splits == 1) return rc;
+    return LaunchPdl(CombineKv4Kernel<D>, dim3(G, a.Hkv, batch), dim3(kGroups * D / 4), 0, s, a);
+  }
 }
 
 // Row tiles of a CTA: as few CTAs as the registers allow read the same blocks.
-template <int D>
+template <int D, bool CLUSTER>
 int LaunchDecodeRows(const DecodeArgs& a, int batch, cudaStream_t s) {
   const int G = a.Hq / a.Hkv * a.T;
-  if (G <= 8) return LaunchDecode<D, 1>(a, batch, s);
+  if (G <= 8) return LaunchDecode<D, 1, CLUSTER>(a, batch, s);
   if constexpr (D == 256) {
-    return LaunchDecode<D, 2>(a, batch, s);
+    return LaunchDecode<D, 2, CLUSTER>(a, batch, s);
   } else {
-    return G <= 16 ? LaunchDecode<D, 2>(a, batch, s) : LaunchDecode<D, 4>(a, batch, s);
+    return G <= 16 ? LaunchDecode<D, 2, CLUSTER>(a, batch, s) : LaunchDecode<D, 4, CLUSTER>(a, batch, s);
   }
+}
+
+template <bool CLUSTER>
+int LaunchDecodeDim(const DecodeArgs& a, int batch, int D, cudaStream_t s) {
+  return D == 256 ? LaunchDecodeRows<256, CLUSTER>(a, batch, s) : (D == 128 ? LaunchDecodeRows<128, CLUSTER>(a, batch, s) : LaunchDecodeRows<64, CLUSTER>(a, batch, s));
 }
 
 }  // namespace
@@ -680,15 +774,15 @@ int LaunchDecodeRows(const DecodeArgs& a, int batch, cudaStream_t s) {
 
 using namespace r4dxb;
 
-/* scratch (splits > 1): batch * Hkv * G * splits * (D + 2) floats, 16-byte aligned: the partial sums, then (maximum, sum) pairs */
+/* scratch (splits > 1, no cluster): batch * Hkv * G * splits * (D + 2) floats, 16-byte aligned: the partial sums, then (maximum, sum) pairs */
 extern "C" int r4dxb_attn_decode_kv4(const void* q, const void* qg, const void* cache, const int* block_tables, const int* row_slot, int slots,
                                      int table_length, int pool, const int* positions, float* scratch, void* out, int T, int batch, int Hq,
-                                     int Hkv, int D, int splits, int window, int* status, void* stream) {
+                                     int Hkv, int D, int splits, int cluster, int window, int* status, void* stream) {
   if (T < 1 || T > 32 || batch < 1 || batch > 65535 || (row_slot == nullptr && batch != 1) || (row_slot != nullptr && T != 1) || Hkv < 1 || Hq < 1 ||
-      Hq % Hkv || (D != 64 && D != 128 && D != 256) || splits < 1 || splits > kMaxSplits || slots < 1 || table_length < 1 || pool < 1 || window < 0)
+      Hq % Hkv || (D != 64 && D != 128 && D != 256) || splits < 1 || splits > (cluster ? kMaxCluster : kMaxSplits) || slots < 1 || table_length < 1 || pool < 1 || window < 0)
     return R4DXB_BAD_ARG;
   if ((static_cast<long long>(Hq / Hkv) * T + 7) / 8 * Hkv > 65535) return R4DXB_TOO_LARGE;
-  if (q == nullptr || cache == nullptr || block_tables == nullptr || positions == nullptr || out == nullptr || (splits > 1 && scratch == nullptr))
+  if (q == nullptr || cache == nullptr || block_tables == nullptr || positions == nullptr || out == nullptr || (splits > 1 && !cluster && scratch == nullptr))
     return R4DXB_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(scratch)) & 15 ||
       (reinterpret_cast<uintptr_t>(qg) | reinterpret_cast<uintptr_t>(out)) & 7)
@@ -706,5 +800,5 @@ extern "C" int r4dxb_attn_decode_kv4(const void* q, const void* qg, const void* 
   a.status = status;
   a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.splits = splits; a.slots = slots; a.window = window;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return D == 256 ? LaunchDecodeRows<256>(a, batch, s) : (D == 128 ? LaunchDecodeRows<128>(a, batch, s) : LaunchDecodeRows<64>(a, batch, s));
+  return cluster ? LaunchDecodeDim<true>(a, batch, D, s) : LaunchDecodeDim<false>(a, batch, D, s);
 }

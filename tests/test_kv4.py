@@ -75,16 +75,18 @@ def test_calls_without_a_gpu_pool_are_refused():
             call()
 
 
-def test_splits_fill_the_chip_once():
+def test_splits_fill_the_chip_once_and_clusters_fit_it():
     from r4dx_b200.ops import kernels as K
     for rows in (1, 6, 48):
         for heads in (1, 2, 8):
             for batch in (1, 3, 64):
-                for length in (1, 8, 9, 5000):
+                for length in (1, 8, 9, 600, 5000):
                     for D, most in ((64, 32), (128, 32), (256, 16)):
-                        s = K.kv4_splits(rows, heads, batch, length, D)
+                        s, cluster = K.kv4_splits(rows, heads, batch, length, D)
                         least = -(-length // 2048)          # 4096 tokens a warp
-                        assert least <= s <= max(least, min(148, (length + 7) // 8)) and (s == least or s * heads * batch * -(-rows // most) <= 148)
+                        groups = heads * batch * -(-rows // most)
+                        assert least <= s <= max(least, min(148, (length + 7) // 8)) and (s == least or s * groups <= 148)
+                        assert not cluster or (1 < s <= 16 and groups <= {16: 7, 9: 15}.get(s, 74))
 
 
 def test_flag_of_the_commands():

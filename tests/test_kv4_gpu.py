@@ -181,6 +181,7 @@ DECODE = [
     (256, 24, 4, 1, 1, 0, True, None), (256, 24, 4, 1, 16, 0, True, None), (256, 8, 2, 1, 17, 0, True, 1), (256, 16, 2, 1, 1500, 0, True, None),
     (256, 24, 4, 8, 700, 0, True, None), (256, 6, 1, 3, 333, 100, False, 7), (128, 32, 8, 1, 2049, 0, False, None), (128, 5, 5, 2, 130, 0, True, 3),
     (128, 9, 1, 4, 4000, 513, False, None), (64, 32, 8, 1, 129, 0, False, 2), (64, 4, 4, 8, 40, 9, True, None), (64, 64, 1, 32, 260, 0, False, None),
+    (128, 32, 8, 1, 12001, 0, True, None), (256, 24, 4, 1, 13000, 3000, False, None), (64, 8, 1, 6, 20000, 0, False, None),
     (128, 3, 3, 1, 900, 1, False, None), (256, 2, 1, 5, 5, 0, False, 1), (256, 2, 2, 1, 9000, 0, True, None),
 ]
 
