@@ -15,6 +15,7 @@
 // kernel.  A sequence short enough for one CTA is finished by it.
 // A row with no visible token (position -1) gives zeros; a block that the table or pool does not have gives NaN to the rows that see it.
 #include <atomic>
+#include <type_traits>
 
 #include "kv4.cuh"
 #include "sm100_ptx.cuh"
@@ -44,13 +45,14 @@ struct DecodeArgs {
   __device__ __forceinline__ int Row(int r) const { return per_token != 0u ? static_cast<int>(__umulhi(static_cast<uint32_t>(r), per_token)) : r; }
 };
 
-// Warps of a CTA and blocks in flight per warp, by head dimension and row tiles.
+// Warps of a CTA, blocks that a warp takes at a time and slots of so many in its ring, by head dimension and row tiles.
 template <int D, int NT>
 struct Plan {
-  static constexpr int kWarps = D == 256 ? (NT == 1 ? 12 : 8) : (D == 128 ? (NT == 1 ? 16 : (NT == 2 ? 12 : 8)) : (NT == 4 ? 12 : 16));
-  static constexpr int kStages = D == 256 ? (NT == 1 ? 3 : 4) : 4;
+  static constexpr int kWarps = D == 256 ? 8 : (D == 128 ? (NT == 4 ? 8 : 12) : (NT == 4 ? 12 : 16));
+  static constexpr int kPair = NT == 1 ? 2 : 1;
+  static constexpr int kStages = NT == 1 ? 2 : 4;
   static constexpr int kRows = 8 * NT;
-  static constexpr int kRing = kWarps * kStages * kv4::Shape<D>::kRun;
+  static constexpr int kRing = kWarps * kStages * kPair * kv4::Shape<D>::kRun;
   static constexpr int kStride = D + 4;                          // floats between rows of the merge
   static constexpr int kMerge = kWarps * kRows * kStride * 4;
   static constexpr int kQuery = NT * (D / 32) * 512;             // operand B of the scores
@@ -143,7 +145,7 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
   PdlEnter();
   using S = kv4::Shape<D>;
   using P = Plan<D, NT>;
-  constexpr int NG = S::kGroups, NJ = D / 32, kWarps = P::kWarps, kRows = P::kRows, kStages = P::kStages;
+  constexpr int NG = S::kGroups, NJ = D / 32, kWarps = P::kWarps, kRows = P::kRows, kStages = P::kStages, kPair = P::kPair, kSlot = kPair * S::kRun;
   extern __shared__ __align__(128) unsigned char smem[];
   uint4* query = reinterpret_cast<uint4*>(smem + P::kBody);                     // [row tile][32 channels][lane]
   float* sums = reinterpret_cast<float*>(smem + P::kBody + P::kQuery);          // [row tile][32 channels][row]
@@ -175,11 +177,16 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
   const Span span = Visible(a.positions, a.T, a.window, a.splits, kWarps);
   if (split >= (CLUSTER && span.active > 1 ? a.splits : span.active)) return;       // (a cluster stays together, its CTAs without blocks merge too)
   const int per = (span.blocks + span.active - 1) / span.active;
-  const int b0 = span.first + split * per + warp, b1 = min(span.first + span.blocks, span.first + (split + 1) * per);
-  const int steps = b1 > b0 ? (b1 - b0 + kWarps - 1) / kWarps : 0;
+  // the CTA's blocks b0 .. b1 - 1 go around its warps, kPair at a time where there are more of them than warps
+  const int b0 = span.first + split * per, b1 = min(span.first + span.blocks, b0 + per);
+  const int take = b1 - b0 > kWarps ? kPair : 1, mine = b0 + warp * take, turn = kWarps * take;
+  const int steps = b1 > mine ? (b1 - mine + turn - 1) / turn : 0;
 
-  unsigned char* ring = smem + warp * kStages * S::kRun;
+  unsigned char* ring = smem + warp * kStages * kSlot;
   uint64_t* full = bars + warp * kStages;
+  const uint32_t ring_at = ptx::SmemAddr(ring), full_at = ptx::SmemAddr(full);
+  const uint8_t* head_run = a.cache + static_cast<size_t>(hkv) * S::kRun;
+  const size_t block_bytes = static_cast<size_t>(a.Hkv) * S::kRun;
   if (lane == 0) {
     for (int i = 0; i < kStages; ++i) ptx::MbarInit(full + i, 1);
     ptx::MbarFenceInit();
@@ -188,20 +195,27 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
   if (threadIdx.x < kRows) nan_groups[threadIdx.x] = 0;
   __syncwarp();
 
-  // ---- copies: block b0 + i warps into slot i % kStages ----
-  uint32_t missing = 0u;                         // by slot: there is no such block
+  // ---- copies: the blocks mine + i turn .. of step i into slot i % kStages ----
+  uint32_t missing = 0u;                         // a bit per block of the ring: there is none such
   int entry = -1;
   auto issue = [&](int i, int slot) {
-    if ((i & 31) == 0) entry = i + lane < steps && known ? a.table.BlockAt(b0 + (i + lane) * kWarps) : -1;
-    const int blk = __shfl_sync(0xffffffffu, entry, i & 31);
-    missing = blk < 0 ? missing | 1u << slot : missing & ~(1u << slot);
+    if ((i * kPair & 31) == 0) {
+      const int k = i + lane / kPair, b = mine + k * turn + lane % kPair;
+      entry = lane % kPair < take && b < b1 && known ? a.table.BlockAt(b) : -1;
+    }
+    int blk[kPair], copies = 0;
+#pragma unroll
+    for (int h = 0; h < kPair; ++h) {
+      blk[h] = __shfl_sync(0xffffffffu, entry, (i * kPair + h) & 31);
+      copies += blk[h] >= 0;
+      const uint32_t bit = 1u << (slot * kPair + h);
+      missing = blk[h] < 0 ? missing | bit : missing & ~bit;
+    }
     if (lane == 0) {
-      if (blk < 0) {
-        ptx::MbarArrive(full + slot);
-      } else {
-        ptx::MbarArriveExpectTx(full + slot, S::kRun);
-        ptx::BulkLoad(ring + slot * S::kRun, a.cache + (static_cast<size_t>(blk) * a.Hkv + hkv) * S::kRun, S::kRun, full + slot);
-      }
+      ptx::MbarArriveExpectTxAt(full_at + slot * 8, copies * S::kRun);
+#pragma unroll
+      for (int h = 0; h < kPair; ++h)
+        if (blk[h] >= 0) ptx::BulkLoadAt(ring_at + slot * kSlot + h * S::kRun, head_run + blk[h] * block_bytes, S::kRun, full_at + slot * 8);
     }
   };
   for (int i = 0; i < min(steps, kStages); ++i) issue(i, i);
@@ -248,7 +262,7 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
     qpair[nt][1] = NG == 4 ? PackBf16(0.f, next) : 0u;
   }
 
-  const float scale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f / kUnit, step = kRescaleStep / scale;
+  const float scale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f / kUnit, rise = kRescaleStep / scale;
   int pos[NT][2], p_min = 0x7fffffff, p_max = -1;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -262,11 +276,6 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
   p_min = __reduce_min_sync(0xffffffffu, p_min);
   p_max = __reduce_max_sync(0xffffffffu, p_max);
   auto sees = [&](int at, int kp) { return kp <= at && (a.window == 0 || kp > at - a.window); };
-
-  // steps whose blocks all rows see whole: [whole0, whole1)
-  const int stride = kWarps * kv4::kBlock, begin = b0 * kv4::kBlock;
-  const int whole1 = p_min >= begin + kv4::kBlock - 1 ? (p_min - (begin + kv4::kBlock - 1)) / stride + 1 : 0;
-  const int whole0 = a.window > 0 && p_max - a.window >= begin ? (p_max - a.window - begin) / stride + 1 : 0;
 
   float m[NT][2], ms[NT][2], l[NT][2];           // rows 8 nt + 2 c, + 1: maximum, the same times the scale (0 for -inf), sum over this lane's tokens
   Frag acc[NT][NG][4];
@@ -282,154 +291,157 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
       for (int e = 0; e < 4; ++e) acc[nt][j][e] = {{0.f, 0.f, 0.f, 0.f}};
     }
   }
-  uint32_t limit = 39u << 7;                     // scales (bf16 bits) from which the sums need a smaller power of two ..
+  float limit = __uint_as_float(39u << 23);      // scales from which the sums need a smaller power of two ..
   float power = __uint_as_float((254u - 32u) << 23);      // .. than this: 2^-(exponent of the largest scale), at first 2^95
 
-  bool ok = true;
-  int i = 0, slot = 0, kp0 = begin;
-  uint32_t phase = 0u;
-#pragma unroll 1
-  for (; i < steps; ++i, kp0 += stride) {
-    if (!__all_sync(0xffffffffu, ptx::MbarTestWait(full + slot, phase))) ok = ptx::WarpMbarWait(full + slot, phase, abort_flag, 1);
-    if (!ok) break;
-    if (missing >> slot & 1u) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          if (pos[nt][r] >= kp0 && (a.window == 0 || kp0 + kv4::kBlock - 1 > pos[nt][r] - a.window)) l[nt][r] = __int_as_float(0x7fc00000);
-    } else {
-      uint32_t* kw = reinterpret_cast<uint32_t*>(ring + slot * S::kRun);
-      uint32_t* vw = kw + S::kPart / 4;
-      const bool whole = i >= whole0 && i < whole1;
-      if (!whole) {
-        // Value pairs that are no numbers, or of tokens that no row here sees (whose bytes may be anything), are zeros from here on: what
-        // a row does not see has the weight 0, and 0 x NaN would reach it.  Rows that do see a NaN are noted.
-        bool used = false;
-        for (int t = a.Row(row0); t <= a.Row(min(G, row0 + kRows) - 1); ++t) used |= sees(__shfl_sync(0xffffffffu, span.position, t), kp0 + lane);
-        if (lane < kv4::kBlock) {
-#pragma unroll
-          for (int j = 0; j < NG; ++j) {
-            uint32_t& pair = vw[2 * D + lane * NG + j];
-            const bool number = (pair & 0x7f80u) != 0x7f80u && (pair & 0x7f800000u) != 0x7f800000u;
-            if (used && !number)
-              for (int r = row0; r < min(G, row0 + kRows); ++r)
-                if (sees(a.positions[a.Row(r)], kp0 + lane)) atomicOr(nan_groups + r - row0, 1 << j);
-            if (!used || !number) pair = 0u;
-          }
-        }
-        ptx::FenceProxyAsyncShared();            // (the next copy into the slot comes after these stores)
-        __syncwarp();
-      }
-
-      // ---- scores: tokens g (x[0], x[1]) and g + 8 (x[2], x[3]) of rows 2 c, 2 c + 1 ----
-      Frag sc[NT];
-      {
-        uint32_t pa[NG], pb[NG];
-        LoadWords<NG>(kw + 2 * D + g * NG, pa);
-        LoadWords<NG>(kw + 2 * D + (g + 8) * NG, pb);
-        const uint32_t mine_a = kw[2 * D + g * NG + c % NG], mine_b = kw[2 * D + (g + 8) * NG + c % NG];
-        uint32_t ca[NJ], cb[NJ];
-        if constexpr (D == 256) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int at = ((h ^ (g & 1)) * 16) + c * 4;
-            const uint4 x = *reinterpret_cast<const uint4*>(kw + g * 32 + at), y = *reinterpret_cast<const uint4*>(kw + (g + 8) * 32 + at);
-            ca[4 * h] = x.x; ca[4 * h + 1] = x.y; ca[4 * h + 2] = x.z; ca[4 * h + 3] = x.w;
-            cb[4 * h] = y.x; cb[4 * h + 1] = y.y; cb[4 * h + 2] = y.z; cb[4 * h + 3] = y.w;
-          }
-        } else {
-          LoadWords<NJ>(kw + g * (D / 8) + c * NJ, ca);
-          LoadWords<NJ>(kw + (g + 8) * (D / 8) + c * NJ, cb);
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sc[nt] = MmaBf16(mine_a, mine_b, NG == 4 ? mine_a : 0u, NG == 4 ? mine_b : 0u, qpair[nt][0], qpair[nt][1], Frag{{0.f, 0.f, 0.f, 0.f}});
+  // N consecutive blocks from token kp0 on, as they lie in the ring
+  auto blocks = [&](auto count, uint32_t* const run, const int kp0) {
+    constexpr int N = decltype(count)::value, kWords = S::kRun / 4, kValues = S::kPart / 4;
+    const bool whole = kp0 + N * kv4::kBlock - 1 <= p_min && (a.window == 0 || kp0 > p_max - a.window);
+    if (!whole) {
+      // Value pairs that are no numbers, or of tokens that no row here sees (whose bytes may be anything), are zeros from here on: what
+      // a row does not see has the weight 0, and 0 x NaN would reach it.  Rows that do see a NaN are noted.
+      bool used = false;
+      const int kp = kp0 + lane;
+      for (int t = a.Row(row0); t <= a.Row(min(G, row0 + kRows) - 1); ++t) used |= sees(__shfl_sync(0xffffffffu, span.position, t), kp);
+      if (lane < N * kv4::kBlock) {
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
-          Frag s4[NT];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) s4[nt] = {{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t x = ca[2 * j + h], y = cb[2 * j + h], x8 = x >> 8, y8 = y >> 8;
-            const uint32_t a0 = Codes(x), a1 = Codes(y), a2 = Codes16(x), a3 = Codes16(y), a4 = Codes(x8), a5 = Codes(y8), a6 = Codes16(x8), a7 = Codes16(y8);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const uint4 b = query[(nt * NJ + 2 * j + h) * 32 + lane];
-              s4[nt] = MmaF16(a0, a1, a2, a3, b.x, b.y, s4[nt]);
-              s4[nt] = MmaF16(a4, a5, a6, a7, b.z, b.w, s4[nt]);
-            }
-          }
-          const float sa = BfLo(pa[j]), sb = BfLo(pb[j]);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            sc[nt].x[0] = fmaf(sa, s4[nt].x[0], sc[nt].x[0]);
-            sc[nt].x[1] = fmaf(sa, s4[nt].x[1], sc[nt].x[1]);
-            sc[nt].x[2] = fmaf(sb, s4[nt].x[2], sc[nt].x[2]);
-            sc[nt].x[3] = fmaf(sb, s4[nt].x[3], sc[nt].x[3]);
-          }
+          uint32_t& pair = run[lane / kv4::kBlock * kWords + kValues + 2 * D + lane % kv4::kBlock * NG + j];
+          const bool number = (pair & 0x7f80u) != 0x7f80u && (pair & 0x7f800000u) != 0x7f800000u;
+          if (used && !number)
+            for (int r = row0; r < min(G, row0 + kRows); ++r)
+              if (sees(a.positions[a.Row(r)], kp)) atomicOr(nan_groups + r - row0, 1 << j);
+          if (!used || !number) pair = 0u;
         }
       }
-      if (!whole) {
+      ptx::FenceProxyAsyncShared();              // (the next copy into the slot comes after these stores)
+      __syncwarp();
+    }
+
+    // ---- scores: tokens g (x[0], x[1]) and g + 8 (x[2], x[3]) of rows 2 c, 2 c + 1 ----
+    Frag sc[N][NT];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const uint32_t* kw = run + n * kWords;
+      uint32_t pa[NG], pb[NG];
+      LoadWords<NG>(kw + 2 * D + g * NG, pa);
+      LoadWords<NG>(kw + 2 * D + (g + 8) * NG, pb);
+      const uint32_t mine_a = kw[2 * D + g * NG + c % NG], mine_b = kw[2 * D + (g + 8) * NG + c % NG];
+      uint32_t ca[NJ], cb[NJ];
+      if constexpr (D == 256) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int at = ((h ^ (g & 1)) * 16) + c * 4;
+          const uint4 x = *reinterpret_cast<const uint4*>(kw + g * 32 + at), y = *reinterpret_cast<const uint4*>(kw + (g + 8) * 32 + at);
+          ca[4 * h] = x.x; ca[4 * h + 1] = x.y; ca[4 * h + 2] = x.z; ca[4 * h + 3] = x.w;
+          cb[4 * h] = y.x; cb[4 * h + 1] = y.y; cb[4 * h + 2] = y.z; cb[4 * h + 3] = y.w;
+        }
+      } else {
+        LoadWords<NJ>(kw + g * (D / 8) + c * NJ, ca);
+        LoadWords<NJ>(kw + (g + 8) * (D / 8) + c * NJ, cb);
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        sc[n][nt] = MmaBf16(mine_a, mine_b, NG == 4 ? mine_a : 0u, NG == 4 ? mine_b : 0u, qpair[nt][0], qpair[nt][1], Frag{{0.f, 0.f, 0.f, 0.f}});
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        Frag s4[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s4[nt] = {{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t x = ca[2 * j + h], y = cb[2 * j + h], x8 = x >> 8, y8 = y >> 8;
+          const uint32_t a0 = Codes(x), a1 = Codes(y), a2 = Codes16(x), a3 = Codes16(y), a4 = Codes(x8), a5 = Codes(y8), a6 = Codes16(x8), a7 = Codes16(y8);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint4 b = query[(nt * NJ + 2 * j + h) * 32 + lane];
+            s4[nt] = MmaF16(a0, a1, a2, a3, b.x, b.y, s4[nt]);
+            s4[nt] = MmaF16(a4, a5, a6, a7, b.z, b.w, s4[nt]);
+          }
+        }
+        const float sa = BfLo(pa[j]), sb = BfLo(pb[j]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          sc[n][nt].x[0] = fmaf(sa, s4[nt].x[0], sc[n][nt].x[0]);
+          sc[n][nt].x[1] = fmaf(sa, s4[nt].x[1], sc[n][nt].x[1]);
+          sc[n][nt].x[2] = fmaf(sb, s4[nt].x[2], sc[n][nt].x[2]);
+          sc[n][nt].x[3] = fmaf(sb, s4[nt].x[3], sc[n][nt].x[3]);
+        }
+      }
+    }
+    if (!whole) {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (!sees(pos[nt][e & 1], kp0 + g + (e >> 1) * 8)) sc[nt].x[e] = -INFINITY;
-      }
+            if (!sees(pos[nt][e & 1], kp0 + n * kv4::kBlock + g + (e >> 1) * 8)) sc[n][nt].x[e] = -INFINITY;
+    }
 
-      // ---- running maximum, power of two of the scales, probabilities ----
-      uint32_t pa[NG], pb[NG];
-      LoadWords<NG>(vw + 2 * D + g * NG, pa);
-      LoadWords<NG>(vw + 2 * D + (g + 8) * NG, pb);
-      uint32_t largest = 0u;                     // (of the lower halves)
+    // ---- running maximum, power of two of the scales, probabilities ----
+    uint32_t pa[N][NG], pb[N][NG];
+    float largest = 0.f, top[NT][2];
 #pragma unroll
-      for (int j = 0; j < NG; ++j) largest = __vmaxu2(largest, __vmaxu2(pa[j], pb[j]));
-      largest &= 0xffffu;
-      bool move = largest >= limit;
+    for (int n = 0; n < N; ++n) {
+      LoadWords<NG>(run + n * kWords + kValues + 2 * D + g * NG, pa[n]);
+      LoadWords<NG>(run + n * kWords + kValues + 2 * D + (g + 8) * NG, pb[n]);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) move = move || fmaxf(sc[nt].x[0], sc[nt].x[2]) > m[nt][0] + step || fmaxf(sc[nt].x[1], sc[nt].x[3]) > m[nt][1] + step;
-      if (__any_sync(0xffffffffu, move)) {
-        largest = __reduce_max_sync(0xffffffffu, largest >= 0x7f80u ? 0u : largest);
-        float shrink = 1.f;
-        if (largest >= limit) {
-          const uint32_t e = largest >> 7;
-          const float now = __uint_as_float((254u - e) << 23);
-          shrink = now / power;
-          power = now;
-          limit = (e + 7u) << 7;
+      for (int j = 0; j < NG; ++j) largest = fmaxf(largest, fmaxf(BfLo(pa[n][j]), BfLo(pb[n][j])));
+    }
+    bool move = largest >= limit;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        top[nt][r] = fmaxf(sc[0][nt].x[r], sc[0][nt].x[2 + r]);
+#pragma unroll
+        for (int n = 1; n < N; ++n) top[nt][r] = fmaxf(top[nt][r], fmaxf(sc[n][nt].x[r], sc[n][nt].x[2 + r]));
+        move = move || top[nt][r] > m[nt][r] + rise;
+      }
+    if (__any_sync(0xffffffffu, move)) {
+      const uint32_t bits = __reduce_max_sync(0xffffffffu, largest < INFINITY ? __float_as_uint(largest) : 0u);
+      float shrink = 1.f;
+      if (bits >= __float_as_uint(limit)) {
+        const uint32_t e = bits >> 23;
+        const float now = __uint_as_float((254u - e) << 23);
+        shrink = now / power;
+        power = now;
+        limit = __uint_as_float((e + 7u) << 23);
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float f[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float n = fmaxf(m[nt][r], top[nt][r]);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, o));
+          f[r] = n == -INFINITY ? 1.f : Exp2((m[nt][r] - n) * scale);
+          m[nt][r] = n;
+          ms[nt][r] = n == -INFINITY ? 0.f : n * scale;
+          l[nt][r] *= f[r];
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float f[2];
+        for (int j = 0; j < NG; ++j) {
+          base[nt][j][0] *= f[0];
+          base[nt][j][1] *= f[1];
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float n = fmaxf(m[nt][r], fmaxf(sc[nt].x[r], sc[nt].x[2 + r]));
+          for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, o));
-            f[r] = n == -INFINITY ? 1.f : Exp2((m[nt][r] - n) * scale);
-            m[nt][r] = n;
-            ms[nt][r] = n == -INFINITY ? 0.f : n * scale;
-            l[nt][r] *= f[r];
-          }
-#pragma unroll
-          for (int j = 0; j < NG; ++j) {
-            base[nt][j][0] *= f[0];
-            base[nt][j][1] *= f[1];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-              for (int x = 0; x < 4; ++x) acc[nt][j][e].x[x] *= f[x & 1] * shrink;
-          }
+            for (int x = 0; x < 4; ++x) acc[nt][j][e].x[x] *= f[x & 1] * shrink;
         }
       }
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const uint32_t* vw = run + n * kWords + kValues;
       float p[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        p[nt][0] = Exp2(fmaf(sc[nt].x[0], scale, -ms[nt][0]));
-        p[nt][1] = Exp2(fmaf(sc[nt].x[1], scale, -ms[nt][1]));
-        p[nt][2] = Exp2(fmaf(sc[nt].x[2], scale, -ms[nt][0]));
-        p[nt][3] = Exp2(fmaf(sc[nt].x[3], scale, -ms[nt][1]));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[nt][e] = Exp2(fmaf(sc[n][nt].x[e], scale, -ms[nt][e & 1]));
         l[nt][0] += p[nt][0] + p[nt][2];
         l[nt][1] += p[nt][1] + p[nt][3];
       }
@@ -455,7 +467,7 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
       }
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
-        const float sa = BfLo(pa[j]) * power, sb = BfLo(pb[j]) * power, la = BfHi(pa[j]), lb = BfHi(pb[j]);
+        const float sa = BfLo(pa[n][j]) * power, sb = BfLo(pb[n][j]) * power, la = BfHi(pa[n][j]), lb = BfHi(pb[n][j]);
         uint32_t w0[NT], w1[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -478,8 +490,37 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
           for (int k = 0; k < 4; ++k) t[k] >>= 8;
         }
       }
-      __syncwarp();                              // every lane has read the slot
     }
+  };
+
+  bool ok = true;
+  int i = 0, slot = 0;
+  uint32_t phase = 0u;
+#pragma unroll 1
+  for (; i < steps; ++i) {
+    if (!__all_sync(0xffffffffu, ptx::MbarTestWaitAt(full_at + slot * 8, phase))) ok = ptx::WarpMbarWait(full + slot, phase, abort_flag, 1);
+    if (!ok) break;
+    uint32_t* run = reinterpret_cast<uint32_t*>(ring + slot * kSlot);
+    const int b = mine + i * turn, there = min(take, b1 - b);
+    const uint32_t gone = missing >> (slot * kPair) & ((1u << there) - 1u);
+    if (there == kPair && gone == 0u) {
+      blocks(std::integral_constant<int, kPair>{}, run, b * kv4::kBlock);
+    } else {
+#pragma unroll 1
+      for (int h = 0; h < there; ++h) {
+        const int kp0 = (b + h) * kv4::kBlock;
+        if (gone >> h & 1u) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+              if (pos[nt][r] >= kp0 && (a.window == 0 || kp0 + kv4::kBlock - 1 > pos[nt][r] - a.window)) l[nt][r] = __int_as_float(0x7fc00000);
+        } else if constexpr (kPair > 1) {
+          blocks(std::integral_constant<int, 1>{}, run + h * (S::kRun / 4), kp0);
+        }
+      }
+    }
+    __syncwarp();                                // every lane has read the slot
     if (i + kStages < steps) issue(i + kStages, slot);
     if (++slot == kStages) {
       slot = 0;
@@ -510,7 +551,7 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
   float* merge = reinterpret_cast<float*>(smem);
   float* sums_lo = reinterpret_cast<float*>(smem + P::kMerge);                  // [warps][rows][groups]
   // warps that had blocks (the first ones)
-  const int used = max(1, min(kWarps, min(per, span.blocks - split * per)));
+  const int used = max(1, min(kWarps, (b1 - b0 + take - 1) / take));
   if (warp < used) {
     const float back = 16777216.f / power, back16 = back * 0.0625f;             // codes n 2^-24, n 2^-20
 #pragma unroll

@@ -1271,7 +1271,7 @@ def kv4_read(cache, block_table, positions, k: Optional[torch.Tensor] = None, v:
 # Clusters of the decode kernel (one CTA to an SM) that run at a time, by CTAs of a cluster: (size, clusters), of the sizes that fill the chip
 _KV4_CLUSTERS = ((16, 7), (9, 15), (6, 22), (5, 26), (4, 33), (3, 45), (2, 74))
 # warps of a CTA by head dimension and query rows of a CTA
-_KV4_WARPS = {(64, 8): 16, (64, 16): 16, (64, 32): 12, (128, 8): 16, (128, 16): 12, (128, 32): 8, (256, 8): 12, (256, 16): 8}
+_KV4_WARPS = {(64, 8): 16, (64, 16): 16, (64, 32): 12, (128, 8): 12, (128, 16): 12, (128, 32): 8, (256, 8): 8, (256, 16): 8}
 
 
 @functools.lru_cache(maxsize=4096)
