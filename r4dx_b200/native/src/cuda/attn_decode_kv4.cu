@@ -39,7 +39,7 @@ struct DecodeArgs {
   __nv_bfloat16* out;          // [T, Hq, D]
   int* status;
   int T, Hq, Hkv, splits, slots, window;
-  int warps;                   // of a CTA
+  int chunk;                   // blocks of a sequence for which another CTA joins
   uint32_t per_token;          // 2^32 / (query heads per kv head), rounded up; 0: one query head
   // row r of a kv head's G = T Hq / Hkv belongs to token Row(r)
   __device__ __forceinline__ int Row(int r) const { return per_token != 0u ? static_cast<int>(__umulhi(static_cast<uint32_t>(r), per_token)) : r; }
@@ -48,7 +48,8 @@ struct DecodeArgs {
 // Warps of a CTA, blocks that a warp takes at a time and slots of so many in its ring, by head dimension and row tiles.
 template <int D, int NT>
 struct Plan {
-  static constexpr int kWarps = D == 256 ? 8 : (D == 128 ? (NT == 4 ? 8 : 12) : (NT == 4 ? 12 : 16));
+  static constexpr int kWarps = D == 256 ? 8 : (D == 128 ? (NT == 4 ? 8 : 12) : (NT == 4 ? 12 : (NT == 1 ? 8 : 16)));
+  static constexpr int kCtas = D == 64 && NT == 1 ? 2 : 1;
   static constexpr int kPair = NT == 1 ? 2 : 1;
   static constexpr int kStages = NT == 1 ? 2 : 4;
   static constexpr int kRows = 8 * NT;
@@ -64,12 +65,12 @@ struct Plan {
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
-// The blocks that the rows of a call may see and the number of CTAs that share them: a block per warp at least.
+// The blocks that the rows of a call may see and the number of CTAs that share them: one for every `chunk` blocks.
 struct Span {
   int first, blocks, active;
   int position;                // of token `lane`, -1 beyond the last
 };
-__device__ __forceinline__ Span Visible(const int* positions, int T, int window, int splits, int warps) {
+__device__ __forceinline__ Span Visible(const int* positions, int T, int window, int splits, int chunk) {
   const int lane = threadIdx.x & 31;
   const int p = lane < T ? positions[lane] : -1;
   Span s;
@@ -77,7 +78,7 @@ __device__ __forceinline__ Span Visible(const int* positions, int T, int window,
   const int high = __reduce_max_sync(0xffffffffu, p), low = __reduce_min_sync(0xffffffffu, p < 0 ? 0x7fffffff : p);
   s.first = window > 0 && high >= 0 ? max(0, low - window + 1) / kv4::kBlock : 0;
   s.blocks = high >= 0 ? high / kv4::kBlock + 1 - s.first : 0;
-  s.active = max(1, min(splits, (s.blocks + warps - 1) / warps));
+  s.active = max(1, min(splits, static_cast<int>((static_cast<unsigned>(s.blocks) + chunk - 1) / chunk)));
   return s;
 }
 
@@ -141,7 +142,7 @@ __device__ __forceinline__ void StoreRow(const DecodeArgs& a, size_t row, int D,
 }
 
 template <int D, int NT, bool CLUSTER>
-__global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(DecodeArgs a) {
+__global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) DecodeKv4Kernel(DecodeArgs a) {
   PdlEnter();
   using S = kv4::Shape<D>;
   using P = Plan<D, NT>;
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, 1) DecodeKv4Kernel(D
                  : make_uint4(0u, 0u, 0u, 0u);
   };
   uint4 query_next = warp < NT * NJ ? load_query(warp) : make_uint4(0u, 0u, 0u, 0u);
-  const Span span = Visible(a.positions, a.T, a.window, a.splits, kWarps);
+  const Span span = Visible(a.positions, a.T, a.window, a.splits, a.chunk);
   if (split >= (CLUSTER && span.active > 1 ? a.splits : span.active)) return;       // (a cluster stays together, its CTAs without blocks merge too)
   const int per = (span.blocks + span.active - 1) / span.active;
   // the CTA's blocks b0 .. b1 - 1 go around its warps, kPair at a time where there are more of them than warps
@@ -697,7 +698,7 @@ __global__ void __launch_bounds__(kGroups * D / 4) CombineKv4Kernel(DecodeArgs a
 #pragma unroll
   for (int k = 0; k < (kMaxSplits + kThreads - 1) / kThreads; ++k)
     x[k] = static_cast<int>(threadIdx.x) + k * kThreads < a.splits ? a.part_ml[at + threadIdx.x + k * kThreads] : make_float2(0.f, 0.f);
-  const int active = Visible(a.positions, a.T, a.window, a.splits, a.warps).active;
+  const int active = Visible(a.positions, a.T, a.window, a.splits, a.chunk).active;
   if (active == 1) return;                       // the first kernel has finished the rows
   float m = -INFINITY;
 #pragma unroll
@@ -765,7 +766,6 @@ int LaunchDecode(DecodeArgs a, int batch, cudaStream_t s) {
     if (device < 64) allowed.fetch_or(uint64_t{1} << device, std::memory_order_release);
   }
   using P = Plan<D, NT>;
-  a.warps = P::kWarps;
   a.per_token = a.Hq == a.Hkv ? 0u : static_cast<uint32_t>((0x100000000ull + a.Hq / a.Hkv - 1) / (a.Hq / a.Hkv));
   const int G = a.Hq / a.Hkv * a.T, chunks = (G + P::kRows - 1) / P::kRows;
   const dim3 grid(a.splits, a.Hkv * chunks, batch);
@@ -818,9 +818,9 @@ using namespace r4dxb;
 /* scratch (splits > 1, no cluster): batch * Hkv * G * splits * (D + 2) floats, 16-byte aligned: the partial sums, then (maximum, sum) pairs */
 extern "C" int r4dxb_attn_decode_kv4(const void* q, const void* qg, const void* cache, const int* block_tables, const int* row_slot, int slots,
                                      int table_length, int pool, const int* positions, float* scratch, void* out, int T, int batch, int Hq,
-                                     int Hkv, int D, int splits, int cluster, int window, int* status, void* stream) {
+                                     int Hkv, int D, int splits, int chunk, int cluster, int window, int* status, void* stream) {
   if (T < 1 || T > 32 || batch < 1 || batch > 65535 || (row_slot == nullptr && batch != 1) || (row_slot != nullptr && T != 1) || Hkv < 1 || Hq < 1 ||
-      Hq % Hkv || (D != 64 && D != 128 && D != 256) || splits < 1 || splits > (cluster ? kMaxCluster : kMaxSplits) || slots < 1 || table_length < 1 || pool < 1 || window < 0)
+      Hq % Hkv || (D != 64 && D != 128 && D != 256) || chunk < 1 || splits < 1 || splits > (cluster ? kMaxCluster : kMaxSplits) || slots < 1 || table_length < 1 || pool < 1 || window < 0)
     return R4DXB_BAD_ARG;
   if ((static_cast<long long>(Hq / Hkv) * T + 7) / 8 * Hkv > 65535) return R4DXB_TOO_LARGE;
   if (q == nullptr || cache == nullptr || block_tables == nullptr || positions == nullptr || out == nullptr || (splits > 1 && !cluster && scratch == nullptr))
@@ -839,7 +839,7 @@ extern "C" int r4dxb_attn_decode_kv4(const void* q, const void* qg, const void* 
   a.part_ml = reinterpret_cast<float2*>(scratch + static_cast<size_t>(batch) * Hq * T * splits * D);
   a.out = static_cast<__nv_bfloat16*>(out);
   a.status = status;
-  a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.splits = splits; a.slots = slots; a.window = window;
+  a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.splits = splits; a.chunk = chunk; a.slots = slots; a.window = window;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return cluster ? LaunchDecodeDim<true>(a, batch, D, s) : LaunchDecodeDim<false>(a, batch, D, s);
 }

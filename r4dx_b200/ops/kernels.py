@@ -1163,7 +1163,7 @@ def q4x_hc_gate(h, norm_w, w_down_inject, w_up, mid, injv, rstd, x, T: int, hc: 
 # ---- attention over a 4-bit paged KV cache (format: quant/kv4.py) ------------------------------------------------------------------
 register_cuda_sig("r4dxb_attn_precore_kv4", _I, [_P] * 8 + [_I] * 3 + [_P, _P] + [_I] * 5 + [_F, _F, _I, _P])
 register_cuda_sig("r4dxb_kv4_read", _I, [_P] * 3 + [_I] * 3 + [_P] * 3 + [_I] * 3 + [_P])
-register_cuda_sig("r4dxb_attn_decode_kv4", _I, [_P] * 5 + [_I] * 3 + [_P] * 3 + [_I] * 8 + [_P, _P])
+register_cuda_sig("r4dxb_attn_decode_kv4", _I, [_P] * 5 + [_I] * 3 + [_P] * 3 + [_I] * 9 + [_P, _P])
 register_cuda_sig("r4dxb_attn_prefill_kv4", _I, [_P] * 4 + [_I] * 2 + [_P] + [_I] * 6 + [_P] * 3)
 
 KV4_MAX_ROWS = 32           # rows of one sequence that attn_decode_kv4 takes
@@ -1270,32 +1270,40 @@ def kv4_read(cache, block_table, positions, k: Optional[torch.Tensor] = None, v:
 
 # Clusters of the decode kernel (one CTA to an SM) that run at a time, by CTAs of a cluster: (size, clusters), of the sizes that fill the chip
 _KV4_CLUSTERS = ((16, 7), (9, 15), (6, 22), (5, 26), (4, 33), (3, 45), (2, 74))
-# warps of a CTA by head dimension and query rows of a CTA
-_KV4_WARPS = {(64, 8): 16, (64, 16): 16, (64, 32): 12, (128, 8): 12, (128, 16): 12, (128, 32): 8, (256, 8): 8, (256, 16): 8}
+# warps of a CTA, and CTAs of an SM, by head dimension and query rows of a CTA
+_KV4_CTAS = {(64, 8): (8, 2), (64, 16): (16, 1), (64, 32): (12, 1), (128, 8): (12, 1), (128, 16): (12, 1), (128, 32): (8, 1), (256, 8): (8, 1),
+             (256, 16): (8, 1)}
 
 
 @functools.lru_cache(maxsize=4096)
 def kv4_splits(rows: int, Hkv: int, batch: int, length: int, D: int) -> tuple:
-    """(CTAs that share a sequence's blocks, whether they are a cluster) for tables of ``length`` blocks.
+    """(CTAs that may share a sequence's blocks, visible blocks for which another one joins, whether they are a cluster) for tables of
+    ``length`` blocks.
 
     A cluster merges its results itself, where more CTAs need a second kernel; but no more than 7 clusters of 16, 15 of 9 .. fit the chip at
     a time.  Up to 256 / D blocks to a warp of a full table it is faster (us on the device by keys, cluster / two kernels: 24 heads over 4 of 256
-    1000 8.6 / 9.1, 4096 11.0 / 9.6; 32 over 8 of 128 2000 7.6 / 8.5, 8192 11.1 / 10.9; of 64 4096 7.9 / 8.1, 8192 9.5 / 9.0).
-    Longer tables: all 148 SMs once, and 128 tokens or more
-    to a CTA.  Never so few CTAs that a warp adds up more than 4096 tokens: tensor-core sums round towards zero, by up to 2^-24 of the sum of codes
+    1000 6.9 / 7.6, 4096 9.3 / 8.0; 32 over 8 of 128 2000 6.2 / 7.2, 8192 9.5 / 9.4; of 64 8192 8.0 / 8.4, 16384 10.3 / 9.7).
+    Longer tables: all SMs once, a block to a warp at least.  Batches that leave less than four CTAs to a sequence: twice as many,
+    since their lengths differ, and for four blocks to a warp at least (16 sequences up to 8192 keys, 24 heads over 4 of 256, by CTAs 1 2 3 4 6 8:
+    62 38 29 28 33 37 us; 32 over 8 of 128 36 26 31 34 38 45; 64 sequences up to 1000 keys of the first 19 37 42 46 55 59).
+    Never so few CTAs that a warp adds up more than 4096 tokens: tensor-core sums round towards zero, by up to 2^-24 of the sum of codes
     (7.5 a token) at each of its blocks, which stays below 0.1 % of a mean over equal weights there."""
     tile = 8 if rows <= 8 else (16 if rows <= 16 or D == 256 else 32)
     groups = Hkv * batch * -(-rows // tile)
-    least, most = -(-length // 2048), -(-length // 8)
+    warps, ctas = _KV4_CTAS[D, tile]
+    least, most = -(-length // (256 * warps)), -(-length // 8)
     size = next((n for n, fit in _KV4_CLUSTERS if groups <= fit), 1)
-    if size > 1 and length * D <= 256 * size * _KV4_WARPS[D, tile]:
-        return max(least, min(size, most)), most > 1
-    return min(_KV4_MAX_SPLITS, max(1, min(148 // groups, most), least)), False
+    if size > 1 and length * D <= 256 * size * warps * ctas:
+        return max(least, min(size, most)), warps, most > 1
+    splits, chunk = min(148 * ctas // groups, most), warps
+    if batch > 1 and splits < 4:
+        splits, chunk = min(296 * ctas // groups, most), 4 * warps
+    return min(_KV4_MAX_SPLITS, max(1, splits, least)), chunk, False
 
 
 def kv4_scratch_floats(T: int, batch: int, Hq: int, Hkv: int, D: int, length: int) -> int:
     """Scratch of an ``attn_decode_kv4`` call of T rows (of each of ``batch`` sequences) on tables of ``length`` blocks."""
-    splits, cluster = kv4_splits(T * (Hq // Hkv), Hkv, batch, length, D)
+    splits, _, cluster = kv4_splits(T * (Hq // Hkv), Hkv, batch, length, D)
     return 0 if splits == 1 or cluster else batch * T * Hq * splits * (D + 2)
 
 
@@ -1311,9 +1319,9 @@ def attn_decode_kv4(q, qg, cache, block_table, positions, out, T: int, Hq: int, 
     if T < 1 or rows > KV4_MAX_ROWS or batch > 65535 or Hkv != heads or D != dim or Hq < 1 or Hq % Hkv or window < 0:
         raise KernelError(f"attn_decode_kv4: unsupported shape T={T}, Hq={Hq}, Hkv={Hkv}, D={D}, window={window}")
     n = T * Hq * D
-    cluster = False
+    chunk, cluster = 8, False
     if splits is None:
-        splits, cluster = kv4_splits(rows * (Hq // Hkv), Hkv, batch, length, D)
+        splits, chunk, cluster = kv4_splits(rows * (Hq // Hkv), Hkv, batch, length, D)
     elif not 1 <= splits <= _KV4_MAX_SPLITS:
         raise KernelError(f"attn_decode_kv4: splits={splits} not in 1 .. {_KV4_MAX_SPLITS}")
     need = 0 if splits == 1 or cluster else n * splits // D * (D + 2)
@@ -1326,7 +1334,7 @@ def attn_decode_kv4(q, qg, cache, block_table, positions, out, T: int, Hq: int, 
     _check(_lib().r4dxb_attn_decode_kv4(
         _kv4_rows(q, "q", n, dev), _kv4_rows(qg, "qg", 2 * n, dev) if gated else None, cache.data_ptr(), block_table.data_ptr(), _p(row_slot),
         slots, length, pool, _kv4_ints(positions, "positions", T, dev), scratch.data_ptr() if need else None, _kv4_rows(out, "out", n, dev),
-        rows, batch, Hq, Hkv, D, splits, cluster, window, _status_word(dev), _raw_stream(dev)), "attn_decode_kv4")
+        rows, batch, Hq, Hkv, D, splits, chunk, cluster, window, _status_word(dev), _raw_stream(dev)), "attn_decode_kv4")
     return out
 
 

@@ -82,10 +82,14 @@ def test_splits_fill_the_chip_once_and_clusters_fit_it():
             for batch in (1, 3, 64):
                 for length in (1, 8, 9, 600, 5000):
                     for D, most in ((64, 32), (128, 32), (256, 16)):
-                        s, cluster = K.kv4_splits(rows, heads, batch, length, D)
-                        least = -(-length // 2048)          # 4096 tokens a warp
+                        s, chunk, cluster = K.kv4_splits(rows, heads, batch, length, D)
+                        least = -(-length // (256 * 16))    # 4096 tokens a warp, 16 warps at most
                         groups = heads * batch * -(-rows // most)
-                        assert least <= s <= max(least, min(148, (length + 7) // 8)) and (s == least or s * groups <= 148)
+                        assert least <= s <= max(1, 2 * least, min(296, (length + 7) // 8)) and chunk >= 8
+                        if batch == 1:
+                            assert s <= 2 * least or s * groups <= 296
+                        else:
+                            assert s <= 2 * least or s * groups <= 592
                         assert not cluster or (1 < s <= 16 and groups <= {16: 7, 9: 15}.get(s, 74))
 
 
