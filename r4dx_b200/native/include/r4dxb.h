@@ -132,9 +132,11 @@ int r4dxb_attn_decode_kv4(const void* q, const void* qg, const void* cache, cons
                           int table_length, int pool, const int* positions, float* scratch, void* out, int T, int batch, int Hq, int Hkv, int D,
                           int splits, int chunk, int cluster, int window, int* status, void* stream);
 /* T rows at positions pos0 .. pos0 + T - 1 (already written), causal; window 0 or the number of keys a row sees; key_limit as for
- * r4dxb_attn_prefill_ex; status as for r4dxb_attn_prefill_tc. */
+ * r4dxb_attn_prefill_ex; status as for r4dxb_attn_prefill_tc.  splits (1 .. 64) CTA pairs share the keys of a row tile; above 1 scratch:
+ * splits * T * Hq * (D + 2) floats, 16-byte aligned. */
 int r4dxb_attn_prefill_kv4(const void* q, const void* qg, const void* cache, const int* block_table, int table_length, int pool, void* out, int T,
-                           int Hq, int Hkv, int D, int pos0, int window, const int* key_limit, int* status, void* stream);
+                           int Hq, int Hkv, int D, int pos0, int window, const int* key_limit, int splits, float* scratch, int* status,
+                           void* stream);
 
 /* Sibling projections in one launch of the weight-streaming kernel: `count` (2 or 3) trellis weights of the same K and
  * bit width read the same rows x through the same prologue; weight i writes y[i] [T, n[i]] (no residual). */

@@ -32,6 +32,8 @@
 //
 // The reference's counterpart is a query-tiled WMMA kernel (reference:
 // third_party/libr4d/r4d_attn_prefill_h256_gqa6.hip:112); nothing is shared with it.
+#include <type_traits>
+
 #include "common.cuh"
 #include "kv4.cuh"
 #include "sm100_ptx.cuh"
@@ -63,10 +65,18 @@ struct TcArgs {
   int T, Hq, Hkv, pos0, gated, window;
   int by_head;                 // a pair is two query heads of a kv head over the same rows, else two row tiles of a head
   int* status;
-  // 4-bit cache only
+};
+
+struct Kv4Args : TcArgs {
   kv4::Table table;
   const int* key_limit;        // [T] or null: row t also sees this call's keys up to that position
+  int splits;                  // pairs that share the keys of a row tile; more than one: partial results
+  float* part_acc;             // [splits][T][Hq][D]
+  float2* part_ml;             // [splits][T][Hq]: maximum (log2 domain) and sum
 };
+// (what a kernel is given differs, not only the code: with the longer arguments the fp8 kernels spilled 60 bytes where they spill 24)
+template <bool KV4>
+using Args = std::conditional_t<KV4, Kv4Args, TcArgs>;
 
 struct Control {
   uint64_t q_full, k_full[2], v_full[2], p_full[2];      // those of the first CTA count both
@@ -131,7 +141,7 @@ __device__ __forceinline__ void Kv4ToHalf(uint32_t w, __half2 s, __half2 lo, uin
 //     (NaN keys need nothing: a score that a row does not see is replaced before it is used.)
 //   - pages that the table or pool does not have are NaN keys.
 template <int D, bool KV4>
-__global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) {
   constexpr int NS = D / 64;                          // 64-dimension slabs (one 128-byte swizzle row of fp16 each)
   constexpr int kQBytes = NS * kQRows * 128;
   constexpr int kKBytes = NS * kHalfTile * 128;       // [slab][64 keys][128 B]
@@ -154,11 +164,26 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
   const int q0 = a.by_head ? first_row : first_row + rank * kQRows;
   const int rows = max(0, min(kQRows, a.T - q0));
   const int kv_limit = a.pos0 + a.T;                  // tokens present in the cache
-  const bool limits = KV4 && a.key_limit != nullptr;
+  int splits = 1;
+  const int* key_limit = nullptr;
+  if constexpr (KV4) {
+    splits = a.splits;
+    key_limit = a.key_limit;
+  }
+  const bool limits = KV4 && key_limit != nullptr, partial = KV4 && splits > 1;
   const int kv_end = limits ? kv_limit : a.pos0 + min(a.T, first_row + (a.by_head ? kQRows : 2 * kQRows));      // first key no row of the pair may see
   const int kv_first = a.window > 0 ? max(0, a.pos0 + first_row - a.window + 1) : 0;
-  const int tile0 = kv_first / kKvTile;
-  const int ntiles = (kv_end + kKvTile - 1) / kKvTile - tile0;              // at least 1
+  // (a pair that shares the keys with others has one part of their tiles, `per` of them at most)
+  const int tiles = (kv_end + kKvTile - 1) / kKvTile - kv_first / kKvTile;  // at least 1
+  const int per = KV4 ? (tiles + splits - 1) / splits : tiles, skip = KV4 ? static_cast<int>(blockIdx.z) * per : 0;
+  const int tile0 = kv_first / kKvTile + skip, ntiles = min(per, tiles - skip);
+  if constexpr (KV4) {
+    if (ntiles <= 0) {                                // no tile is left for this part: no row sees any of it
+      for (int r = threadIdx.x; r < rows; r += kThreads)
+        a.part_ml[(static_cast<size_t>(blockIdx.z) * a.T + q0 + r) * a.Hq + hq] = make_float2(-INFINITY, 0.f);
+      return;
+    }
+  }
 
   if (threadIdx.x == 0) {
     ptx::MbarInit(&ctl->q_full, 2 * kConvWarps);
@@ -357,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
                   const int first = a.by_head ? first_row : first_row + peer * kQRows;
                   const uint32_t flags = ptx::MapToRank(ptx::SmemAddr(&ctl->nan_groups[0]), peer);
                   for (int r = 0; r < kQRows && first + r < a.T; ++r) {
-                    const int qpos = a.pos0 + first + r, last = limits ? max(qpos, a.key_limit[first + r]) : qpos;
+                    const int qpos = a.pos0 + first + r, last = limits ? max(qpos, key_limit[first + r]) : qpos;
                     if (kp <= last && (a.window == 0 || kp > qpos - a.window)) OrRemote(flags + 4 * r, 1u << vgroup);
                   }
                 }
@@ -453,8 +478,8 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
       }
     }
     // the output gates of this CTA's rows, into K's buffers once the last scores have read them
-    if (ok && a.gated) ok = ptx::WarpMbarWait(&ctl->s_full[(ntiles - 1) & 1], static_cast<uint32_t>((ntiles - 1) >> 1) & 1u, abort_flag, 13);
-    if (ok && a.gated) {
+    if (ok && a.gated && !partial) ok = ptx::WarpMbarWait(&ctl->s_full[(ntiles - 1) & 1], static_cast<uint32_t>((ntiles - 1) >> 1) & 1u, abort_flag, 13);
+    if (ok && a.gated && !partial) {
 #pragma unroll 4
       for (int i = tid; i < rows * (D / 8); i += kConvThreads) {
         const int r = i / (D / 8), c = i % (D / 8);
@@ -520,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
     // ---------------- softmax warps: thread = query row = TMEM lane, two warps share a row ----------------
     const int half = warp >> 2, r = (warp & 3) * 32 + lane;
     const int qp = a.pos0 + q0 + r;                               // position of this row's query
-    const int last_key = limits && r < rows ? max(qp, min(a.key_limit[q0 + r], kv_limit - 1)) : qp;
+    const int last_key = limits && r < rows ? max(qp, min(key_limit[q0 + r], kv_limit - 1)) : qp;
     const uint32_t t_lane = tbase + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t p_full = ptx::MapToRank(ptx::SmemAddr(&ctl->p_full[0]), 0);
     float m_used = -INFINITY, l_run = 0.f;
@@ -612,9 +637,33 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
     }
     // ---------------- epilogue: O / l, output gate, bf16 rows; each warp half of the columns ----------------
     const float l = l_run + exchange(ntiles & 1, l_run);
-    if (ok && a.gated) ok = ptx::WarpMbarWait(&ctl->gates, 0, abort_flag, 10);
+    if (ok && a.gated && !partial) ok = ptx::WarpMbarWait(&ctl->gates, 0, abort_flag, 10);
     if (ok) ok = ptx::WarpMbarWait(&ctl->o_final, 0, abort_flag, 9);
-    if (ok) {
+    if constexpr (KV4) {
+      if (partial) {
+        // this share's sums as they are (NaN where a wait ran out), joined by a kernel of their own
+        const size_t at = (static_cast<size_t>(blockIdx.z) * a.T + q0 + r) * a.Hq + hq;
+        if (r < rows && half == 0) a.part_ml[at] = make_float2(ok ? m_used : 0.f, ok ? l : __uint_as_float(0x7fc00000u));
+        if (ok) {
+          ptx::TcFenceAfter();
+          const int nan_groups = ctl->nan_groups[r];
+          float* dst = a.part_acc + at * D + half * (D / 2);
+  #pragma unroll 1
+          for (int c0 = 0; c0 < D / 2; c0 += 32) {
+            uint32_t o[32];
+            ptx::TmemLoad32x32(t_lane + half * (D / 2) + c0, o);
+            ptx::TmemLoadWait();
+            const bool nan = nan_groups >> ((half * (D / 2) + c0) >> 6) & 1;
+            if (r < rows) {
+  #pragma unroll
+              for (int v = 0; v < 8; ++v)
+                *reinterpret_cast<uint4*>(dst + c0 + 4 * v) = nan ? make_uint4(0x7fc00000u, 0x7fc00000u, 0x7fc00000u, 0x7fc00000u) : make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+            }
+          }
+        }
+      }
+    }
+    if (ok && !partial) {
       ptx::TcFenceAfter();
       const float inv = (l > 0.f ? 1.f / l : 0.f) * (KV4 ? 1.f : a.v_descale[hkv]);
       const int nan_groups = KV4 ? ctl->nan_groups[r] : 0;
@@ -675,8 +724,41 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(TcArgs a) {
   }
 }
 
+// The shares of split keys joined: D / 4 threads a row, its gate and its rounding.
+template <int D>
+__global__ void __launch_bounds__(256) JoinKv4Kernel(Kv4Args a) {
+  constexpr int kRow = D / 4;
+  const long long row = static_cast<long long>(blockIdx.x) * (256 / kRow) + threadIdx.x / kRow, rows = static_cast<long long>(a.T) * a.Hq;
+  if (row >= rows) return;
+  const int col = threadIdx.x % kRow * 4;
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int z = 0; z < a.splits; ++z) m = fmaxf(m, a.part_ml[z * rows + row].x);
+  for (int z = 0; z < a.splits; ++z) {
+    const float2 x = a.part_ml[z * rows + row];
+    if (x.x == -INFINITY && x.y == 0.f) continue;               // (no key of that share is seen; it may have written nothing else)
+    const float f = x.x == -INFINITY ? 1.f : exp2f(x.x - m);    // (-inf with a sum: its scores were NaN, and so is the sum)
+    const float4 v = __ldcs(reinterpret_cast<const float4*>(a.part_acc + (z * rows + row) * D + col));
+    l = fmaf(f, x.y, l);
+    o.x = fmaf(f, v.x, o.x);
+    o.y = fmaf(f, v.y, o.y);
+    o.z = fmaf(f, v.z, o.z);
+    o.w = fmaf(f, v.w, o.w);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  if (a.gated) {
+    const uint32_t* gate = reinterpret_cast<const uint32_t*>(a.qg + row * 2 * D + D + col);
+    o.x *= Sigmoid(BfLo(gate[0]));
+    o.y *= Sigmoid(BfHi(gate[0]));
+    o.z *= Sigmoid(BfLo(gate[1]));
+    o.w *= Sigmoid(BfHi(gate[1]));
+  }
+  *reinterpret_cast<uint2*>(a.out + row * D + col) = make_uint2(PackBf16(o.x, o.y), PackBf16(o.z, o.w));
+}
+
 template <int D, bool KV4 = false>
-int LaunchTc(const TcArgs& a, cudaStream_t s) {
+int LaunchTc(const Args<KV4>& a, cudaStream_t s) {
   constexpr int NS = D / 64;
   // kClusterAlone: so much of an SM's shared memory that no other CTA shares the SM whose cluster may wait with tensor memory in its
   // hands (sm100_ptx.cuh).  More would cost L1: 8192 rows of 32 heads of 128 columns take 808 us with 131 KB, 821 with 156, 878 with 227.
@@ -687,6 +769,7 @@ int LaunchTc(const TcArgs& a, cudaStream_t s) {
   if (e != cudaSuccess) return static_cast<int>(e);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = a.by_head ? dim3(a.Hq, (a.T + kQRows - 1) / kQRows) : dim3(2 * a.Hq, (a.T + 2 * kQRows - 1) / (2 * kQRows));
+  if constexpr (KV4) cfg.gridDim.z = a.splits;
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -698,6 +781,13 @@ int LaunchTc(const TcArgs& a, cudaStream_t s) {
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, kern, a);
   if (e != cudaSuccess) return static_cast<int>(e);
+  if constexpr (KV4) {
+    if (a.splits > 1) {
+      ++g_launch_count;
+      constexpr int kPer = 256 / (D / 4);
+      JoinKv4Kernel<D><<<static_cast<unsigned>((static_cast<long long>(a.T) * a.Hq + kPer - 1) / kPer), 256, 0, s>>>(a);
+    }
+  }
   return FinishLaunch();
 }
 
@@ -712,7 +802,7 @@ extern "C" int r4dxb_attn_prefill_tc(const void* q, const void* qg, const void* 
                                      const float* k_descale, const float* v_descale, void* out, int T, int Hq, int Hkv, int D,
                                      int pos0, int flags, int* status, void* stream) {
   if (T < 1 || Hq % Hkv || (D != 256 && D != 128)) return R4DXB_BAD_ARG;
-  TcArgs a = {};
+  TcArgs a;
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.qg = static_cast<const __nv_bfloat16*>(qg);
   a.cache = static_cast<const uint8_t*>(cache);
@@ -727,16 +817,19 @@ extern "C" int r4dxb_attn_prefill_tc(const void* q, const void* qg, const void* 
   return D == 256 ? LaunchTc<256>(a, s) : LaunchTc<128>(a, s);
 }
 
-/* The same over the 4-bit cache (kv4.cuh), head dimensions 64, 128 and 256; key_limit as for r4dxb_attn_prefill_ex. */
+/* The same over the 4-bit cache (kv4.cuh), head dimensions 64, 128 and 256; key_limit as for r4dxb_attn_prefill_ex.  splits > 1: the keys of a row
+   tile are shared by so many pairs; scratch: splits * T * Hq * (D + 2) floats, 16-byte aligned. */
 extern "C" int r4dxb_attn_prefill_kv4(const void* q, const void* qg, const void* cache, const int* block_table, int table_length, int pool, void* out,
-                                      int T, int Hq, int Hkv, int D, int pos0, int window, const int* key_limit, int* status, void* stream) {
+                                      int T, int Hq, int Hkv, int D, int pos0, int window, const int* key_limit, int splits, float* scratch, int* status,
+                                      void* stream) {
+  if (splits < 1 || splits > 64 || (splits > 1 && scratch == nullptr) || reinterpret_cast<uintptr_t>(scratch) & 15) return R4DXB_BAD_ARG;
   if (T < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || (D != 64 && D != 128 && D != 256) || pos0 < 0 || pos0 > 0x7fffffff - T - kKvTile || window < 0 ||
       table_length < 1 || pool < 1 || q == nullptr || cache == nullptr || block_table == nullptr || out == nullptr)
     return R4DXB_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out)) & 15 || reinterpret_cast<uintptr_t>(qg) & 3)
     return R4DXB_BAD_ARG;
   if (Hq > 32767 || (T + kQRows - 1) / kQRows > 65535) return R4DXB_TOO_LARGE;
-  TcArgs a = {};
+  Kv4Args a = {};
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.qg = static_cast<const __nv_bfloat16*>(qg);
   a.cache = static_cast<const uint8_t*>(cache);
@@ -746,6 +839,9 @@ extern "C" int r4dxb_attn_prefill_kv4(const void* q, const void* qg, const void*
   a.status = status;
   a.table = {block_table, table_length, pool};
   a.key_limit = key_limit;
+  a.splits = splits;
+  a.part_acc = scratch;
+  a.part_ml = reinterpret_cast<float2*>(scratch + static_cast<size_t>(splits) * T * Hq * D);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return D == 256 ? LaunchTc<256, true>(a, s) : (D == 128 ? LaunchTc<128, true>(a, s) : LaunchTc<64, true>(a, s));
 }

@@ -1164,7 +1164,7 @@ def q4x_hc_gate(h, norm_w, w_down_inject, w_up, mid, injv, rstd, x, T: int, hc: 
 register_cuda_sig("r4dxb_attn_precore_kv4", _I, [_P] * 8 + [_I] * 3 + [_P, _P] + [_I] * 5 + [_F, _F, _I, _P])
 register_cuda_sig("r4dxb_kv4_read", _I, [_P] * 3 + [_I] * 3 + [_P] * 3 + [_I] * 3 + [_P])
 register_cuda_sig("r4dxb_attn_decode_kv4", _I, [_P] * 5 + [_I] * 3 + [_P] * 3 + [_I] * 9 + [_P, _P])
-register_cuda_sig("r4dxb_attn_prefill_kv4", _I, [_P] * 4 + [_I] * 2 + [_P] + [_I] * 6 + [_P] * 3)
+register_cuda_sig("r4dxb_attn_prefill_kv4", _I, [_P] * 4 + [_I] * 2 + [_P] + [_I] * 6 + [_P, _I] + [_P] * 3)
 
 KV4_MAX_ROWS = 32           # rows of one sequence that attn_decode_kv4 takes
 _KV4_MAX_SPLITS = 256
@@ -1338,17 +1338,32 @@ def attn_decode_kv4(q, qg, cache, block_table, positions, out, T: int, Hq: int, 
     return out
 
 
+@functools.lru_cache(maxsize=4096)
+def kv4_prefill_splits(T: int, Hq: int, Hkv: int, pos0: int, window: int) -> int:
+    """CTA pairs that share the keys of a row tile: few rows leave SMs idle that a long context keeps busy; eight tiles of 128 keys or more
+    each."""
+    paired = Hq // Hkv % 2 == 0              # two heads, else two row tiles to a pair
+    ctas = Hq * -(-T // 128) if paired else 2 * Hq * -(-T // 256)
+    tiles = (pos0 + T - (max(0, pos0 - window + 1) // 128 * 128 if window else 0) + 127) // 128
+    return max(1, min(148 // ctas, tiles // 8, 64))
+
+
 def attn_prefill_kv4(q, qg, cache, block_table, out, T: int, Hq: int, Hkv: int, D: int, pos0: int, gated: bool = True, window: int = 0,
-                     key_limit: Optional[torch.Tensor] = None):
+                     key_limit: Optional[torch.Tensor] = None, splits: Optional[int] = None):
     """Causal attention of T rows at positions pos0 .. over a 4-bit cache that already holds them (``attn_prefill`` for that cache, on
     tcgen05 for every head dimension, key limits included).  Keys and values are widened to fp16 values, in which magnitudes below 6e-5
-    lose bits."""
+    lose bits.  ``splits``: CTA pairs that share the keys of a row tile (by ``kv4_prefill_splits`` unless given)."""
     dev, slots, length, pool, heads, dim = _kv4_pool(cache, block_table, None, T)
     if T < 1 or Hkv != heads or D != dim or Hq < 1 or Hq % Hkv or window < 0 or pos0 < 0 or pos0 + T > 1 << 30:
         raise KernelError(f"attn_prefill_kv4: unsupported shape T={T}, Hq={Hq}, Hkv={Hkv}, D={D}, pos0={pos0}, window={window}")
     n = T * Hq * D
+    if splits is None:
+        splits = kv4_prefill_splits(T, Hq, Hkv, pos0, window)
+    elif not 1 <= splits <= 64:
+        raise KernelError(f"attn_prefill_kv4: splits={splits} not in 1 .. 64")
+    scratch = torch.empty(splits * n // D * (D + 2), dtype=torch.float32, device=cache.device) if splits > 1 else None
     _check(_lib().r4dxb_attn_prefill_kv4(
         _kv4_rows(q, "q", n, dev), _kv4_rows(qg, "qg", 2 * n, dev) if gated else None, cache.data_ptr(), block_table.data_ptr(), length, pool,
         _kv4_rows(out, "out", n, dev), T, Hq, Hkv, D, pos0, window, None if key_limit is None else _kv4_ints(key_limit, "key_limit", T, dev),
-        _status_word(dev), _raw_stream(dev)), "attn_prefill_kv4")
+        splits, _p(scratch), _status_word(dev), _raw_stream(dev)), "attn_prefill_kv4")
     return out

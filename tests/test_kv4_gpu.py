@@ -264,20 +264,22 @@ def score_slack(q, k, v):
 
 
 PREFILL = [
-    # D, Hq, Hkv, T, pos0, window, gated
-    (256, 6, 1, 1, 0, 0, True), (256, 24, 4, 333, 0, 0, True), (256, 3, 1, 129, 127, 0, True), (128, 8, 2, 260, 500, 130, False),
-    (128, 5, 5, 257, 300, 64, True), (64, 32, 8, 100, 29, 0, False), (64, 3, 3, 300, 1000, 17, True), (256, 2, 2, 17, 2000, 0, False),
-    (64, 4, 2, 513, 0, 0, True), (128, 2, 1, 40, 16, 1, False), (256, 4, 2, 128, 128, 0, False),
+    # D, Hq, Hkv, T, pos0, window, gated, splits
+    (256, 6, 1, 1, 0, 0, True, None), (256, 24, 4, 333, 0, 0, True, None), (256, 3, 1, 129, 127, 0, True, None), (128, 8, 2, 260, 500, 130, False, None),
+    (128, 5, 5, 257, 300, 64, True, None), (64, 32, 8, 100, 29, 0, False, None), (64, 3, 3, 300, 1000, 17, True, None), (256, 2, 2, 17, 2000, 0, False, None),
+    (64, 4, 2, 513, 0, 0, True, None), (128, 2, 1, 40, 16, 1, False, None), (256, 4, 2, 128, 128, 0, False, None),
+    (256, 24, 4, 16, 3000, 0, True, None), (128, 8, 2, 130, 2500, 0, False, 4), (64, 6, 2, 140, 900, 300, True, 5), (256, 2, 1, 300, 200, 0, True, 7),
 ]
 
 
-@pytest.mark.parametrize("D,Hq,Hkv,T,pos0,window,gated", PREFILL)
-def test_prefill_attention(K, D, Hq, Hkv, T, pos0, window, gated):
+@pytest.mark.parametrize("D,Hq,Hkv,T,pos0,window,gated,splits", PREFILL)
+def test_prefill_attention(K, D, Hq, Hkv, T, pos0, window, gated, splits):
     g = torch.Generator().manual_seed(T + pos0)
     pool = Pool(D, Hkv, [pos0 + T], seed=T)
     q, qg = torch.randn(T, Hq, D, generator=g).to(BF), torch.randn(T, Hq, 2 * D, generator=g).to(BF)
     out = torch.full((T, Hq, D), NAN, dtype=BF, device="cuda")
-    K.attn_prefill_kv4(q.cuda(), qg.cuda() if gated else None, pool.cache.cuda(), pool.tables[0].cuda(), out, T, Hq, Hkv, D, pos0, gated, window)
+    K.attn_prefill_kv4(q.cuda(), qg.cuda() if gated else None, pool.cache.cuda(), pool.tables[0].cuda(), out, T, Hq, Hkv, D, pos0, gated, window,
+                       splits=splits)
     K.check_gemm_status(out.device)
     want = attention(q, pool.k[0], pool.v[0], torch.arange(pos0, pos0 + T), window)
     if gated:
@@ -321,9 +323,10 @@ def test_nan_keys_and_values_reach_the_rows_that_see_them_only(K, D):
     nan[75:75 + window, 2:, :64] = True
     cache, table = pool.cache.cuda(), pool.tables[0].cuda()
     out = torch.empty(n, Hq, D, dtype=BF, device="cuda")
-    K.attn_prefill_kv4(q.cuda(), None, cache, table, out, n, Hq, Hkv, D, 0, False, window)
-    assert torch.equal(out.cpu().isnan(), nan)
-    check(out.cpu().masked_fill(nan, 0.0), want.masked_fill(nan, 0.0), pool.v[0], slack=score_slack(q, pool.k[0], pool.v[0]))
+    for splits in (1, 2):
+        K.attn_prefill_kv4(q.cuda(), None, cache, table, out, n, Hq, Hkv, D, 0, False, window, splits=splits)
+        assert torch.equal(out.cpu().isnan(), nan), splits
+        check(out.cpu().masked_fill(nan, 0.0), want.masked_fill(nan, 0.0), pool.v[0], slack=score_slack(q, pool.k[0], pool.v[0]))
     for first in (64, 68, 72, 96, 104):
         r = slice(first, first + 8)
         K.attn_decode_kv4(q[r].contiguous().cuda(), None, cache, table, at[r].int().cuda(), out[:8], 8, Hq, Hkv, D, False, window)
@@ -447,7 +450,7 @@ def test_refusals(K):
            (decode, dict(positions=pos.long())), (decode, dict(row_slot=pos)), (decode, dict(qg=q)), (decode, dict(qg=None)), (decode, dict(out=out[:, :2])),
            (decode, dict(splits=3, scratch=e(8, dtype=torch.float32))), (decode, dict(splits=0)), (decode, dict(splits=1000)),
            (prefill, dict(D=64)), (prefill, dict(T=2)), (prefill, dict(pos0=-1)), (prefill, dict(q=odd)), (prefill, dict(window=-2)),
-           (prefill, dict(key_limit=pos.long())), (prefill, dict(cache=cache.transpose(0, 1))), (prefill, dict(T=0)),
+           (prefill, dict(key_limit=pos.long())), (prefill, dict(cache=cache.transpose(0, 1))), (prefill, dict(T=0)), (prefill, dict(splits=0)), (prefill, dict(splits=65)),
            (precore, dict(rotary_dim=3)), (precore, dict(rotary_dim=130)), (precore, dict(q_stride=100)), (precore, dict(k=odd[:, :2])), (precore, dict(T=2)),
            (precore, dict(q_norm=e(64))), (precore, dict(Hq=0))]
     for f, kw in bad:
