@@ -102,6 +102,12 @@ __device__ __forceinline__ float Exp2Approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// without the division's dozen instructions (its result is off by 2^-22)
+__device__ __forceinline__ float SigmoidApprox(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + __expf(-x)));
+  return y;
+}
 // offset of 16-byte chunk c of row r inside a [rows][128 B] tile in the K-major 128-byte-swizzled UMMA layout
 __device__ __forceinline__ int Sw128(int r, int c) { return (r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4); }
 
@@ -478,8 +484,36 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
       }
     }
     // the output gates of this CTA's rows, into K's buffers once the last scores have read them
-    if (ok && a.gated && !partial) ok = ptx::WarpMbarWait(&ctl->s_full[(ntiles - 1) & 1], static_cast<uint32_t>((ntiles - 1) >> 1) & 1u, abort_flag, 13);
-    if (ok && a.gated && !partial) {
+    if constexpr (KV4) {
+      // (16-byte aligned; eight loads a thread in flight, the first ones before the wait)
+      if (ok && a.gated && !partial) {
+        constexpr int kAhead = 8, kPieces = kQRows * (D / 8);
+        const __nv_bfloat16* gates = a.qg + (static_cast<size_t>(q0) * a.Hq + hq) * 2 * D + D;
+        const size_t row_step = static_cast<size_t>(a.Hq) * 2 * D;
+        uint4 g[kAhead];
+        auto fetch = [&](int i0) {
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) {
+            const int i = i0 + k * kConvThreads, r = i / (D / 8);
+            g[k] = i < kPieces && r < rows ? __ldg(reinterpret_cast<const uint4*>(gates + r * row_step + i % (D / 8) * 8)) : make_uint4(0u, 0u, 0u, 0u);
+          }
+        };
+        fetch(tid);
+        ok = ptx::WarpMbarWait(&ctl->s_full[(ntiles - 1) & 1], static_cast<uint32_t>((ntiles - 1) >> 1) & 1u, abort_flag, 13);
+        for (int i0 = tid; i0 < kPieces && ok; i0 += kAhead * kConvThreads) {
+          if (i0 != tid) fetch(i0);
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) {
+            const int i = i0 + k * kConvThreads;
+            if (i < kPieces) *reinterpret_cast<uint4*>(Ks + GateChunk<D>(i / (D / 8), i % (D / 8))) = g[k];
+          }
+        }
+        __syncwarp();
+        if (ok && lane == 0) ptx::MbarArrive(&ctl->gates);
+      }
+    } else {
+    if (ok && a.gated) ok = ptx::WarpMbarWait(&ctl->s_full[(ntiles - 1) & 1], static_cast<uint32_t>((ntiles - 1) >> 1) & 1u, abort_flag, 13);
+    if (ok && a.gated) {
 #pragma unroll 4
       for (int i = tid; i < rows * (D / 8); i += kConvThreads) {
         const int r = i / (D / 8), c = i % (D / 8);
@@ -495,6 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
       }
       __syncwarp();
       if (lane == 0) ptx::MbarArrive(&ctl->gates);
+    }
     }
   } else if (warp == kMmaWarp) {
     // ---------------- MMA issuer (one thread of the first CTA) ----------------
@@ -693,8 +728,8 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
               const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
-                x[2 * c] *= Sigmoid(BfLo(gw[c]));
-                x[2 * c + 1] *= Sigmoid(BfHi(gw[c]));
+                x[2 * c] *= KV4 ? SigmoidApprox(BfLo(gw[c])) : Sigmoid(BfLo(gw[c]));
+                x[2 * c + 1] *= KV4 ? SigmoidApprox(BfHi(gw[c])) : Sigmoid(BfHi(gw[c]));
               }
             }
             *reinterpret_cast<uint4*>(stage + (c0 + 8 * v) * 2) =
@@ -826,7 +861,7 @@ extern "C" int r4dxb_attn_prefill_kv4(const void* q, const void* qg, const void*
   if (T < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || (D != 64 && D != 128 && D != 256) || pos0 < 0 || pos0 > 0x7fffffff - T - kKvTile || window < 0 ||
       table_length < 1 || pool < 1 || q == nullptr || cache == nullptr || block_table == nullptr || out == nullptr)
     return R4DXB_BAD_ARG;
-  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out)) & 15 || reinterpret_cast<uintptr_t>(qg) & 3)
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(qg)) & 15)
     return R4DXB_BAD_ARG;
   if (Hq > 32767 || (T + kQRows - 1) / kQRows > 65535) return R4DXB_TOO_LARGE;
   Kv4Args a = {};

@@ -1338,14 +1338,44 @@ def attn_decode_kv4(q, qg, cache, block_table, positions, out, T: int, Hq: int, 
     return out
 
 
+# us of a tile of 128 keys in a CTA of the prefill kernel by head dimension, and of what a CTA and the joining kernel take besides
+_KV4_TILE_US = {64: 1.4, 128: 1.5, 256: 2.2}
+_KV4_START_US, _KV4_JOIN_US = 5.0, 4.0
+KV4_FEW_ROWS_WORK = 6144
+
+
 @functools.lru_cache(maxsize=4096)
-def kv4_prefill_splits(T: int, Hq: int, Hkv: int, pos0: int, window: int) -> int:
-    """CTA pairs that share the keys of a row tile: few rows leave SMs idle that a long context keeps busy; eight tiles of 128 keys or more
-    each."""
-    paired = Hq // Hkv % 2 == 0              # two heads, else two row tiles to a pair
-    ctas = Hq * -(-T // 128) if paired else 2 * Hq * -(-T // 256)
-    tiles = (pos0 + T - (max(0, pos0 - window + 1) // 128 * 128 if window else 0) + 127) // 128
-    return max(1, min(148 // ctas, tiles // 8, 64))
+def kv4_prefill_splits(T: int, Hq: int, Hkv: int, D: int, pos0: int, window: int) -> int:
+    """CTA pairs that share the keys of a row tile (0: the decode kernel takes the call): the fewest us by waves of the 148 SMs.
+
+    Few rows leave SMs idle that a long context keeps busy (24 heads over 4 of 256, 128 rows after 29000 keys: 500 us alone, 109 in six), and
+    so does a second wave that is part empty.  Up to 32 rows the decode kernel is faster where its row tiles are few enough (kv heads x row
+    tiles x D up to 6144) or the context short: 16 rows after 29000 keys 69 us against 95, 32 rows 129 against 97, 32 after 1000 17 against 30."""
+    if T <= KV4_MAX_ROWS:
+        rows = T * (Hq // Hkv)
+        tile = 8 if rows <= 8 else (16 if rows <= 16 or D == 256 else 32)
+        if pos0 + T <= 4096 or Hkv * -(-rows // tile) * D <= KV4_FEW_ROWS_WORK:
+            return 0
+    tiles = lambda first, end: -(-end // 128) - (max(0, first - window + 1) // 128 if window else 0)  # noqa: E731
+    step = 128 if Hq // Hkv % 2 == 0 else 256             # rows of a pair: two heads, else two row tiles
+    pairs = -(-T // step)
+    ctas = Hq * pairs * (step // 128)
+    short, long = tiles(pos0, pos0 + min(T, step)), tiles(pos0 + (pairs - 1) * step, pos0 + T)
+    even = 5 * short >= 4 * long
+    best, best_us = 1, None
+    for s in (1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 24, 32, 48, 64):
+        if s > 1 and (2 * s > long or s * T * Hq * D > 1 << 26):
+            break                                         # (two tiles a pair at least; 256 MB of partial sums)
+        n, us = ctas * s, -(-long // s) * _KV4_TILE_US[D]
+        if even or n <= 148:
+            us = -(-n // 148) * (us + _KV4_START_US)
+        else:                                             # (long row tiles come first, short ones fill the gaps)
+            us = n / 148 * ((short + long) / 2 / s * _KV4_TILE_US[D] + _KV4_START_US) + us / 2
+        if s > 1:
+            us += _KV4_JOIN_US + s * T * Hq * D * 8 / 5e6
+        if best_us is None or us < best_us - 1e-9:
+            best, best_us = s, us
+    return best
 
 
 def attn_prefill_kv4(q, qg, cache, block_table, out, T: int, Hq: int, Hkv: int, D: int, pos0: int, gated: bool = True, window: int = 0,
@@ -1358,7 +1388,11 @@ def attn_prefill_kv4(q, qg, cache, block_table, out, T: int, Hq: int, Hkv: int, 
         raise KernelError(f"attn_prefill_kv4: unsupported shape T={T}, Hq={Hq}, Hkv={Hkv}, D={D}, pos0={pos0}, window={window}")
     n = T * Hq * D
     if splits is None:
-        splits = kv4_prefill_splits(T, Hq, Hkv, pos0, window)
+        splits = kv4_prefill_splits(T, Hq, Hkv, D, pos0, window)
+        if not splits and key_limit is None:
+            positions = torch.arange(pos0, pos0 + T, dtype=torch.int32, device=cache.device)
+            return attn_decode_kv4(q, qg, cache, block_table, positions, out, T, Hq, Hkv, D, gated, window)
+        splits = splits or 1
     elif not 1 <= splits <= 64:
         raise KernelError(f"attn_prefill_kv4: splits={splits} not in 1 .. 64")
     scratch = torch.empty(splits * n // D * (D + 2), dtype=torch.float32, device=cache.device) if splits > 1 else None

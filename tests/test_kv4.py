@@ -107,3 +107,16 @@ def test_four_stream_family_keeps_its_fp8_cache():
     from r4dx_b200.cli.loader import _load_qwen4_exp
     with pytest.raises(SystemExit, match="--kv-cache int4"):
         _load_qwen4_exp(SimpleNamespace(tp=1, kv_cache="int4"), None, {}, "m", "m", "cpu")
+
+
+def test_prefill_shares_fill_the_chip():
+    from r4dx_b200.ops import kernels as K
+    for D in (64, 128, 256):
+        for Hq, Hkv in ((24, 4), (32, 8), (3, 1), (16, 8)):
+            for T in (1, 9, 32, 33, 128, 333, 1024, 8192):
+                for pos0 in (0, 100, 4000, 29000, 250000):
+                    for window in (0, 64, 1024):
+                        s = K.kv4_prefill_splits(T, Hq, Hkv, D, pos0, window)
+                        keys = min(window + T, pos0 + T) if window else pos0 + T
+                        assert 0 <= s <= 64 and (s > 0 or T <= K.KV4_MAX_ROWS) and (s < 2 or s * 256 <= keys + 256 and s * T * Hq * D <= 1 << 26)
+    assert K.kv4_prefill_splits(8192, 24, 4, 256, 0, 0) == 1 and K.kv4_prefill_splits(128, 24, 4, 256, 29000, 0) >= 4
