@@ -437,25 +437,42 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
     load_k(0);
     {
       const float scale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f * (KV4 ? 1.f : a.k_descale[hkv]);
-#pragma unroll 4
-      for (int i = tid; i < kQRows * (D / 8); i += kConvThreads) {
-        const int r = i / (D / 8), c = i % (D / 8);
-        uint4 o = make_uint4(0u, 0u, 0u, 0u);
-        if (r < rows) {
-          const uint4 v = *reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(q0 + r) * a.Hq + hq) * D + c * 8);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          uint32_t h[4];
+      auto widen = [&](const uint4& v) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t h[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const __half2 p = __floats2half2_rn(BfLo(w[j]) * scale, BfHi(w[j]) * scale);
-            h[j] = *reinterpret_cast<const uint32_t*>(&p);
-          }
-          if constexpr (KV4)                    // channels 0 4 1 5 2 6 3 7
-            o = make_uint4(__byte_perm(h[0], h[2], 0x5410), __byte_perm(h[0], h[2], 0x7632), __byte_perm(h[1], h[3], 0x5410), __byte_perm(h[1], h[3], 0x7632));
-          else
-            o = make_uint4(h[0], h[1], h[2], h[3]);
+        for (int j = 0; j < 4; ++j) {
+          const __half2 p = __floats2half2_rn(BfLo(w[j]) * scale, BfHi(w[j]) * scale);
+          h[j] = *reinterpret_cast<const uint32_t*>(&p);
         }
-        *reinterpret_cast<uint4*>(Qs + (c >> 3) * (kQRows * 128) + Sw128(r, c & 7)) = o;
+        if constexpr (KV4)                      // channels 0 4 1 5 2 6 3 7
+          return make_uint4(__byte_perm(h[0], h[2], 0x5410), __byte_perm(h[0], h[2], 0x7632), __byte_perm(h[1], h[3], 0x5410), __byte_perm(h[1], h[3], 0x7632));
+        else
+          return make_uint4(h[0], h[1], h[2], h[3]);
+      };
+      if constexpr (KV4) {
+        constexpr int kAhead = 8;               // loads of a thread in flight
+        for (int i0 = tid; i0 < kQRows * (D / 8); i0 += kAhead * kConvThreads) {
+          uint4 v[kAhead];
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) {
+            const int i = i0 + k * kConvThreads, r = i / (D / 8), c = i % (D / 8);
+            v[k] = r < rows ? __ldg(reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(q0 + r) * a.Hq + hq) * D + c * 8)) : make_uint4(0u, 0u, 0u, 0u);
+          }
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) {
+            const int i = i0 + k * kConvThreads, r = i / (D / 8), c = i % (D / 8);
+            if (r < kQRows) *reinterpret_cast<uint4*>(Qs + (c >> 3) * (kQRows * 128) + Sw128(r, c & 7)) = widen(v[k]);
+          }
+        }
+      } else {
+#pragma unroll 4
+        for (int i = tid; i < kQRows * (D / 8); i += kConvThreads) {
+          const int r = i / (D / 8), c = i % (D / 8);
+          uint4 o = make_uint4(0u, 0u, 0u, 0u);
+          if (r < rows) o = widen(*reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(q0 + r) * a.Hq + hq) * D + c * 8));
+          *reinterpret_cast<uint4*>(Qs + (c >> 3) * (kQRows * 128) + Sw128(r, c & 7)) = o;
+        }
       }
       ptx::FenceProxyAsyncShared();
       __syncwarp();
@@ -741,7 +758,8 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
       if (r < rows) {
         ptx::BulkStore(a.out + (static_cast<size_t>(q0 + r) * a.Hq + hq) * D + half * (D / 2), ptx::SmemAddr(stage), kHalfRow);
         ptx::BulkStoreCommit();
-        ptx::BulkStoreWait();
+        if constexpr (KV4) ptx::BulkStoreWaitRead();          // (the rows have left shared memory; they arrive before the kernel ends)
+        else ptx::BulkStoreWait();
       }
     }
   }
