@@ -246,18 +246,35 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
     const int vword = D == 256 ? (cw & 3) * 2 + (vsub & 1) + (vsub >> 1) * 8 : (cw & 3) * (VWords / 4) + vsub;
     const int vtok = (cw >> 2) * kHalfTile + lane % VUnits * VT, vgroup = (rank * VWords + vword) >> 3;
     uint32_t kcodes[NJ], kpairs[NG], vcodes[VT], vpairs[VT];
+    // the blocks of the next tiles' keys and values are looked up a tile ahead: an address that waits for its table entry held a warp up
+    // for a quarter of a tile's time
+    auto block_of = [&](int j, int first) {
+      if constexpr (KV4) return a.table.BlockAt(((tile0 + j) * kKvTile + first) >> 4);
+      else return 0;
+    };
+    const int kfirst = rank * kHalfTile + kkey;
+    int kblk = block_of(0, kfirst), vblk = block_of(0, vtok);
+    // where a thread's words lie in a block: the same in every tile, since tiles begin with blocks
+    int kword[2] = {}, vwords[VT] = {};
+    if constexpr (KV4) {
+      kword[0] = kv4::Word<D, false>(kfirst & 15, kc);
+      kword[1] = kv4::Word<D, false>(kfirst & 15, D == 256 ? 16 + kc : kc);
+#pragma unroll
+      for (int t = 0; t < VT; ++t) vwords[t] = kv4::Word<D, true>((vtok & 15) + t, rank * VWords + vword);
+    }
+    const int kpair = 2 * D + (kfirst & 15) * NG, vpair = kv4::Shape<D>::kPart / 4 + 2 * D + (vtok & 15) * NG + vgroup;
     const uint32_t* cache4 = reinterpret_cast<const uint32_t*>(a.cache) + static_cast<size_t>(hkv) * (kv4::Shape<D>::kRun / 4);
     const size_t page_words = static_cast<size_t>(a.Hkv) * (kv4::Shape<D>::kRun / 4);
     // raw bytes of a tile into registers, zeros past the last token
     auto load_k = [&](int j) {
       if constexpr (KV4) {
-        const int kp = (tile0 + j) * kKvTile + rank * kHalfTile + kkey;
+        const int kp = (tile0 + j) * kKvTile + kfirst, blk = kblk;
+        kblk = block_of(j + 1, kfirst);
 #pragma unroll
         for (int i = 0; i < NJ; ++i) kcodes[i] = 0u;
 #pragma unroll
         for (int i = 0; i < NG; ++i) kpairs[i] = 0u;
         if (j < ntiles && kp < kv_limit) {
-          const int blk = a.table.BlockAt(kp >> 4), t = kp & 15;
           if (blk < 0) {
 #pragma unroll
             for (int i = 0; i < NG; ++i) kpairs[i] = 0x7fc07fc0u;
@@ -266,20 +283,20 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
             if constexpr (D == 256) {
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(at + kv4::Word<D, false>(t, 16 * h + kc)));
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(at + kword[h]));
                 kcodes[4 * h] = v.x; kcodes[4 * h + 1] = v.y; kcodes[4 * h + 2] = v.z; kcodes[4 * h + 3] = v.w;
               }
-              const uint4 p = __ldg(reinterpret_cast<const uint4*>(at + 2 * D + t * NG));
+              const uint4 p = __ldg(reinterpret_cast<const uint4*>(at + kpair));
               kpairs[0] = p.x; kpairs[1] = p.y; kpairs[2] = p.z; kpairs[3] = p.w;
             } else if constexpr (D == 128) {
-              const uint4 v = __ldg(reinterpret_cast<const uint4*>(at + kv4::Word<D, false>(t, kc)));
+              const uint4 v = __ldg(reinterpret_cast<const uint4*>(at + kword[0]));
               kcodes[0] = v.x; kcodes[1] = v.y; kcodes[2] = v.z; kcodes[3] = v.w;
-              const uint2 p = __ldg(reinterpret_cast<const uint2*>(at + 2 * D + t * NG));
+              const uint2 p = __ldg(reinterpret_cast<const uint2*>(at + kpair));
               kpairs[0] = p.x; kpairs[1] = p.y;
             } else {
-              const uint2 v = __ldg(reinterpret_cast<const uint2*>(at + kv4::Word<D, false>(t, kc)));
+              const uint2 v = __ldg(reinterpret_cast<const uint2*>(at + kword[0]));
               kcodes[0] = v.x; kcodes[1] = v.y;
-              kpairs[0] = __ldg(at + 2 * D + t);
+              kpairs[0] = __ldg(at + kpair);
             }
           }
         }
@@ -299,20 +316,26 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
     };
     auto load_v = [&](int j) {
       if constexpr (KV4) {
-        const int kp0 = (tile0 + j) * kKvTile + vtok;
+        const int kp0 = (tile0 + j) * kKvTile + vtok, blk = vblk;
+        vblk = block_of(j + 1, vtok);
 #pragma unroll
         for (int t = 0; t < VT; ++t) vcodes[t] = vpairs[t] = 0u;
         if (j < ntiles && kp0 < kv_limit) {
-          const int blk = a.table.BlockAt(kp0 >> 4);
           if (blk >= 0) {
-            const uint32_t* at = cache4 + blk * page_words + kv4::Shape<D>::kPart / 4;
+            const uint32_t* at = cache4 + blk * page_words;
+            if (kp0 + VT <= kv_limit) {
 #pragma unroll
-            for (int t = 0; t < VT; ++t) {
-              const int tok = (kp0 & 15) + t;
-              if (kp0 + t < kv_limit) {
-                vcodes[t] = __ldg(at + kv4::Word<D, true>(tok, rank * VWords + vword));
-                vpairs[t] = __ldg(at + 2 * D + tok * NG + vgroup);
+              for (int t = 0; t < VT; ++t) {
+                vcodes[t] = __ldg(at + kv4::Shape<D>::kPart / 4 + vwords[t]);
+                vpairs[t] = __ldg(at + vpair + t * NG);
               }
+            } else {
+#pragma unroll
+              for (int t = 0; t < VT; ++t)
+                if (kp0 + t < kv_limit) {
+                  vcodes[t] = __ldg(at + kv4::Shape<D>::kPart / 4 + vwords[t]);
+                  vpairs[t] = __ldg(at + vpair + t * NG);
+                }
             }
           }
         }

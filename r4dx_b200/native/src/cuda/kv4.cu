@@ -55,14 +55,14 @@ __device__ __forceinline__ float2 Mul2(float2 a, float2 b) {
 // What a warp knows of its token.
 struct Token {
   int t, tok, blk, lane, li;
-  float2 fc[4], fs[4];         // this lane's rotated channels: own value x fc + the partner channel's x fs
+  const float4* turns;         // [4][32 lanes] of shared memory: of two channels each, own value x (x, y) + the partner channel's x (z, w)
   float* rows;                 // [32 lanes][8] of shared memory
 };
 
-// Rounds of heads `first` .. (one, two or four at a time, lane / (D / 8)) of one kind: q (KIND 0), k (1) or v (2); two rounds in flight.
-template <int D, int KIND>
+// Rounds of heads `first` .. (one, two or four at a time, lane / (D / 8)) of one kind: q (KIND 0), k (1) or v (2); AHEAD rounds in flight.
+template <int D, int AHEAD, int KIND>
 __device__ __forceinline__ void Heads(const PrecoreArgs& a, const Token& tk, int first, int rounds) {
-  constexpr int LPH = D / 8, HPW = 32 / LPH, AHEAD = 2;
+  constexpr int LPH = D / 8, HPW = 32 / LPH;
   const int heads = KIND == 0 ? a.Hq : a.Hkv, li = tk.li, lane = tk.lane;
   const __nv_bfloat16* src = KIND == 0 ? a.qg + static_cast<size_t>(tk.t) * a.Hq * a.q_stride : (KIND == 1 ? a.k : a.v) + static_cast<size_t>(tk.t) * a.Hkv * D;
   const int step = KIND == 0 ? a.q_stride : D;
@@ -121,7 +121,10 @@ __device__ __forceinline__ void Heads(const PrecoreArgs& a, const Token& tk, int
           for (int i = 0; i < 4; ++i) y[i] = make_float2(__shfl_xor_sync(0xffffffffu, x[u][i].x, hop), __shfl_xor_sync(0xffffffffu, x[u][i].y, hop));
           if (8 * li < a.rotary_dim) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[u][i] = ptx::Fma2(x[u][i], tk.fc[i], Mul2(y[i], tk.fs[i]));
+            for (int i = 0; i < 4; ++i) {
+              const float4 f = tk.turns[i * 32 + lane];
+              x[u][i] = ptx::Fma2(x[u][i], make_float2(f.x, f.y), Mul2(y[i], make_float2(f.z, f.w)));
+            }
           }
         } else {
           __syncwarp();
@@ -133,8 +136,9 @@ __device__ __forceinline__ void Heads(const PrecoreArgs& a, const Token& tk, int
           };
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            turn(x[u][i].x, 8 * li + 2 * i, tk.fc[i].x, tk.fs[i].x);
-            turn(x[u][i].y, 8 * li + 2 * i + 1, tk.fc[i].y, tk.fs[i].y);
+            const float4 f = tk.turns[i * 32 + lane];
+            turn(x[u][i].x, 8 * li + 2 * i, f.x, f.z);
+            turn(x[u][i].y, 8 * li + 2 * i + 1, f.y, f.w);
           }
         }
       }
@@ -202,8 +206,10 @@ __device__ __forceinline__ void Heads(const PrecoreArgs& a, const Token& tk, int
 
 // A warp has one token and some of its q, its k or its v heads: eight channels a lane, D / 8 lanes a head.  A channel pair's angle is position x
 // frequency in turns, in 64 bits; what its whole turns leave fits 32 bits for the sine and cosine.
-template <int D>
-__global__ void __launch_bounds__(256) PrecoreKv4Kernel(PrecoreArgs a) {
+// What bounds many rows is the time between dependent instructions, so warps count: factors of the rotation in shared memory and 64 registers (32
+// warps to an SM) took 8192 rows of 24 + 4 + 4 heads of 256 from 105 to 78 us, one round in flight instead of two is 83; one row 3.0 / 2.3 us.
+template <int D, int AHEAD>
+__global__ void __launch_bounds__(256, D == 256 || AHEAD == 1 ? 4 : 3) PrecoreKv4Kernel(PrecoreArgs a) {
   PdlEnter();
   constexpr int LPH = D / 8, HPW = 32 / LPH;
   extern __shared__ float smem[];
@@ -231,8 +237,12 @@ __global__ void __launch_bounds__(256) PrecoreKv4Kernel(PrecoreArgs a) {
     }
     if (tk.blk < 0) return;
   }
-  float* cs = smem + warp * (a.rotary_dim + 32 * 8);             // [half] cosines, [half] sines
-  tk.rows = cs + a.rotary_dim;
+  // of a warp: [4][32] float4 of factors, [32 lanes][8] for channels that change lanes - before that the cosines and sines of the pairs
+  float* own = smem + warp * (4 * 32 * 4 + 32 * 8);
+  float4* turns = reinterpret_cast<float4*>(own);
+  float* cs = own + 4 * 32 * 4;
+  tk.turns = turns;
+  tk.rows = cs;
   if (kind != 2) {
     for (int i = lane; i < half; i += 32) {
       const double turns = static_cast<double>(pos) * exp2(a.turn_exponent + i * a.turn_step);
@@ -249,14 +259,17 @@ __global__ void __launch_bounds__(256) PrecoreKv4Kernel(PrecoreArgs a) {
     };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      turn(8 * li + 2 * i, tk.fc[i].x, tk.fs[i].x);
-      turn(8 * li + 2 * i + 1, tk.fc[i].y, tk.fs[i].y);
+      float4 f;
+      turn(8 * li + 2 * i, f.x, f.z);
+      turn(8 * li + 2 * i + 1, f.y, f.w);
+      turns[i * 32 + lane] = f;
     }
+    __syncwarp();                                // (the cosines are read: what follows may take their place)
   }
   const int first = part * a.steps * HPW + lane / LPH, rounds = min(a.steps, (kind == 0 ? rounds_q : rounds_kv) - part * a.steps);
-  if (kind == 0) Heads<D, 0>(a, tk, first, rounds);
-  else if (kind == 1) Heads<D, 1>(a, tk, first, rounds);
-  else Heads<D, 2>(a, tk, first, rounds);
+  if (kind == 0) Heads<D, AHEAD, 0>(a, tk, first, rounds);
+  else if (kind == 1) Heads<D, AHEAD, 1>(a, tk, first, rounds);
+  else Heads<D, AHEAD, 2>(a, tk, first, rounds);
 }
 
 // Rows read back: a thread has one word (eight channels) of a row and up to ITEMS of its 2 Hkv heads' keys and values, whose codes and pairs it
@@ -310,8 +323,9 @@ int LaunchPrecore(PrecoreArgs a, cudaStream_t s) {
   a.groups = (rounds_q + a.steps - 1) / a.steps + 2 * ((rounds_kv + a.steps - 1) / a.steps);
   const long long tasks = static_cast<long long>(a.T) * a.groups;
   if (tasks > 0x7fffffffll - 8) return R4DXB_TOO_LARGE;
-  const size_t smem = 8 * (a.rotary_dim + 32 * 8) * sizeof(float);
-  return LaunchPdl(PrecoreKv4Kernel<D>, dim3(static_cast<unsigned>((tasks + 7) / 8)), dim3(256), smem, s, a);
+  const size_t smem = 8 * (4 * 32 * 4 + 32 * 8) * sizeof(float);      // (D of the 256 floats hold a token's cosines and sines)
+  const dim3 grid(static_cast<unsigned>((tasks + 7) / 8));
+  return a.steps == 1 ? LaunchPdl(PrecoreKv4Kernel<D, 1>, grid, dim3(256), smem, s, a) : LaunchPdl(PrecoreKv4Kernel<D, 2>, grid, dim3(256), smem, s, a);
 }
 
 template <int D>
