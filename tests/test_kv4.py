@@ -120,3 +120,48 @@ def test_prefill_shares_fill_the_chip():
                         keys = min(window + T, pos0 + T) if window else pos0 + T
                         assert 0 <= s <= 64 and (s > 0 or T <= K.KV4_MAX_ROWS) and (s < 2 or s * 256 <= keys + 256 and s * T * Hq * D <= 1 << 26)
     assert K.kv4_prefill_splits(8192, 24, 4, 256, 0, 0) == 1 and K.kv4_prefill_splits(128, 24, 4, 256, 29000, 0) >= 4
+
+
+def test_entry_points_refuse_bad_arguments_without_a_gpu():
+    """Each C entry answers before it touches a pointer or the device."""
+    from r4dx_b200 import native
+    from r4dx_b200.ops import kernels  # noqa: F401  (signatures)
+    L, bad, large = native.cuda(), 10001, 10003
+    p, odd = 1 << 20, (1 << 20) + 4
+
+    def decode(q=p, qg=p, cache=p, tables=p, slots_of=None, slots=1, length=4, pool=4, pos=p, scratch=p, out=p, T=1, batch=1, Hq=4, Hkv=2, D=128,
+               splits=2, chunk=8, cluster=0, window=0):
+        return L.r4dxb_attn_decode_kv4(q, qg, cache, tables, slots_of, slots, length, pool, pos, scratch, out, T, batch, Hq, Hkv, D, splits, chunk,
+                                       cluster, window, None, None)
+
+    for kw in (dict(T=0), dict(T=33), dict(batch=2), dict(batch=0), dict(slots_of=p, T=2), dict(Hq=3), dict(Hkv=0), dict(D=96), dict(splits=0),
+               dict(splits=257), dict(splits=17, cluster=1), dict(chunk=0), dict(window=-1), dict(length=0), dict(pool=0), dict(slots=0), dict(q=None),
+               dict(cache=None), dict(tables=None), dict(pos=None), dict(out=None), dict(scratch=None), dict(q=odd), dict(cache=odd), dict(out=odd),
+               dict(scratch=odd), dict(slots_of=p, batch=70000)):
+        assert decode(**kw) == bad, kw
+    assert decode(Hq=1 << 20, Hkv=1 << 16) == large
+
+    def prefill(q=p, qg=p, cache=p, table=p, length=4, pool=4, out=p, T=1, Hq=4, Hkv=2, D=128, pos0=0, window=0, splits=1, scratch=None):
+        return L.r4dxb_attn_prefill_kv4(q, qg, cache, table, length, pool, out, T, Hq, Hkv, D, pos0, window, None, splits, scratch, None, None)
+
+    for kw in (dict(T=0), dict(Hq=3), dict(Hq=0), dict(D=32), dict(pos0=-1), dict(pos0=2 ** 31 - 2), dict(window=-1), dict(splits=0), dict(splits=65),
+               dict(splits=2), dict(splits=2, scratch=odd), dict(q=odd), dict(qg=odd), dict(out=odd), dict(q=None), dict(cache=None), dict(table=None),
+               dict(out=None), dict(length=0), dict(pool=0)):
+        assert prefill(**kw) == bad, kw
+    assert prefill(Hq=40000, Hkv=1) == large
+
+    def precore(qg=p, k=p, v=p, pos=p, tables=p, slots=1, length=4, pool=4, q=p, cache=p, T=1, Hq=4, Hkv=2, D=128, rot=64, theta=1e4, stride=256):
+        return L.r4dxb_attn_precore_kv4(qg, k, v, None, None, pos, tables, None, slots, length, pool, q, cache, T, Hq, Hkv, D, rot, theta, 1e-6, stride, None)
+
+    for kw in (dict(T=0), dict(Hq=-1), dict(Hkv=0), dict(D=80), dict(rot=-2), dict(rot=63), dict(rot=130), dict(theta=0.0), dict(theta=math.nan),
+               dict(stride=64), dict(stride=130), dict(qg=None), dict(q=None), dict(k=None), dict(v=None), dict(pos=None), dict(tables=None),
+               dict(cache=None), dict(k=odd), dict(cache=odd), dict(q=odd), dict(length=0), dict(pool=0), dict(slots=0)):
+        assert precore(**kw) == bad, kw
+
+    def read(cache=p, tables=p, slots=1, length=4, pool=4, pos=p, k=p, v=p, T=1, Hkv=2, D=128):
+        return L.r4dxb_kv4_read(cache, tables, None, slots, length, pool, pos, k, v, T, Hkv, D, None)
+
+    for kw in (dict(T=0), dict(Hkv=0), dict(D=48), dict(cache=None), dict(tables=None), dict(pos=None), dict(k=None), dict(v=None), dict(k=odd),
+               dict(cache=odd), dict(length=0), dict(pool=0), dict(slots=0)):
+        assert read(**kw) == bad, kw
+    assert read(Hkv=40000) == large

@@ -335,6 +335,69 @@ def test_nan_keys_and_values_reach_the_rows_that_see_them_only(K, D):
     K.check_gemm_status(out.device)
 
 
+def test_rows_in_any_order_of_positions(K):
+    """Rows of one sequence need not be sorted, some may be padding, some beyond the table; sixteen of them take two row tiles."""
+    D, Hq, Hkv, n = 128, 4, 2, 300
+    g = torch.Generator().manual_seed(12)
+    pool = Pool(D, Hkv, [n], seed=12)
+    pos = torch.tensor([299, 0, -1, 17, 17, 150, 16, 5, -7, 299, 31, 32, 128, 1, 2, 3], dtype=torch.int32)
+    q = torch.randn(16, Hq, D, generator=g).to(BF)
+    out = torch.full((16, Hq, D), NAN, dtype=BF, device="cuda")
+    for window in (0, 20):
+        K.attn_decode_kv4(q.cuda(), None, pool.cache.cuda(), pool.tables[0].cuda(), pos.cuda(), out, 16, Hq, Hkv, D, False, window)
+        check(out, attention(q, pool.k[0], pool.v[0], pos.long(), window), pool.v[0])
+        assert (out[2] == 0).all() and (out[8] == 0).all()
+    far = pos.clone()
+    far[5] = 2 ** 31 - 1
+    K.attn_decode_kv4(q.cuda(), None, pool.cache.cuda(), pool.tables[0].cuda(), far.cuda(), out, 16, Hq, Hkv, D, False, 20)
+    assert torch.equal(out.isnan().flatten(1).all(1).cpu(), far == 2 ** 31 - 1)
+    K.check_gemm_status(out.device)
+
+
+def test_blocks_beyond_four_gigabytes(K):
+    """A pool of 4.7 GB of which only the blocks at its ends are used."""
+    D, Hq, Hkv, n = 256, 16, 8, 70
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 12 GB of device memory")
+    blocks = 130000
+    cache = torch.empty(kv4.pool_shape(blocks, Hkv, D), dtype=torch.uint8, device="cuda")
+    assert cache.numel() > 1 << 32
+    table = torch.tensor([blocks - 1, 0, blocks - 2, 1, blocks - 3], dtype=torch.int32)
+    g = torch.Generator().manual_seed(0)
+    k, v, q = rows(g, n, Hkv, D), rows(g, n, Hkv, D), torch.randn(n, Hq, D, generator=g).to(BF)
+    pos = torch.arange(n, dtype=torch.int32)
+    K.kv4_write(k.cuda(), v.cuda(), pos.cuda(), table.cuda(), cache)
+    rk, rv = K.kv4_read(cache, table.cuda(), pos.cuda())
+    kr, vr = kv4.round_trip(k), kv4.round_trip(v)
+    assert torch.equal(rk.cpu(), kr.to(BF)) and torch.equal(rv.cpu(), vr.to(BF))
+    want = attention(q, kr.double(), vr.double(), pos.long())
+    out = torch.empty(n, Hq, D, dtype=BF, device="cuda")
+    K.attn_prefill_kv4(q.cuda(), None, cache, table.cuda(), out, n, Hq, Hkv, D, 0, False)
+    check(out, want, vr, slack=score_slack(q, kr.double(), vr.double()))
+    K.attn_decode_kv4(q[-5:].contiguous().cuda(), None, cache, table.cuda(), pos[-5:].contiguous().cuda(), out, 5, Hq, Hkv, D, False)
+    check(out[:5], want[-5:], vr)
+
+
+def test_two_streams_at_once_and_rows_behind_the_last_one(K):
+    """Calls on two streams with scratch of their own; what lies behind the last row of an output stays as it was."""
+    D, Hq, Hkv, n = 256, 24, 4, 3000
+    g = torch.Generator().manual_seed(21)
+    pools = [Pool(D, Hkv, [n], seed=s) for s in (1, 2)]
+    q = torch.randn(2, 1, Hq, D, generator=g).to(BF)
+    pos = torch.tensor([n - 1], dtype=torch.int32).cuda()
+    state = [(q[i].cuda(), p.cache.cuda(), p.tables[0].cuda(), torch.full((3, Hq, D), 7.0, dtype=BF, device="cuda")) for i, p in enumerate(pools)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for st, (a, c, t, o) in zip(streams, state):
+            with torch.cuda.stream(st):
+                K.attn_decode_kv4(a, None, c, t, pos, o, 1, Hq, Hkv, D, False)
+    torch.cuda.synchronize()
+    for i, p in enumerate(pools):
+        check(state[i][3][:1], attention(q[i], p.k[0], p.v[0], torch.tensor([n - 1])), p.v[0])
+        assert (state[i][3][1:] == 7.0).all()
+
+
 def test_large_scores_and_uniform_attention(K):
     """One key that takes all the weight, late, so that everything before it is scaled away; and equal keys over a long context, where the
     result is a small mean of large terms."""
