@@ -32,7 +32,7 @@ struct DecodeArgs {
   const __nv_bfloat16* qg;     // [T, Hq, 2 D], the gate behind (null: none)
   const uint8_t* cache;
   kv4::Table table;
-  const int* positions;        // [T]; batched: one row each
+  const int* positions;        // [T]; batched: one row each; null: pos0, pos0 + 1 ..
   const int* row_slot;         // batched: sequence of each row
   float* part_acc;             // [batch][Hkv][G][splits][D]
   float2* part_ml;             // [batch][Hkv][G][splits]
@@ -40,8 +40,10 @@ struct DecodeArgs {
   int* status;
   int T, Hq, Hkv, splits, slots, window;
   int chunk;                   // blocks of a sequence for which another CTA joins
+  int pos0;
   uint32_t per_token;          // 2^32 / (query heads per kv head), rounded up; 0: one query head
   // row r of a kv head's G = T Hq / Hkv belongs to token Row(r)
+  __device__ __forceinline__ int Position(int t) const { return positions != nullptr ? positions[t] : pos0 + t; }
   __device__ __forceinline__ int Row(int r) const { return per_token != 0u ? static_cast<int>(__umulhi(static_cast<uint32_t>(r), per_token)) : r; }
 };
 
@@ -70,15 +72,15 @@ struct Span {
   int first, blocks, active;
   int position;                // of token `lane`, -1 beyond the last
 };
-__device__ __forceinline__ Span Visible(const int* positions, int T, int window, int splits, int chunk) {
+__device__ __forceinline__ Span Visible(const DecodeArgs& a) {
   const int lane = threadIdx.x & 31;
-  const int p = lane < T ? positions[lane] : -1;
+  const int p = lane < a.T ? a.Position(lane) : -1;
   Span s;
   s.position = p;
   const int high = __reduce_max_sync(0xffffffffu, p), low = __reduce_min_sync(0xffffffffu, p < 0 ? 0x7fffffff : p);
-  s.first = window > 0 && high >= 0 ? max(0, low - window + 1) / kv4::kBlock : 0;
+  s.first = a.window > 0 && high >= 0 ? max(0, low - a.window + 1) / kv4::kBlock : 0;
   s.blocks = high >= 0 ? high / kv4::kBlock + 1 - s.first : 0;
-  s.active = max(1, min(splits, static_cast<int>((static_cast<unsigned>(s.blocks) + chunk - 1) / chunk)));
+  s.active = max(1, min(a.splits, static_cast<int>((static_cast<unsigned>(s.blocks) + a.chunk - 1) / a.chunk)));
   return s;
 }
 
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
                  : make_uint4(0u, 0u, 0u, 0u);
   };
   uint4 query_next = warp < NT * NJ ? load_query(warp) : make_uint4(0u, 0u, 0u, 0u);
-  const Span span = Visible(a.positions, a.T, a.window, a.splits, a.chunk);
+  const Span span = Visible(a);
   if (split >= (CLUSTER && span.active > 1 ? a.splits : span.active)) return;       // (a cluster stays together, its CTAs without blocks merge too)
   const int per = (span.blocks + span.active - 1) / span.active;
   // the CTA's blocks b0 .. b1 - 1 go around its warps, kPair at a time where there are more of them than warps
@@ -312,7 +314,7 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
           const bool number = (pair & 0x7f80u) != 0x7f80u && (pair & 0x7f800000u) != 0x7f800000u;
           if (used && !number)
             for (int r = row0; r < min(G, row0 + kRows); ++r)
-              if (sees(a.positions[a.Row(r)], kp)) atomicOr(nan_groups + r - row0, 1 << j);
+              if (sees(a.Position(a.Row(r)), kp)) atomicOr(nan_groups + r - row0, 1 << j);
           if (!used || !number) pair = 0u;
         }
       }
@@ -698,7 +700,7 @@ __global__ void __launch_bounds__(kGroups * D / 4) CombineKv4Kernel(DecodeArgs a
 #pragma unroll
   for (int k = 0; k < (kMaxSplits + kThreads - 1) / kThreads; ++k)
     x[k] = static_cast<int>(threadIdx.x) + k * kThreads < a.splits ? a.part_ml[at + threadIdx.x + k * kThreads] : make_float2(0.f, 0.f);
-  const int active = Visible(a.positions, a.T, a.window, a.splits, a.chunk).active;
+  const int active = Visible(a).active;
   if (active == 1) return;                       // the first kernel has finished the rows
   float m = -INFINITY;
 #pragma unroll
@@ -817,13 +819,13 @@ using namespace r4dxb;
 
 /* scratch (splits > 1, no cluster): batch * Hkv * G * splits * (D + 2) floats, 16-byte aligned: the partial sums, then (maximum, sum) pairs */
 extern "C" int r4dxb_attn_decode_kv4(const void* q, const void* qg, const void* cache, const int* block_tables, const int* row_slot, int slots,
-                                     int table_length, int pool, const int* positions, float* scratch, void* out, int T, int batch, int Hq,
+                                     int table_length, int pool, const int* positions, int pos0, float* scratch, void* out, int T, int batch, int Hq,
                                      int Hkv, int D, int splits, int chunk, int cluster, int window, int* status, void* stream) {
   if (T < 1 || T > 32 || batch < 1 || batch > 65535 || (row_slot == nullptr && batch != 1) || (row_slot != nullptr && T != 1) || Hkv < 1 || Hq < 1 ||
       Hq % Hkv || (D != 64 && D != 128 && D != 256) || chunk < 1 || splits < 1 || splits > (cluster ? kMaxCluster : kMaxSplits) || slots < 1 || table_length < 1 || pool < 1 || window < 0)
     return R4DXB_BAD_ARG;
   if ((static_cast<long long>(Hq / Hkv) * T + 7) / 8 * Hkv > 65535) return R4DXB_TOO_LARGE;
-  if (q == nullptr || cache == nullptr || block_tables == nullptr || positions == nullptr || out == nullptr || (splits > 1 && !cluster && scratch == nullptr))
+  if (q == nullptr || cache == nullptr || block_tables == nullptr || (positions == nullptr && (row_slot != nullptr || pos0 < 0 || pos0 > 0x7fffffff - T)) || out == nullptr || (splits > 1 && !cluster && scratch == nullptr))
     return R4DXB_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(scratch)) & 15 ||
       (reinterpret_cast<uintptr_t>(qg) | reinterpret_cast<uintptr_t>(out)) & 7)
@@ -839,7 +841,7 @@ extern "C" int r4dxb_attn_decode_kv4(const void* q, const void* qg, const void* 
   a.part_ml = reinterpret_cast<float2*>(scratch + static_cast<size_t>(batch) * Hq * T * splits * D);
   a.out = static_cast<__nv_bfloat16*>(out);
   a.status = status;
-  a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.splits = splits; a.chunk = chunk; a.slots = slots; a.window = window;
+  a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.splits = splits; a.chunk = chunk; a.pos0 = pos0; a.slots = slots; a.window = window;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return cluster ? LaunchDecodeDim<true>(a, batch, D, s) : LaunchDecodeDim<false>(a, batch, D, s);
 }

@@ -1163,7 +1163,7 @@ def q4x_hc_gate(h, norm_w, w_down_inject, w_up, mid, injv, rstd, x, T: int, hc: 
 # ---- attention over a 4-bit paged KV cache (format: quant/kv4.py) ------------------------------------------------------------------
 register_cuda_sig("r4dxb_attn_precore_kv4", _I, [_P] * 8 + [_I] * 3 + [_P, _P] + [_I] * 5 + [_F, _F, _I, _P])
 register_cuda_sig("r4dxb_kv4_read", _I, [_P] * 3 + [_I] * 3 + [_P] * 3 + [_I] * 3 + [_P])
-register_cuda_sig("r4dxb_attn_decode_kv4", _I, [_P] * 5 + [_I] * 3 + [_P] * 3 + [_I] * 9 + [_P, _P])
+register_cuda_sig("r4dxb_attn_decode_kv4", _I, [_P] * 5 + [_I] * 3 + [_P, _I, _P, _P] + [_I] * 9 + [_P, _P])
 register_cuda_sig("r4dxb_attn_prefill_kv4", _I, [_P] * 4 + [_I] * 2 + [_P] + [_I] * 6 + [_P, _I] + [_P] * 3)
 
 KV4_MAX_ROWS = 32           # rows of one sequence that attn_decode_kv4 takes
@@ -1308,15 +1308,17 @@ def kv4_scratch_floats(T: int, batch: int, Hq: int, Hkv: int, D: int, length: in
 
 
 def attn_decode_kv4(q, qg, cache, block_table, positions, out, T: int, Hq: int, Hkv: int, D: int, gated: bool = True, window: int = 0,
-                    row_slot: Optional[torch.Tensor] = None, splits: Optional[int] = None, scratch: Optional[torch.Tensor] = None):
+                    row_slot: Optional[torch.Tensor] = None, splits: Optional[int] = None, scratch: Optional[torch.Tensor] = None,
+                    pos0: int = 0):
     """Attention of T (at most 32) rows of one sequence over a 4-bit cache, each up to its position; with ``row_slot`` of one row of each of
     T sequences (tables ``block_table[row_slot[t]]``).  ``gated``: times the sigmoid of the upper half of qg's heads.  ``window`` > 0: only
-    the last ``window`` keys.  A position of -1 sees nothing and gives zeros; a row that sees a block which the table or pool does not have
+    the last ``window`` keys.  ``positions`` None: pos0, pos0 + 1 .. of one sequence.  A position of -1 sees nothing and gives zeros; a row that sees a block which the table or pool does not have
     gives NaN.  ``splits``: CTAs that share a sequence (by ``kv4_splits`` unless given).  ``scratch``: fp32, ``kv4_scratch_floats`` of it, not
     shared with a call that may run at the same time; allocated for the call unless given."""
     dev, slots, length, pool, heads, dim = _kv4_pool(cache, block_table, row_slot, T)
     rows, batch = (T, 1) if row_slot is None else (1, T)
-    if T < 1 or rows > KV4_MAX_ROWS or batch > 65535 or Hkv != heads or D != dim or Hq < 1 or Hq % Hkv or window < 0:
+    if T < 1 or rows > KV4_MAX_ROWS or batch > 65535 or Hkv != heads or D != dim or Hq < 1 or Hq % Hkv or window < 0 \
+            or positions is None and (row_slot is not None or not 0 <= pos0 < 1 << 30):
         raise KernelError(f"attn_decode_kv4: unsupported shape T={T}, Hq={Hq}, Hkv={Hkv}, D={D}, window={window}")
     n = T * Hq * D
     chunk, cluster = 8, False
@@ -1333,7 +1335,8 @@ def attn_decode_kv4(q, qg, cache, block_table, positions, out, T: int, Hq: int, 
             raise KernelError(f"scratch must be a contiguous, 16-byte aligned fp32 tensor of {need} or more elements on cuda:{dev}")
     _check(_lib().r4dxb_attn_decode_kv4(
         _kv4_rows(q, "q", n, dev), _kv4_rows(qg, "qg", 2 * n, dev) if gated else None, cache.data_ptr(), block_table.data_ptr(), _p(row_slot),
-        slots, length, pool, _kv4_ints(positions, "positions", T, dev), scratch.data_ptr() if need else None, _kv4_rows(out, "out", n, dev),
+        slots, length, pool, None if positions is None else _kv4_ints(positions, "positions", T, dev), pos0,
+        scratch.data_ptr() if need else None, _kv4_rows(out, "out", n, dev),
         rows, batch, Hq, Hkv, D, splits, chunk, cluster, window, _status_word(dev), _raw_stream(dev)), "attn_decode_kv4")
     return out
 
@@ -1390,8 +1393,7 @@ def attn_prefill_kv4(q, qg, cache, block_table, out, T: int, Hq: int, Hkv: int, 
     if splits is None:
         splits = kv4_prefill_splits(T, Hq, Hkv, D, pos0, window)
         if not splits and key_limit is None:
-            positions = torch.arange(pos0, pos0 + T, dtype=torch.int32, device=cache.device)
-            return attn_decode_kv4(q, qg, cache, block_table, positions, out, T, Hq, Hkv, D, gated, window)
+            return attn_decode_kv4(q, qg, cache, block_table, None, out, T, Hq, Hkv, D, gated, window, pos0=pos0)
         splits = splits or 1
     elif not 1 <= splits <= 64:
         raise KernelError(f"attn_prefill_kv4: splits={splits} not in 1 .. 64")

@@ -129,14 +129,14 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu():
     L, bad, large = native.cuda(), 10001, 10003
     p, odd = 1 << 20, (1 << 20) + 4
 
-    def decode(q=p, qg=p, cache=p, tables=p, slots_of=None, slots=1, length=4, pool=4, pos=p, scratch=p, out=p, T=1, batch=1, Hq=4, Hkv=2, D=128,
+    def decode(q=p, qg=p, cache=p, tables=p, slots_of=None, slots=1, length=4, pool=4, pos=p, pos0=0, scratch=p, out=p, T=1, batch=1, Hq=4, Hkv=2, D=128,
                splits=2, chunk=8, cluster=0, window=0):
-        return L.r4dxb_attn_decode_kv4(q, qg, cache, tables, slots_of, slots, length, pool, pos, scratch, out, T, batch, Hq, Hkv, D, splits, chunk,
+        return L.r4dxb_attn_decode_kv4(q, qg, cache, tables, slots_of, slots, length, pool, pos, pos0, scratch, out, T, batch, Hq, Hkv, D, splits, chunk,
                                        cluster, window, None, None)
 
     for kw in (dict(T=0), dict(T=33), dict(batch=2), dict(batch=0), dict(slots_of=p, T=2), dict(Hq=3), dict(Hkv=0), dict(D=96), dict(splits=0),
                dict(splits=257), dict(splits=17, cluster=1), dict(chunk=0), dict(window=-1), dict(length=0), dict(pool=0), dict(slots=0), dict(q=None),
-               dict(cache=None), dict(tables=None), dict(pos=None), dict(out=None), dict(scratch=None), dict(q=odd), dict(cache=odd), dict(out=odd),
+               dict(cache=None), dict(tables=None), dict(pos=None, pos0=-1), dict(pos=None, slots_of=p), dict(out=None), dict(scratch=None), dict(q=odd), dict(cache=odd), dict(out=odd),
                dict(scratch=odd), dict(slots_of=p, batch=70000)):
         assert decode(**kw) == bad, kw
     assert decode(Hq=1 << 20, Hkv=1 << 16) == large

@@ -201,6 +201,10 @@ def test_decode_attention(K, D, Hq, Hkv, T, ctx, window, gated, splits):
     if gated:
         want = want * torch.sigmoid(qg[..., D:].double())
     check(out, want, pool.v[0])
+    again = torch.full_like(out, NAN)
+    K.attn_decode_kv4(q.cuda(), qg.cuda() if gated else None, pool.cache.cuda(), pool.tables[0].cuda(), None, again, T, Hq, Hkv, D, gated=gated,
+                      window=window, splits=splits, pos0=ctx - T)
+    assert torch.equal(out, again)
 
 
 @pytest.mark.parametrize("D,Hq,Hkv,window,splits", [(256, 24, 4, 0, None), (128, 8, 2, 0, 4), (64, 32, 8, 50, None), (128, 16, 1, 0, 1)])
@@ -510,7 +514,8 @@ def test_refusals(K):
     bad = [(decode, dict(D=64)), (decode, dict(Hkv=1)), (decode, dict(Hq=3)), (decode, dict(T=2)), (decode, dict(T=0)), (decode, dict(window=-1)),
            (decode, dict(q=q.half())), (decode, dict(q=odd)), (decode, dict(q=q.cpu())), (decode, dict(cache=cache[:, :, :1])),
            (decode, dict(cache=cache.float())), (decode, dict(block_table=table.long())), (decode, dict(block_table=table[None])),
-           (decode, dict(positions=pos.long())), (decode, dict(row_slot=pos)), (decode, dict(qg=q)), (decode, dict(qg=None)), (decode, dict(out=out[:, :2])),
+           (decode, dict(positions=pos.long())), (decode, dict(positions=None, pos0=-1)),
+           (decode, dict(positions=None, row_slot=pos, block_table=table[None])), (decode, dict(row_slot=pos)), (decode, dict(qg=q)), (decode, dict(qg=None)), (decode, dict(out=out[:, :2])),
            (decode, dict(splits=3, scratch=e(8, dtype=torch.float32))), (decode, dict(splits=0)), (decode, dict(splits=1000)),
            (prefill, dict(D=64)), (prefill, dict(T=2)), (prefill, dict(pos0=-1)), (prefill, dict(q=odd)), (prefill, dict(window=-2)),
            (prefill, dict(key_limit=pos.long())), (prefill, dict(cache=cache.transpose(0, 1))), (prefill, dict(T=0)), (prefill, dict(splits=0)), (prefill, dict(splits=65)),
