@@ -180,6 +180,29 @@ def main() -> None:
             us = timed(lambda: K.attn_prefill(q, qg, cache, table, ds, ds, out, Tq, Hq, Hkv, D, ctx, True), a.iters, flush)
             K.check_gemm_status(dev)
             print(f"attn_prefill[{impl}] T={Tq} ctx={ctx}: {us:9.1f} us  {flops / us / 1e6:7.1f} TFLOP/s (causal-effective)")
+    if a.only in ("kv4",):
+        # the 4-bit cache's calls: rows written (and read back), decode attention of --rows rows, prefill of max(--rows, 128) rows
+        Hq, Hkv, D, ctx = 24, 4, 256, a.ctx
+        Tq = max(a.rows, 128)
+        nblk = (ctx + Tq + 15) // 16 + 1
+        cache = K.kv4_cache(nblk, Hkv, D, dev)
+        table = torch.randperm(nblk, device=dev).to(torch.int32)
+        pos = torch.arange(ctx + Tq, dtype=torch.int32, device=dev)
+        for s in range(0, ctx + Tq, 8192):
+            rows = pos[s:s + 8192]
+            K.kv4_write(torch.randn(rows.numel(), Hkv, D, device=dev).to(BF), torch.randn(rows.numel(), Hkv, D, device=dev).to(BF), rows, table, cache)
+        q, qg = torch.randn(Tq, Hq, D, device=dev).to(BF), torch.randn(Tq, Hq, 2 * D, device=dev).to(BF)
+        k, v, out = torch.randn(Tq, Hkv, D, device=dev).to(BF), torch.randn(Tq, Hkv, D, device=dev).to(BF), torch.empty(Tq, Hq, D, dtype=BF, device=dev)
+        held = Hkv * 2 * D * 9 // 16
+        last = pos[ctx:]
+        for name, fn, nbytes, flops in (
+                ("write", lambda: K.attn_precore_kv4(qg, k, v, None, None, last, table, q, cache, Tq, Hq, Hkv, D, 64, 1e7), Tq * (4 * Hq * D + 4 * Hkv * D + held), 0),
+                ("read", lambda: K.kv4_read(cache, table, last, k, v), Tq * (held + 4 * Hkv * D), 0),
+                ("decode", lambda: K.attn_decode_kv4(q, qg, cache, table, last, out, a.rows, Hq, Hkv, D), ctx * held, 4.0 * Hq * D * a.rows * ctx),
+                ("prefill", lambda: K.attn_prefill_kv4(q, qg, cache, table, out, Tq, Hq, Hkv, D, ctx), ctx * held, 4.0 * Hq * D * Tq * (ctx + (Tq + 1) / 2.0))):
+            us = timed(fn, a.iters, flush)
+            K.check_gemm_status(dev)
+            print(f"kv4 {name} ctx={ctx} T={a.rows if name == 'decode' else Tq}: {us:9.1f} us  {nbytes / us / 1e3:7.0f} GB/s  {flops / us / 1e6:7.1f} TFLOP/s")
     if a.only in ("", "attn"):
         Hq, Hkv, D = 24, 4, 256
         ctx = a.ctx

@@ -25,6 +25,7 @@ def main() -> None:
                     "the kernels of one rank at its real shapes, nothing exchanged (results are wrong by design)")
     ap.add_argument("--graph", type=int, default=0, help="also time this many CUDA-graph replays of the step")
     ap.add_argument("--chunk", type=int, default=0, help="rows per prefill chunk (0: the model's own choice)")
+    ap.add_argument("--kv-cache", default="fp8", choices=["fp8", "int4"])
     ap.add_argument("--prefill", type=int, default=0, help="profile one chunked prefill of this many tokens instead of decode steps")
     a = ap.parse_args()
     from r4dx_b200.config import lfm2_moe_config, qwen_hybrid_27b_config, small_hybrid_config
@@ -42,7 +43,7 @@ def main() -> None:
             comm = NoopComm(a.tp, 0, "cuda:0", None)
             cfg = cfg.shard(a.tp, 0)
         w = synthetic_weight_set(cfg, device="cuda", seed=0)
-    m = HybridModel(cfg, w, max_ctx=max(a.ctx, a.prefill) + 64 + a.rows * (a.steps + 2 + a.graph),
+    m = HybridModel(cfg, w, max_ctx=max(a.ctx, a.prefill) + 64 + a.rows * (a.steps + 2 + a.graph), kv_cache=a.kv_cache,
                     **({"comm": comm} if a.model != "lfm2" and comm is not None else {}))
     if a.prefill:
         ids = torch.randint(0, cfg.vocab_size, (a.prefill,), dtype=torch.int32)
