@@ -41,9 +41,10 @@ struct DecodeArgs {
   int T, Hq, Hkv, splits, slots, window;
   int chunk;                   // blocks of a sequence for which another CTA joins
   int pos0;
+  int end;                     // first position behind the table: a row there or further on sees a block that there is not, and no other counts
   uint32_t per_token;          // 2^32 / (query heads per kv head), rounded up; 0: one query head
   // row r of a kv head's G = T Hq / Hkv belongs to token Row(r)
-  __device__ __forceinline__ int Position(int t) const { return positions != nullptr ? positions[t] : pos0 + t; }
+  __device__ __forceinline__ int Position(int t) const { return min(positions != nullptr ? positions[t] : pos0 + t, end); }
   __device__ __forceinline__ int Row(int r) const { return per_token != 0u ? static_cast<int>(__umulhi(static_cast<uint32_t>(r), per_token)) : r; }
 };
 
@@ -842,6 +843,7 @@ extern "C" int r4dxb_attn_decode_kv4(const void* q, const void* qg, const void* 
   a.out = static_cast<__nv_bfloat16*>(out);
   a.status = status;
   a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.splits = splits; a.chunk = chunk; a.pos0 = pos0; a.slots = slots; a.window = window;
+  a.end = min(table_length, 0x7fffffff / kv4::kBlock) * kv4::kBlock;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return cluster ? LaunchDecodeDim<true>(a, batch, D, s) : LaunchDecodeDim<false>(a, batch, D, s);
 }

@@ -552,24 +552,24 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
         if (ok && lane == 0) ptx::MbarArrive(&ctl->gates);
       }
     } else {
-    if (ok && a.gated) ok = ptx::WarpMbarWait(&ctl->s_full[(ntiles - 1) & 1], static_cast<uint32_t>((ntiles - 1) >> 1) & 1u, abort_flag, 13);
-    if (ok && a.gated) {
+      if (ok && a.gated) ok = ptx::WarpMbarWait(&ctl->s_full[(ntiles - 1) & 1], static_cast<uint32_t>((ntiles - 1) >> 1) & 1u, abort_flag, 13);
+      if (ok && a.gated) {
 #pragma unroll 4
-      for (int i = tid; i < rows * (D / 8); i += kConvThreads) {
-        const int r = i / (D / 8), c = i % (D / 8);
-        const __nv_bfloat16* src = a.qg + ((static_cast<size_t>(q0 + r) * a.Hq + hq) * 2 + 1) * D + c * 8;
-        uint4 g;
-        if (reinterpret_cast<uintptr_t>(a.qg) % 16 == 0) {
-          g = *reinterpret_cast<const uint4*>(src);
-        } else {                              // (their base may lie at any 4 bytes)
-          const uint32_t* w = reinterpret_cast<const uint32_t*>(src);
-          g = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int i = tid; i < rows * (D / 8); i += kConvThreads) {
+          const int r = i / (D / 8), c = i % (D / 8);
+          const __nv_bfloat16* src = a.qg + ((static_cast<size_t>(q0 + r) * a.Hq + hq) * 2 + 1) * D + c * 8;
+          uint4 g;
+          if (reinterpret_cast<uintptr_t>(a.qg) % 16 == 0) {
+            g = *reinterpret_cast<const uint4*>(src);
+          } else {                              // (their base may lie at any 4 bytes)
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(src);
+            g = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          *reinterpret_cast<uint4*>(Ks + GateChunk<D>(r, c)) = g;
         }
-        *reinterpret_cast<uint4*>(Ks + GateChunk<D>(r, c)) = g;
+        __syncwarp();
+        if (lane == 0) ptx::MbarArrive(&ctl->gates);
       }
-      __syncwarp();
-      if (lane == 0) ptx::MbarArrive(&ctl->gates);
-    }
     }
   } else if (warp == kMmaWarp) {
     // ---------------- MMA issuer (one thread of the first CTA) ----------------
@@ -723,14 +723,14 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
           ptx::TcFenceAfter();
           const int nan_groups = ctl->nan_groups[r];
           float* dst = a.part_acc + at * D + half * (D / 2);
-  #pragma unroll 1
+#pragma unroll 1
           for (int c0 = 0; c0 < D / 2; c0 += 32) {
             uint32_t o[32];
             ptx::TmemLoad32x32(t_lane + half * (D / 2) + c0, o);
             ptx::TmemLoadWait();
             const bool nan = nan_groups >> ((half * (D / 2) + c0) >> 6) & 1;
             if (r < rows) {
-  #pragma unroll
+#pragma unroll
               for (int v = 0; v < 8; ++v)
                 *reinterpret_cast<uint4*>(dst + c0 + 4 * v) = nan ? make_uint4(0x7fc00000u, 0x7fc00000u, 0x7fc00000u, 0x7fc00000u) : make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
             }
@@ -900,7 +900,7 @@ extern "C" int r4dxb_attn_prefill_kv4(const void* q, const void* qg, const void*
                                       void* stream) {
   if (splits < 1 || splits > 64 || (splits > 1 && scratch == nullptr) || reinterpret_cast<uintptr_t>(scratch) & 15) return R4DXB_BAD_ARG;
   if (T < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || (D != 64 && D != 128 && D != 256) || pos0 < 0 || pos0 > 0x7fffffff - T - kKvTile || window < 0 ||
-      table_length < 1 || pool < 1 || q == nullptr || cache == nullptr || block_table == nullptr || out == nullptr)
+      table_length < 1 || pos0 > static_cast<long long>(table_length) * kv4::kBlock || pool < 1 || q == nullptr || cache == nullptr || block_table == nullptr || out == nullptr)
     return R4DXB_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(qg)) & 15)
     return R4DXB_BAD_ARG;

@@ -4,7 +4,7 @@
 // of a row are a group: codes n of 4 bits, a scale s and a low end lo (the group's minimum), both bf16; a value is n s + lo.  4.5 bits
 // a value: 64 channels a group keep the pairs at an eighth of the codes, and each kernel's work per group small.
 //   bytes 0 .. 8 D:    code words, eight consecutive channels of a token each, the first in the lowest bits; word w (channels
-//                      8 w ..) of token t lies at Kv4Word
+//                      8 w ..) of token t lies at Word
 //   bytes 8 D .. 9 D:  [16 tokens][D / 64 groups] pairs (s in the lower half, lo in the upper)
 // Keys and values of a head's block are one run of 18 D bytes: one copy brings both to shared memory.
 //

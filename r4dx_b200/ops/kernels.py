@@ -1312,8 +1312,8 @@ def attn_decode_kv4(q, qg, cache, block_table, positions, out, T: int, Hq: int, 
                     pos0: int = 0):
     """Attention of T (at most 32) rows of one sequence over a 4-bit cache, each up to its position; with ``row_slot`` of one row of each of
     T sequences (tables ``block_table[row_slot[t]]``).  ``gated``: times the sigmoid of the upper half of qg's heads.  ``window`` > 0: only
-    the last ``window`` keys.  ``positions`` None: pos0, pos0 + 1 .. of one sequence.  A position of -1 sees nothing and gives zeros; a row that sees a block which the table or pool does not have
-    gives NaN.  ``splits``: CTAs that share a sequence (by ``kv4_splits`` unless given).  ``scratch``: fp32, ``kv4_scratch_floats`` of it, not
+    the last ``window`` keys.  ``positions`` None: pos0, pos0 + 1 .. of one sequence.  A position of -1 sees nothing and
+    gives zeros; a row that sees a block which the table or pool does not have gives NaN.  ``splits``: CTAs that share a sequence (by ``kv4_splits`` unless given).  ``scratch``: fp32, ``kv4_scratch_floats`` of it, not
     shared with a call that may run at the same time; allocated for the call unless given."""
     dev, slots, length, pool, heads, dim = _kv4_pool(cache, block_table, row_slot, T)
     rows, batch = (T, 1) if row_slot is None else (1, T)
@@ -1385,10 +1385,11 @@ def attn_prefill_kv4(q, qg, cache, block_table, out, T: int, Hq: int, Hkv: int, 
                      key_limit: Optional[torch.Tensor] = None, splits: Optional[int] = None):
     """Causal attention of T rows at positions pos0 .. over a 4-bit cache that already holds them (``attn_prefill`` for that cache, on
     tcgen05 for every head dimension, key limits included).  Keys and values are widened to fp16 values, in which magnitudes below 6e-5
-    lose bits.  ``splits``: CTA pairs that share the keys of a row tile (by ``kv4_prefill_splits`` unless given)."""
+    lose bits.  Rows that see a block which the table or pool does not have are NaN; pos0 may not lie behind the table.
+    ``splits``: CTA pairs that share the keys of a row tile (by ``kv4_prefill_splits`` unless given)."""
     dev, slots, length, pool, heads, dim = _kv4_pool(cache, block_table, None, T)
-    if T < 1 or Hkv != heads or D != dim or Hq < 1 or Hq % Hkv or window < 0 or pos0 < 0 or pos0 + T > 1 << 30:
-        raise KernelError(f"attn_prefill_kv4: unsupported shape T={T}, Hq={Hq}, Hkv={Hkv}, D={D}, pos0={pos0}, window={window}")
+    if T < 1 or Hkv != heads or D != dim or Hq < 1 or Hq % Hkv or window < 0 or pos0 < 0 or pos0 > 16 * length or pos0 + T > 1 << 30:
+        raise KernelError(f"attn_prefill_kv4: unsupported shape T={T}, Hq={Hq}, Hkv={Hkv}, D={D}, pos0={pos0}, window={window}, table of {length} blocks")
     n = T * Hq * D
     if splits is None:
         splits = kv4_prefill_splits(T, Hq, Hkv, D, pos0, window)

@@ -144,7 +144,7 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu():
     def prefill(q=p, qg=p, cache=p, table=p, length=4, pool=4, out=p, T=1, Hq=4, Hkv=2, D=128, pos0=0, window=0, splits=1, scratch=None):
         return L.r4dxb_attn_prefill_kv4(q, qg, cache, table, length, pool, out, T, Hq, Hkv, D, pos0, window, None, splits, scratch, None, None)
 
-    for kw in (dict(T=0), dict(Hq=3), dict(Hq=0), dict(D=32), dict(pos0=-1), dict(pos0=2 ** 31 - 2), dict(window=-1), dict(splits=0), dict(splits=65),
+    for kw in (dict(T=0), dict(Hq=3), dict(Hq=0), dict(D=32), dict(pos0=-1), dict(pos0=65), dict(pos0=2 ** 31 - 2), dict(window=-1), dict(splits=0), dict(splits=65),
                dict(splits=2), dict(splits=2, scratch=odd), dict(q=odd), dict(qg=odd), dict(out=odd), dict(q=None), dict(cache=None), dict(table=None),
                dict(out=None), dict(length=0), dict(pool=0)):
         assert prefill(**kw) == bad, kw

@@ -308,7 +308,7 @@ def test_prefill_key_limits(K, D, window):
 
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_nan_keys_and_values_reach_the_rows_that_see_them_only(K, D):
-    """Position 70's second... key (head 0) and position 75's value (first 64 channels of head 1) are NaN: rows before them are as if nothing
+    """A key at position 70 (head 0) and a value at position 75 (first 64 channels of head 1) are NaN: rows before them are as if nothing
     were there, rows after are NaN (of the value: in its channels), rows whose window has passed them are clean again."""
     Hq, Hkv, n, window = 4, 2, 200, 30
     g = torch.Generator().manual_seed(D)
@@ -356,6 +356,37 @@ def test_rows_in_any_order_of_positions(K):
     K.attn_decode_kv4(q.cuda(), None, pool.cache.cuda(), pool.tables[0].cuda(), far.cuda(), out, 16, Hq, Hkv, D, False, 20)
     assert torch.equal(out.isnan().flatten(1).all(1).cpu(), far == 2 ** 31 - 1)
     K.check_gemm_status(out.device)
+
+
+@pytest.mark.parametrize("D,splits", [(64, None), (128, 3), (256, None), (256, 1)])
+def test_positions_far_behind_the_table(K, D, splits):
+    """Rows whose position no table has are NaN and cost no more than a full table; the others are what they are without them."""
+    Hq, Hkv, n = 4, 2, 300
+    g = torch.Generator().manual_seed(13)
+    pool = Pool(D, Hkv, [n], seed=13)
+    end = 16 * pool.tables.shape[1]
+    pos = torch.tensor([299, end, 2 ** 31 - 1, -1, 40, 2 ** 30], dtype=torch.int32)
+    q = torch.randn(6, Hq, D, generator=g).to(BF)
+    for window in (0, 33):
+        out = torch.zeros(6, Hq, D, dtype=BF, device="cuda")
+        args = (q.cuda(), None, pool.cache.cuda(), pool.tables[0].cuda(), pos.cuda(), out, 6, Hq, Hkv, D, False, window)
+        ms = []
+        for _ in range(5):
+            start, stop = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            K.attn_decode_kv4(*args, splits=splits)
+            stop.record()
+            stop.synchronize()
+            ms.append(start.elapsed_time(stop))
+        K.check_gemm_status(out.device)
+        assert min(ms) < 5.0                                # (2^27 missing blocks, one after the other, are tens of ms and more)
+        assert out[[1, 2, 5]].isnan().all() and (out[3] == 0).all()
+        want = attention(q[[0, 4]], pool.k[0], pool.v[0], pos[[0, 4]].long(), window)
+        check(out[[0, 4]], want, pool.v[0])
+        one = torch.zeros(1, Hq, D, dtype=BF, device="cuda")
+        K.attn_decode_kv4(q[:1].cuda(), None, pool.cache.cuda(), pool.tables[0].cuda(), None, one, 1, Hq, Hkv, D, False, window, splits=splits,
+                          pos0=(1 << 30) - 1)
+        assert one.isnan().all()
 
 
 def test_blocks_beyond_four_gigabytes(K):
@@ -518,6 +549,7 @@ def test_refusals(K):
            (decode, dict(positions=None, row_slot=pos, block_table=table[None])), (decode, dict(row_slot=pos)), (decode, dict(qg=q)), (decode, dict(qg=None)), (decode, dict(out=out[:, :2])),
            (decode, dict(splits=3, scratch=e(8, dtype=torch.float32))), (decode, dict(splits=0)), (decode, dict(splits=1000)),
            (prefill, dict(D=64)), (prefill, dict(T=2)), (prefill, dict(pos0=-1)), (prefill, dict(q=odd)), (prefill, dict(window=-2)),
+           (prefill, dict(pos0=65)), (prefill, dict(pos0=1 << 29)),
            (prefill, dict(key_limit=pos.long())), (prefill, dict(cache=cache.transpose(0, 1))), (prefill, dict(T=0)), (prefill, dict(splits=0)), (prefill, dict(splits=65)),
            (precore, dict(rotary_dim=3)), (precore, dict(rotary_dim=130)), (precore, dict(q_stride=100)), (precore, dict(k=odd[:, :2])), (precore, dict(T=2)),
            (precore, dict(q_norm=e(64))), (precore, dict(Hq=0))]
