@@ -125,12 +125,13 @@ int r4dxb_attn_precore_kv4(const void* qg, const void* k, const void* v, const v
 int r4dxb_kv4_read(const void* cache, const int* block_tables, const int* row_slot, int slots, int table_length, int pool, const int* positions,
                    void* k, void* v, int T, int Hkv, int D, void* stream);
 /* T (<= 32) rows of one sequence, or (row_slot given, T = 1) one row of each of `batch` sequences; a position of -1 sees nothing and
- * gives zeros.  qg null: no output gate.  positions null (one sequence): pos0, pos0 + 1 ..  splits: CTAs that may share a sequence, of which
- * every `chunk` visible blocks (of 16 keys) take one.  cluster != 0: the splits (up to 16) are a thread-block cluster, which merges its results itself;
+ * gives zeros.  qg null: no output gate.  positions null (one sequence): pos0, pos0 + 1 ..  tile: query rows of a kv head (T x
+ * Hq / Hkv of them) that a CTA takes: 8, or 16 (D = 256) or 32 (64, 128).  splits: CTAs that may share a sequence, of which every `chunk`
+ * visible blocks (of 16 keys) take one.  cluster != 0: the splits (up to 16) are a thread-block cluster, which merges its results itself;
  * else scratch (splits > 1): batch * T * Hq * splits * (D + 2) floats, 16-byte aligned. */
 int r4dxb_attn_decode_kv4(const void* q, const void* qg, const void* cache, const int* block_tables, const int* row_slot, int slots,
                           int table_length, int pool, const int* positions, int pos0, float* scratch, void* out, int T, int batch, int Hq, int Hkv, int D,
-                          int splits, int chunk, int cluster, int window, int* status, void* stream);
+                          int tile, int splits, int chunk, int cluster, int window, int* status, void* stream);
 /* T rows at positions pos0 .. pos0 + T - 1 (already written), causal; window 0 or the number of keys a row sees; key_limit as for
  * r4dxb_attn_prefill_ex; status as for r4dxb_attn_prefill_tc.  splits (1 .. 64) CTA pairs share the keys of a row tile; above 1 scratch:
  * splits * T * Hq * (D + 2) floats, 16-byte aligned. */

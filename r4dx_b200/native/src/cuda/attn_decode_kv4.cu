@@ -48,10 +48,14 @@ struct DecodeArgs {
   __device__ __forceinline__ int Row(int r) const { return per_token != 0u ? static_cast<int>(__umulhi(static_cast<uint32_t>(r), per_token)) : r; }
 };
 
+// Rows of a CTA that takes many: what the registers allow.  Blocks are unpacked once for all of them.
+template <int D>
+constexpr int kWideTile = D == 256 ? 16 : 32;
+
 // Warps of a CTA, blocks that a warp takes at a time and slots of so many in its ring, by head dimension and row tiles.
 template <int D, int NT>
 struct Plan {
-  static constexpr int kWarps = D == 256 ? 8 : (D == 128 ? (NT == 4 ? 8 : 12) : (NT == 4 ? 12 : (NT == 1 ? 8 : 16)));
+  static constexpr int kWarps = D == 256 ? 8 : (D == 128 ? (NT == 4 ? 8 : 12) : (NT == 4 ? 12 : 8));
   static constexpr int kCtas = D == 64 && NT == 1 ? 2 : 1;
   static constexpr int kPair = NT == 1 ? 2 : 1;
   static constexpr int kStages = NT == 1 ? 2 : 4;
@@ -796,21 +800,16 @@ int LaunchDecode(DecodeArgs a, int batch, cudaStream_t s) {
   }
 }
 
-// Row tiles of a CTA: as few CTAs as the registers allow read the same blocks.
+// tile: rows of a CTA, 8 or as many as the registers allow.
 template <int D, bool CLUSTER>
-int LaunchDecodeRows(const DecodeArgs& a, int batch, cudaStream_t s) {
-  const int G = a.Hq / a.Hkv * a.T;
-  if (G <= 8) return LaunchDecode<D, 1, CLUSTER>(a, batch, s);
-  if constexpr (D == 256) {
-    return LaunchDecode<D, 2, CLUSTER>(a, batch, s);
-  } else {
-    return G <= 16 ? LaunchDecode<D, 2, CLUSTER>(a, batch, s) : LaunchDecode<D, 4, CLUSTER>(a, batch, s);
-  }
+int LaunchDecodeRows(const DecodeArgs& a, int batch, int tile, cudaStream_t s) {
+  return tile == 8 ? LaunchDecode<D, 1, CLUSTER>(a, batch, s) : LaunchDecode<D, kWideTile<D> / 8, CLUSTER>(a, batch, s);
 }
 
 template <bool CLUSTER>
-int LaunchDecodeDim(const DecodeArgs& a, int batch, int D, cudaStream_t s) {
-  return D == 256 ? LaunchDecodeRows<256, CLUSTER>(a, batch, s) : (D == 128 ? LaunchDecodeRows<128, CLUSTER>(a, batch, s) : LaunchDecodeRows<64, CLUSTER>(a, batch, s));
+int LaunchDecodeDim(const DecodeArgs& a, int batch, int D, int tile, cudaStream_t s) {
+  return D == 256 ? LaunchDecodeRows<256, CLUSTER>(a, batch, tile, s)
+                  : (D == 128 ? LaunchDecodeRows<128, CLUSTER>(a, batch, tile, s) : LaunchDecodeRows<64, CLUSTER>(a, batch, tile, s));
 }
 
 }  // namespace
@@ -818,14 +817,15 @@ int LaunchDecodeDim(const DecodeArgs& a, int batch, int D, cudaStream_t s) {
 
 using namespace r4dxb;
 
-/* scratch (splits > 1, no cluster): batch * Hkv * G * splits * (D + 2) floats, 16-byte aligned: the partial sums, then (maximum, sum) pairs */
+/* tile: query rows of a kv head that a CTA takes, 8, 16 (D = 256) or 32 (D = 64, 128); scratch (splits > 1, no cluster): batch * Hkv * G * splits * (D + 2) floats, 16-byte aligned: the partial sums, then (maximum, sum) pairs */
 extern "C" int r4dxb_attn_decode_kv4(const void* q, const void* qg, const void* cache, const int* block_tables, const int* row_slot, int slots,
                                      int table_length, int pool, const int* positions, int pos0, float* scratch, void* out, int T, int batch, int Hq,
-                                     int Hkv, int D, int splits, int chunk, int cluster, int window, int* status, void* stream) {
+                                     int Hkv, int D, int tile, int splits, int chunk, int cluster, int window, int* status, void* stream) {
   if (T < 1 || T > 32 || batch < 1 || batch > 65535 || (row_slot == nullptr && batch != 1) || (row_slot != nullptr && T != 1) || Hkv < 1 || Hq < 1 ||
-      Hq % Hkv || (D != 64 && D != 128 && D != 256) || chunk < 1 || splits < 1 || splits > (cluster ? kMaxCluster : kMaxSplits) || slots < 1 || table_length < 1 || pool < 1 || window < 0)
+      Hq % Hkv || (D != 64 && D != 128 && D != 256) || (tile != 8 && tile != (D == 256 ? kWideTile<256> : kWideTile<64>)) ||
+      chunk < 1 || splits < 1 || splits > (cluster ? kMaxCluster : kMaxSplits) || slots < 1 || table_length < 1 || pool < 1 || window < 0)
     return R4DXB_BAD_ARG;
-  if ((static_cast<long long>(Hq / Hkv) * T + 7) / 8 * Hkv > 65535) return R4DXB_TOO_LARGE;
+  if ((static_cast<long long>(Hq / Hkv) * T + tile - 1) / tile * Hkv > 65535) return R4DXB_TOO_LARGE;
   if (q == nullptr || cache == nullptr || block_tables == nullptr || (positions == nullptr && (row_slot != nullptr || pos0 < 0 || pos0 > 0x7fffffff - T)) || out == nullptr || (splits > 1 && !cluster && scratch == nullptr))
     return R4DXB_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(scratch)) & 15 ||
@@ -845,5 +845,5 @@ extern "C" int r4dxb_attn_decode_kv4(const void* q, const void* qg, const void* 
   a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.splits = splits; a.chunk = chunk; a.pos0 = pos0; a.slots = slots; a.window = window;
   a.end = min(table_length, 0x7fffffff / kv4::kBlock) * kv4::kBlock;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return cluster ? LaunchDecodeDim<true>(a, batch, D, s) : LaunchDecodeDim<false>(a, batch, D, s);
+  return cluster ? LaunchDecodeDim<true>(a, batch, D, tile, s) : LaunchDecodeDim<false>(a, batch, D, tile, s);
 }

@@ -1163,7 +1163,7 @@ def q4x_hc_gate(h, norm_w, w_down_inject, w_up, mid, injv, rstd, x, T: int, hc: 
 # ---- attention over a 4-bit paged KV cache (format: quant/kv4.py) ------------------------------------------------------------------
 register_cuda_sig("r4dxb_attn_precore_kv4", _I, [_P] * 8 + [_I] * 3 + [_P, _P] + [_I] * 5 + [_F, _F, _I, _P])
 register_cuda_sig("r4dxb_kv4_read", _I, [_P] * 3 + [_I] * 3 + [_P] * 3 + [_I] * 3 + [_P])
-register_cuda_sig("r4dxb_attn_decode_kv4", _I, [_P] * 5 + [_I] * 3 + [_P, _I, _P, _P] + [_I] * 9 + [_P, _P])
+register_cuda_sig("r4dxb_attn_decode_kv4", _I, [_P] * 5 + [_I] * 3 + [_P, _I, _P, _P] + [_I] * 10 + [_P, _P])
 register_cuda_sig("r4dxb_attn_prefill_kv4", _I, [_P] * 4 + [_I] * 2 + [_P] + [_I] * 6 + [_P, _I] + [_P] * 3)
 
 KV4_MAX_ROWS = 32           # rows of one sequence that attn_decode_kv4 takes
@@ -1271,8 +1271,19 @@ def kv4_read(cache, block_table, positions, k: Optional[torch.Tensor] = None, v:
 # Clusters of the decode kernel (one CTA to an SM) that run at a time, by CTAs of a cluster: (size, clusters), of the sizes that fill the chip
 _KV4_CLUSTERS = ((16, 7), (9, 15), (6, 22), (5, 26), (4, 33), (3, 45), (2, 74))
 # warps of a CTA, and CTAs of an SM, by head dimension and query rows of a CTA
-_KV4_CTAS = {(64, 8): (8, 2), (64, 16): (16, 1), (64, 32): (12, 1), (128, 8): (12, 1), (128, 16): (12, 1), (128, 32): (8, 1), (256, 8): (8, 1),
-             (256, 16): (8, 1)}
+_KV4_CTAS = {(64, 8): (8, 2), (64, 32): (12, 1), (128, 8): (12, 1), (128, 32): (8, 1), (256, 8): (8, 1), (256, 16): (8, 1)}
+
+
+@functools.lru_cache(maxsize=4096)
+def kv4_row_tile(rows: int, D: int, length: int) -> int:
+    """Query rows of a kv head that a CTA of the decode kernel takes: 8, or 16 (D = 256) or 32 (64, 128), for which blocks are unpacked once.
+
+    A block costs a wide CTA as much as 1.8 (256), 3.5 (128), 3.3 (64) narrow ones, whether its rows are there or not; and narrow CTAs share
+    a short table among more SMs.  us, narrow / wide, by rows: 24 heads over 4 of 256, 8192 keys 24 13.0 / 15.3, 48 17.9 / 18.2, 96 28.7 / 28.5;
+    32517 keys 24 28.1 / 33.3, 36 40.8 / 43.7, 48 46.2 / 43.8; 32 over 8 of 128, 1000 keys 32 7.3 / 10.8, 128 9.6 / 15.7; 8192 keys 24
+    12.9 / 15.2, 32 15.6 / 15.6, 64 23.6 / 21.1; 32517 keys 24 28.8 / 32.9, 32 38.7 / 33.4."""
+    wide, worth = (16, 1.8) if D == 256 else (32, 3.5 if D == 128 else 3.3)
+    return 8 if length * rows <= 24576 or -(-rows // 8) <= worth * -(-rows // wide) else wide
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1288,7 +1299,7 @@ def kv4_splits(rows: int, Hkv: int, batch: int, length: int, D: int) -> tuple:
     62 38 29 28 33 37 us; 32 over 8 of 128 36 26 31 34 38 45; 64 sequences up to 1000 keys of the first 19 37 42 46 55 59).
     Never so few CTAs that a warp adds up more than 4096 tokens: tensor-core sums round towards zero, by up to 2^-24 of the sum of codes
     (7.5 a token) at each of its blocks, which stays below 0.1 % of a mean over equal weights there."""
-    tile = 8 if rows <= 8 else (16 if rows <= 16 or D == 256 else 32)
+    tile = kv4_row_tile(rows, D, length)
     groups = Hkv * batch * -(-rows // tile)
     warps, ctas = _KV4_CTAS[D, tile]
     least, most = -(-length // (256 * warps)), -(-length // 8)
@@ -1337,7 +1348,7 @@ def attn_decode_kv4(q, qg, cache, block_table, positions, out, T: int, Hq: int, 
         _kv4_rows(q, "q", n, dev), _kv4_rows(qg, "qg", 2 * n, dev) if gated else None, cache.data_ptr(), block_table.data_ptr(), _p(row_slot),
         slots, length, pool, None if positions is None else _kv4_ints(positions, "positions", T, dev), pos0,
         scratch.data_ptr() if need else None, _kv4_rows(out, "out", n, dev),
-        rows, batch, Hq, Hkv, D, splits, chunk, cluster, window, _status_word(dev), _raw_stream(dev)), "attn_decode_kv4")
+        rows, batch, Hq, Hkv, D, kv4_row_tile(rows * (Hq // Hkv), D, length), splits, chunk, cluster, window, _status_word(dev), _raw_stream(dev)), "attn_decode_kv4")
     return out
 
 
@@ -1352,12 +1363,11 @@ def kv4_prefill_splits(T: int, Hq: int, Hkv: int, D: int, pos0: int, window: int
     """CTA pairs that share the keys of a row tile (0: the decode kernel takes the call): the fewest us by waves of the 148 SMs.
 
     Few rows leave SMs idle that a long context keeps busy (24 heads over 4 of 256, 128 rows after 29000 keys: 500 us alone, 109 in six), and
-    so does a second wave that is part empty.  Up to 32 rows the decode kernel is faster where its row tiles are few enough (kv heads x row
+    so does a second wave that is part empty.  Up to 32 rows the decode kernel is faster where its wide row tiles are few enough (kv heads x row
     tiles x D up to 6144) or the context short: 16 rows after 29000 keys 69 us against 95, 32 rows 129 against 97, 32 after 1000 17 against 30."""
     if T <= KV4_MAX_ROWS:
         rows = T * (Hq // Hkv)
-        tile = 8 if rows <= 8 else (16 if rows <= 16 or D == 256 else 32)
-        if pos0 + T <= 4096 or Hkv * -(-rows // tile) * D <= KV4_FEW_ROWS_WORK:
+        if pos0 + T <= 4096 or Hkv * -(-rows // (16 if D == 256 else 32)) * D <= KV4_FEW_ROWS_WORK:
             return 0
     tiles = lambda first, end: -(-end // 128) - (max(0, first - window + 1) // 128 if window else 0)  # noqa: E731
     step = 128 if Hq // Hkv % 2 == 0 else 256             # rows of a pair: two heads, else two row tiles

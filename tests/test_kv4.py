@@ -93,6 +93,15 @@ def test_splits_fill_the_chip_once_and_clusters_fit_it():
                         assert not cluster or (1 < s <= 16 and groups <= {16: 7, 9: 15}.get(s, 74))
 
 
+def test_row_tile_follows_rows_and_table():
+    """Few rows and short tables: narrow (8 rows to a CTA); wide where the narrow ones would unpack each block more often than that pays."""
+    from r4dx_b200.ops import kernels as K
+    for D, wide in ((64, 32), (128, 32), (256, 16)):
+        assert {K.kv4_row_tile(r, D, n) for r in (1, 8, 24, 40) for n in (1, 100, 100000)} == {8}
+        assert {K.kv4_row_tile(r, D, 64) for r in (32, 128, 384)} == {8}
+        assert {K.kv4_row_tile(r, D, 4000) for r in (32, 64, 96, 192, 1000)} == {wide}
+
+
 def test_flag_of_the_commands():
     from r4dx_b200.cli.args import cli_parser, server_parser
     for parser in (cli_parser(), server_parser()):
@@ -130,14 +139,14 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu():
     p, odd = 1 << 20, (1 << 20) + 4
 
     def decode(q=p, qg=p, cache=p, tables=p, slots_of=None, slots=1, length=4, pool=4, pos=p, pos0=0, scratch=p, out=p, T=1, batch=1, Hq=4, Hkv=2, D=128,
-               splits=2, chunk=8, cluster=0, window=0):
-        return L.r4dxb_attn_decode_kv4(q, qg, cache, tables, slots_of, slots, length, pool, pos, pos0, scratch, out, T, batch, Hq, Hkv, D, splits, chunk,
-                                       cluster, window, None, None)
+               tile=8, splits=2, chunk=8, cluster=0, window=0):
+        return L.r4dxb_attn_decode_kv4(q, qg, cache, tables, slots_of, slots, length, pool, pos, pos0, scratch, out, T, batch, Hq, Hkv, D, tile,
+                                       splits, chunk, cluster, window, None, None)
 
     for kw in (dict(T=0), dict(T=33), dict(batch=2), dict(batch=0), dict(slots_of=p, T=2), dict(Hq=3), dict(Hkv=0), dict(D=96), dict(splits=0),
                dict(splits=257), dict(splits=17, cluster=1), dict(chunk=0), dict(window=-1), dict(length=0), dict(pool=0), dict(slots=0), dict(q=None),
                dict(cache=None), dict(tables=None), dict(pos=None, pos0=-1), dict(pos=None, slots_of=p), dict(out=None), dict(scratch=None), dict(q=odd), dict(cache=odd), dict(out=odd),
-               dict(scratch=odd), dict(slots_of=p, batch=70000)):
+               dict(scratch=odd), dict(slots_of=p, batch=70000), dict(tile=16), dict(tile=0), dict(D=256, tile=32), dict(D=64, tile=16)):
         assert decode(**kw) == bad, kw
     assert decode(Hq=1 << 20, Hkv=1 << 16) == large
 

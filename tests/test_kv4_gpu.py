@@ -433,6 +433,28 @@ def test_two_streams_at_once_and_rows_behind_the_last_one(K):
         assert (state[i][3][1:] == 7.0).all()
 
 
+@pytest.fixture
+def wide_tiles(K, monkeypatch):
+    """Every decode call takes the kernel of many rows to a CTA, as calls of many rows over long tables do."""
+    monkeypatch.setattr(K, "kv4_row_tile", lambda rows, D, length: 16 if D == 256 else 32)
+    K.kv4_splits.cache_clear()
+    yield
+    K.kv4_splits.cache_clear()
+
+
+@pytest.mark.parametrize("case", [c for c in DECODE if c[3] > 1 or c[1] // c[2] > 4] + [
+    (256, 24, 4, 8, 9000, 0, True, None), (128, 32, 8, 16, 7000, 0, False, None), (64, 12, 2, 32, 3000, 1000, True, None)])
+def test_decode_attention_in_wide_row_tiles(K, wide_tiles, case):
+    test_decode_attention(K, *case)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_nan_and_missing_blocks_in_wide_row_tiles(K, wide_tiles, D):
+    test_nan_keys_and_values_reach_the_rows_that_see_them_only(K, D)
+    test_positions_far_behind_the_table(K, D, None)
+    test_rows_in_any_order_of_positions(K)
+
+
 def test_large_scores_and_uniform_attention(K):
     """One key that takes all the weight, late, so that everything before it is scaled away; and equal keys over a long context, where the
     result is a small mean of large terms."""
