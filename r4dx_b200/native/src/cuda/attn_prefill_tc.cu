@@ -85,6 +85,7 @@ struct Control {
   uint32_t tmem_base;
   int abort_flag;
   float row[2][2][kQRows];                               // [tile parity][half of the keys]: what the two warps of a row exchange
+  float inv[kQRows];                                     // 4-bit cache: 1 / l of the rows
   int nan_groups[kQRows];                                // 4-bit cache: groups of 64 columns in which the row sees a NaN among the values
 };
 
@@ -184,6 +185,8 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
   const int per = KV4 ? (tiles + splits - 1) / splits : tiles, skip = KV4 ? static_cast<int>(blockIdx.z) * per : 0;
   const int tile0 = kv_first / kKvTile + skip, ntiles = min(per, tiles - skip);
   if constexpr (KV4) {
+    // Before the allocation of tensor memory, too: a kernel that this one waits for may still have its own before it.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (ntiles <= 0) {                                // no tile is left for this part: no row sees any of it
       for (int r = threadIdx.x; r < rows; r += kThreads)
         a.part_ml[(static_cast<size_t>(blockIdx.z) * a.T + q0 + r) * a.Hq + hq] = make_float2(-INFINITY, 0.f);
@@ -221,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
   if (warp > kMmaWarp) {
     // ---------------- conversion warps: Q once, then this CTA's half of K and of V^T of every key tile ----------------
     const int tid = threadIdx.x - (kMmaWarp + 1) * 32, cw = warp - (kMmaWarp + 1);
-    const uint32_t q_full = ptx::MapToRank(ptx::SmemAddr(&ctl->q_full), 0);
+    [[maybe_unused]] const uint32_t q_full = ptx::MapToRank(ptx::SmemAddr(&ctl->q_full), 0);
     const uint32_t k_full = ptx::MapToRank(ptx::SmemAddr(&ctl->k_full[0]), 0), v_full = ptx::MapToRank(ptx::SmemAddr(&ctl->v_full[0]), 0);
     // K: a thread owns 16 dimensions of KI consecutive keys (16 lanes read a row); which of two neighbouring keys it stores first
     // depends on its slab, so that the 32 stores of an instruction spread over all banks.
@@ -458,8 +461,8 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
     };
 
     load_k(0);
-    {
-      const float scale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f * (KV4 ? 1.f : a.k_descale[hkv]);
+    if constexpr (!KV4) {
+      const float scale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f * a.k_descale[hkv];
       auto widen = [&](const uint4& v) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
         uint32_t h[4];
@@ -468,34 +471,14 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
           const __half2 p = __floats2half2_rn(BfLo(w[j]) * scale, BfHi(w[j]) * scale);
           h[j] = *reinterpret_cast<const uint32_t*>(&p);
         }
-        if constexpr (KV4)                      // channels 0 4 1 5 2 6 3 7
-          return make_uint4(__byte_perm(h[0], h[2], 0x5410), __byte_perm(h[0], h[2], 0x7632), __byte_perm(h[1], h[3], 0x5410), __byte_perm(h[1], h[3], 0x7632));
-        else
-          return make_uint4(h[0], h[1], h[2], h[3]);
+        return make_uint4(h[0], h[1], h[2], h[3]);
       };
-      if constexpr (KV4) {
-        constexpr int kAhead = 8;               // loads of a thread in flight
-        for (int i0 = tid; i0 < kQRows * (D / 8); i0 += kAhead * kConvThreads) {
-          uint4 v[kAhead];
-#pragma unroll
-          for (int k = 0; k < kAhead; ++k) {
-            const int i = i0 + k * kConvThreads, r = i / (D / 8), c = i % (D / 8);
-            v[k] = r < rows ? __ldg(reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(q0 + r) * a.Hq + hq) * D + c * 8)) : make_uint4(0u, 0u, 0u, 0u);
-          }
-#pragma unroll
-          for (int k = 0; k < kAhead; ++k) {
-            const int i = i0 + k * kConvThreads, r = i / (D / 8), c = i % (D / 8);
-            if (r < kQRows) *reinterpret_cast<uint4*>(Qs + (c >> 3) * (kQRows * 128) + Sw128(r, c & 7)) = widen(v[k]);
-          }
-        }
-      } else {
 #pragma unroll 4
-        for (int i = tid; i < kQRows * (D / 8); i += kConvThreads) {
-          const int r = i / (D / 8), c = i % (D / 8);
-          uint4 o = make_uint4(0u, 0u, 0u, 0u);
-          if (r < rows) o = widen(*reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(q0 + r) * a.Hq + hq) * D + c * 8));
-          *reinterpret_cast<uint4*>(Qs + (c >> 3) * (kQRows * 128) + Sw128(r, c & 7)) = o;
-        }
+      for (int i = tid; i < kQRows * (D / 8); i += kConvThreads) {
+        const int r = i / (D / 8), c = i % (D / 8);
+        uint4 o = make_uint4(0u, 0u, 0u, 0u);
+        if (r < rows) o = widen(*reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(q0 + r) * a.Hq + hq) * D + c * 8));
+        *reinterpret_cast<uint4*>(Qs + (c >> 3) * (kQRows * 128) + Sw128(r, c & 7)) = o;
       }
       ptx::FenceProxyAsyncShared();
       __syncwarp();
@@ -524,34 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
       }
     }
     // the output gates of this CTA's rows, into K's buffers once the last scores have read them
-    if constexpr (KV4) {
-      // (16-byte aligned; eight loads a thread in flight, the first ones before the wait)
-      if (ok && a.gated && !partial) {
-        constexpr int kAhead = 8, kPieces = kQRows * (D / 8);
-        const __nv_bfloat16* gates = a.qg + (static_cast<size_t>(q0) * a.Hq + hq) * 2 * D + D;
-        const size_t row_step = static_cast<size_t>(a.Hq) * 2 * D;
-        uint4 g[kAhead];
-        auto fetch = [&](int i0) {
-#pragma unroll
-          for (int k = 0; k < kAhead; ++k) {
-            const int i = i0 + k * kConvThreads, r = i / (D / 8);
-            g[k] = i < kPieces && r < rows ? __ldg(reinterpret_cast<const uint4*>(gates + r * row_step + i % (D / 8) * 8)) : make_uint4(0u, 0u, 0u, 0u);
-          }
-        };
-        fetch(tid);
-        ok = ptx::WarpMbarWait(&ctl->s_full[(ntiles - 1) & 1], static_cast<uint32_t>((ntiles - 1) >> 1) & 1u, abort_flag, 13);
-        for (int i0 = tid; i0 < kPieces && ok; i0 += kAhead * kConvThreads) {
-          if (i0 != tid) fetch(i0);
-#pragma unroll
-          for (int k = 0; k < kAhead; ++k) {
-            const int i = i0 + k * kConvThreads;
-            if (i < kPieces) *reinterpret_cast<uint4*>(Ks + GateChunk<D>(i / (D / 8), i % (D / 8))) = g[k];
-          }
-        }
-        __syncwarp();
-        if (ok && lane == 0) ptx::MbarArrive(&ctl->gates);
-      }
-    } else {
+    if constexpr (!KV4) {
       if (ok && a.gated) ok = ptx::WarpMbarWait(&ctl->s_full[(ntiles - 1) & 1], static_cast<uint32_t>((ntiles - 1) >> 1) & 1u, abort_flag, 13);
       if (ok && a.gated) {
 #pragma unroll 4
@@ -623,6 +579,34 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
     const int last_key = limits && r < rows ? max(qp, min(key_limit[q0 + r], kv_limit - 1)) : qp;
     const uint32_t t_lane = tbase + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t p_full = ptx::MapToRank(ptx::SmemAddr(&ctl->p_full[0]), 0);
+    if constexpr (KV4) {
+      // Q, which these warps have the time to bring.  (Eight loads of a thread at a time: all 16 at D = 256 took 7300 clocks, these
+      // 3900.)
+      const float scale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;
+      constexpr int kThreadsQ = kSoftmaxWarps * 32, kAhead = D / 8 * kQRows / kThreadsQ < 8 ? D / 8 * kQRows / kThreadsQ : 8;
+#pragma unroll 1
+      for (int i0 = threadIdx.x; i0 < kQRows * (D / 8); i0 += kAhead * kThreadsQ) {
+        uint4 v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int i = i0 + k * kThreadsQ, row = i / (D / 8), c = i % (D / 8);
+          v[k] = row < rows ? __ldg(reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(q0 + row) * a.Hq + hq) * D + c * 8)) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int i = i0 + k * kThreadsQ, row = i / (D / 8), c = i % (D / 8);
+          const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+          uint32_t h[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) h[j] = Bits(__floats2half2_rn(BfLo(w[j]) * scale, BfHi(w[j]) * scale));
+          *reinterpret_cast<uint4*>(Qs + (c >> 3) * (kQRows * 128) + Sw128(row, c & 7)) =      // channels 0 4 1 5 2 6 3 7
+              make_uint4(__byte_perm(h[0], h[2], 0x5410), __byte_perm(h[0], h[2], 0x7632), __byte_perm(h[1], h[3], 0x5410), __byte_perm(h[1], h[3], 0x7632));
+        }
+      }
+      ptx::FenceProxyAsyncShared();
+      __syncwarp();
+      if (lane == 0) ptx::MbarArriveRemote(ptx::MapToRank(ptx::SmemAddr(&ctl->q_full), 0));
+    }
     float m_used = -INFINITY, l_run = 0.f;
     bool ok = true;
     // (both warps of a row reach every one of these, also after a wait that ran out)
@@ -712,36 +696,18 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
     }
     // ---------------- epilogue: O / l, output gate, bf16 rows; each warp half of the columns ----------------
     const float l = l_run + exchange(ntiles & 1, l_run);
-    if (ok && a.gated && !partial) ok = ptx::WarpMbarWait(&ctl->gates, 0, abort_flag, 10);
-    if (ok) ok = ptx::WarpMbarWait(&ctl->o_final, 0, abort_flag, 9);
     if constexpr (KV4) {
-      if (partial) {
-        // this share's sums as they are (NaN where a wait ran out), joined by a kernel of their own
-        const size_t at = (static_cast<size_t>(blockIdx.z) * a.T + q0 + r) * a.Hq + hq;
-        if (r < rows && half == 0) a.part_ml[at] = make_float2(ok ? m_used : 0.f, ok ? l : __uint_as_float(0x7fc00000u));
-        if (ok) {
-          ptx::TcFenceAfter();
-          const int nan_groups = ctl->nan_groups[r];
-          float* dst = a.part_acc + at * D + half * (D / 2);
-#pragma unroll 1
-          for (int c0 = 0; c0 < D / 2; c0 += 32) {
-            uint32_t o[32];
-            ptx::TmemLoad32x32(t_lane + half * (D / 2) + c0, o);
-            ptx::TmemLoadWait();
-            const bool nan = nan_groups >> ((half * (D / 2) + c0) >> 6) & 1;
-            if (r < rows) {
-#pragma unroll
-              for (int v = 0; v < 8; ++v)
-                *reinterpret_cast<uint4*>(dst + c0 + 4 * v) = nan ? make_uint4(0x7fc00000u, 0x7fc00000u, 0x7fc00000u, 0x7fc00000u) : make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
-            }
-          }
-        }
-      }
+      // (a share of keys leaves its maximum and sum, NaN where a wait ran out; the rows follow below)
+      if (half == 0) ctl->inv[r] = l == 0.f ? 0.f : 1.f / l;
+      if (partial && r < rows && half == 0)
+        a.part_ml[(static_cast<size_t>(blockIdx.z) * a.T + q0 + r) * a.Hq + hq] = make_float2(ok ? m_used : 0.f, ok ? l : __uint_as_float(0x7fc00000u));
+    } else {
+      if (ok && a.gated) ok = ptx::WarpMbarWait(&ctl->gates, 0, abort_flag, 10);
+      if (ok) ok = ptx::WarpMbarWait(&ctl->o_final, 0, abort_flag, 9);
     }
-    if (ok && !partial) {
+    if constexpr (!KV4) if (ok) {
       ptx::TcFenceAfter();
-      const float inv = (l > 0.f ? 1.f / l : 0.f) * (KV4 ? 1.f : a.v_descale[hkv]);
-      const int nan_groups = KV4 ? ctl->nan_groups[r] : 0;
+      const float inv = (l > 0.f ? 1.f / l : 0.f) * a.v_descale[hkv];
       // a lane's half row, staged where Q (first half) or V (second) was and sent off as one copy
       constexpr int kHalfRow = D / 2 * 2, kStageRow = kHalfRow + 16;
       static_assert(kQRows * kStageRow <= kQBytes && kQRows * kStageRow <= 2 * kVBytes, "the output tile fits");
@@ -757,19 +723,13 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
             float x[8];
 #pragma unroll
             for (int c = 0; c < 8; ++c) x[c] = __uint_as_float(o[8 * v + c]) * inv;
-            if constexpr (KV4) {
-              if (nan_groups >> ((half * (D / 2) + c0) >> 6) & 1) {
-#pragma unroll
-                for (int c = 0; c < 8; ++c) x[c] = __uint_as_float(0x7fc00000u);
-              }
-            }
             if (a.gated) {
               const uint4 g = *reinterpret_cast<const uint4*>(Ks + GateChunk<D>(r, (half * (D / 2) + c0) / 8 + v));
               const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
-                x[2 * c] *= KV4 ? SigmoidApprox(BfLo(gw[c])) : Sigmoid(BfLo(gw[c]));
-                x[2 * c + 1] *= KV4 ? SigmoidApprox(BfHi(gw[c])) : Sigmoid(BfHi(gw[c]));
+                x[2 * c] *= Sigmoid(BfLo(gw[c]));
+                x[2 * c + 1] *= Sigmoid(BfHi(gw[c]));
               }
             }
             *reinterpret_cast<uint4*>(stage + (c0 + 8 * v) * 2) =
@@ -781,8 +741,75 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
       if (r < rows) {
         ptx::BulkStore(a.out + (static_cast<size_t>(q0 + r) * a.Hq + hq) * D + half * (D / 2), ptx::SmemAddr(stage), kHalfRow);
         ptx::BulkStoreCommit();
-        if constexpr (KV4) ptx::BulkStoreWaitRead();          // (the rows have left shared memory; they arrive before the kernel ends)
-        else ptx::BulkStoreWait();
+        ptx::BulkStoreWait();
+      }
+    }
+  }
+
+  if constexpr (KV4) {
+    // ---------------- epilogue of the 4-bit cache: the sums to shared memory as they are, then whole rows through 1 / l and gate ----------------
+    if (warp != kMmaWarp) {
+      const int worker = warp < kMmaWarp ? threadIdx.x : threadIdx.x - 32;
+      // eight columns of every kStep-th row: `piece` of the row's, `col` of its half's
+      constexpr int kRowPieces = D / 8, kWorkers = (kSoftmaxWarps + kConvWarps) * 32, kStep = kWorkers / kRowPieces, kPieces = kQRows / kStep;
+      static_assert(kStep % 8 == 0, "a worker's rows lie alike in shared memory");
+      const int piece = worker % kRowPieces, row0 = worker / kRowPieces, col = piece % (kRowPieces / 2);
+      uint4 gate[kPieces];                       // on their way while the sums are
+      if (a.gated && !partial) {
+        const __nv_bfloat16* at = a.qg + ((static_cast<size_t>(q0 + row0) * a.Hq + hq) * 2 + 1) * D + piece * 8;
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k, at += static_cast<size_t>(kStep) * a.Hq * 2 * D)
+          gate[k] = row0 + k * kStep < rows ? __ldg(reinterpret_cast<const uint4*>(at)) : make_uint4(0u, 0u, 0u, 0u);
+      }
+      asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+      ptx::WarpMbarWait(&ctl->o_final, 0, abort_flag, 9);
+      ptx::TcFenceAfter();
+      // Columns of the first half lie where Q was, of the second where V was (the products have read both): rows of 2 D bytes each, every
+      // second four columns in their second half, places permuted so that the lanes of rows and those of columns meet all banks.
+      auto place = [&](int row, int four) { return row * 2 * D + ((((four >> 1) + (four & 1) * (D / 16)) ^ (row & 7)) << 4); };
+      const int part = worker >> 7, r = (warp & 3) * 32 + lane;              // part: a quarter of the columns
+      const uint32_t t_part = tbase + (static_cast<uint32_t>((warp & 3) * 32) << 16) + part * (D / 4);
+      constexpr int kCols = D / 4 < 32 ? D / 4 : 32;
+#pragma unroll
+      for (int c0 = 0; c0 < D / 4; c0 += kCols) {
+        uint32_t o[kCols];
+        if constexpr (kCols == 32) ptx::TmemLoad32x32(t_part + c0, o);
+        else ptx::TmemLoad32x16(t_part + c0, o);
+        ptx::TmemLoadWait();
+#pragma unroll
+        for (int v = 0; v < kCols / 4; ++v)
+          *reinterpret_cast<uint4*>((part < 2 ? Qs : Vs) + place(r, ((part & 1) * (D / 4) + c0) / 4 + v)) = make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+      }
+      asm volatile("bar.sync 5, %0;" ::"n"(kWorkers) : "memory");
+      if (*abort_flag == 0) {
+        const unsigned char* from = piece < kRowPieces / 2 ? Qs : Vs;
+        const unsigned char *lo_at = from + place(row0, 2 * col), *hi_at = from + place(row0, 2 * col + 1);
+        const size_t first = static_cast<size_t>(q0 + row0) * a.Hq + hq, row_step = static_cast<size_t>(kStep) * a.Hq * D;
+        __nv_bfloat16* out = a.out + first * D + piece * 8;
+        float* sums = partial ? a.part_acc + (static_cast<size_t>(blockIdx.z) * a.T * a.Hq + first) * D + piece * 8 : nullptr;
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+          const int row = row0 + k * kStep;
+          if (row >= rows) break;
+          float4 lo = *reinterpret_cast<const float4*>(lo_at + k * kStep * 2 * D), hi = *reinterpret_cast<const float4*>(hi_at + k * kStep * 2 * D);
+          if (ctl->nan_groups[row] >> (piece >> 3) & 1) lo.x = lo.y = lo.z = lo.w = hi.x = hi.y = hi.z = hi.w = __uint_as_float(0x7fc00000u);
+          if (partial) {
+            *reinterpret_cast<float4*>(sums + k * row_step) = lo;
+            *reinterpret_cast<float4*>(sums + k * row_step + 4) = hi;
+          } else {
+            const float inv = ctl->inv[row];
+            float x[8] = {lo.x * inv, lo.y * inv, lo.z * inv, lo.w * inv, hi.x * inv, hi.y * inv, hi.z * inv, hi.w * inv};
+            if (a.gated) {
+              const uint32_t g[4] = {gate[k].x, gate[k].y, gate[k].z, gate[k].w};
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                x[2 * c] *= SigmoidApprox(BfLo(g[c]));
+                x[2 * c + 1] *= SigmoidApprox(BfHi(g[c]));
+              }
+            }
+            *reinterpret_cast<uint4*>(out + k * row_step) = make_uint4(PackBf16(x[0], x[1]), PackBf16(x[2], x[3]), PackBf16(x[4], x[5]), PackBf16(x[6], x[7]));
+          }
+        }
       }
     }
   }
@@ -803,6 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
 // The shares of split keys joined: D / 4 threads a row, its gate and its rounding.
 template <int D>
 __global__ void __launch_bounds__(256) JoinKv4Kernel(Kv4Args a) {
+  PdlEnter();
   constexpr int kRow = D / 4;
   const long long row = static_cast<long long>(blockIdx.x) * (256 / kRow) + threadIdx.x / kRow, rows = static_cast<long long>(a.T) * a.Hq;
   if (row >= rows) return;
@@ -849,19 +877,21 @@ int LaunchTc(const Args<KV4>& a, cudaStream_t s) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = KV4 && g_use_pdl ? 2 : 1;
   e = cudaLaunchKernelEx(&cfg, kern, a);
   if (e != cudaSuccess) return static_cast<int>(e);
   if constexpr (KV4) {
     if (a.splits > 1) {
-      ++g_launch_count;
       constexpr int kPer = 256 / (D / 4);
-      JoinKv4Kernel<D><<<static_cast<unsigned>((static_cast<long long>(a.T) * a.Hq + kPer - 1) / kPer), 256, 0, s>>>(a);
+      const int rc = LaunchPdl(JoinKv4Kernel<D>, dim3(static_cast<unsigned>((static_cast<long long>(a.T) * a.Hq + kPer - 1) / kPer)), dim3(256), 0, s, a);
+      if (rc) return rc;
     }
   }
   return FinishLaunch();
