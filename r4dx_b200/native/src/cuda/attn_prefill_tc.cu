@@ -216,10 +216,22 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
     ptx::TmemRelinquishPair();
   }
   ptx::TcFenceBefore();
-  __syncthreads();
-  ptx::ClusterSync();                                 // the partner's barriers exist before anything arrives at them
-  ptx::TcFenceAfter();
-  const uint32_t tbase = ctl->tmem_base;
+  // The partner's barriers exist before anything arrives at them.  (4-bit cache: each role waits for that, and for tensor memory, which takes
+  // 1500 clocks, with its first loads under way.)
+  uint32_t tbase = 0u;
+  auto join = [&]() {
+    ptx::ClusterWait();
+    ptx::TcFenceAfter();
+    tbase = ctl->tmem_base;
+  };
+  if constexpr (KV4) {
+    ptx::ClusterArrive();
+  } else {
+    __syncthreads();
+    ptx::ClusterSync();
+    ptx::TcFenceAfter();
+    tbase = ctl->tmem_base;
+  }
 
   if (warp > kMmaWarp) {
     // ---------------- conversion warps: Q once, then this CTA's half of K and of V^T of every key tile ----------------
@@ -461,6 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
     };
 
     load_k(0);
+    if constexpr (KV4) join();
     if constexpr (!KV4) {
       const float scale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f * a.k_descale[hkv];
       auto widen = [&](const uint4& v) {
@@ -529,6 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
     }
   } else if (warp == kMmaWarp) {
     // ---------------- MMA issuer (one thread of the first CTA) ----------------
+    if constexpr (KV4) join();
     if (rank == 0 && lane == 0) {
       constexpr uint32_t idesc_s = ptx::UmmaInstrDescF16(2 * kQRows, kKvTile, false);
       constexpr uint32_t idesc_o = ptx::UmmaInstrDescF16(2 * kQRows, D, false);
@@ -577,8 +591,6 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
     const int half = warp >> 2, r = (warp & 3) * 32 + lane;
     const int qp = a.pos0 + q0 + r;                               // position of this row's query
     const int last_key = limits && r < rows ? max(qp, min(key_limit[q0 + r], kv_limit - 1)) : qp;
-    const uint32_t t_lane = tbase + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t p_full = ptx::MapToRank(ptx::SmemAddr(&ctl->p_full[0]), 0);
     if constexpr (KV4) {
       // Q, which these warps have the time to bring.  (Eight loads of a thread at a time: all 16 at D = 256 took 7300 clocks, these
       // 3900.)
@@ -604,9 +616,11 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
         }
       }
       ptx::FenceProxyAsyncShared();
-      __syncwarp();
+      join();
       if (lane == 0) ptx::MbarArriveRemote(ptx::MapToRank(ptx::SmemAddr(&ctl->q_full), 0));
     }
+    const uint32_t t_lane = tbase + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t p_full = ptx::MapToRank(ptx::SmemAddr(&ctl->p_full[0]), 0);
     float m_used = -INFINITY, l_run = 0.f;
     bool ok = true;
     // (both warps of a row reach every one of these, also after a wait that ran out)
