@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(256, D == 256 || AHEAD == 1 ? 4 : 3) PrecoreKv
 
 // Rows read back: a thread has one word (eight channels) of a row and up to ITEMS of its 2 Hkv heads' keys and values, whose codes and pairs it
 // asks for at once.  (A thread per value word, each with the row's position and table entry to find first, took 62 us for 32517 rows of
-// 8 heads of 128 where the bytes take 26.)
+// 8 heads of 128, this one 31; their bytes take 26.)
 template <int D, int ITEMS>
 __global__ void __launch_bounds__(256) ReadKv4Kernel(const uint32_t* __restrict__ cache, kv4::Table table, const int* __restrict__ positions,
                                                      const int* __restrict__ row_slot, int slots, __nv_bfloat16* __restrict__ k,

@@ -1364,7 +1364,7 @@ def kv4_prefill_splits(T: int, Hq: int, Hkv: int, D: int, pos0: int, window: int
 
     Few rows leave SMs idle that a long context keeps busy (24 heads over 4 of 256, 128 rows after 29000 keys: 500 us alone, 109 in six), and
     so does a second wave that is part empty.  Up to 32 rows the decode kernel is faster where its wide row tiles are few enough (kv heads x row
-    tiles x D up to 6144) or the context short: 16 rows after 29000 keys 69 us against 95, 32 rows 129 against 97, 32 after 1000 17 against 30."""
+    tiles x D up to 6144) or the context short: 16 rows after 29000 keys 71 us against 95, 32 rows 133 against 96, 32 after 1000 14 against 18."""
     if T <= KV4_MAX_ROWS:
         rows = T * (Hq // Hkv)
         if pos0 + T <= 4096 or Hkv * -(-rows // (16 if D == 256 else 32)) * D <= KV4_FEW_ROWS_WORK:
