@@ -122,7 +122,6 @@ __device__ __forceinline__ float Exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ __half2 AsHalf2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
 __device__ __forceinline__ uint32_t Bits(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
 __device__ __forceinline__ uint32_t PackHalf(float lo, float hi) { return Bits(__floats2half2_rn(lo, hi)); }
 // codes of the lowest bits of a word's halves (n 2^-24 as fp16), of the next four (n 2^-20)

@@ -622,6 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
       }
       ptx::FenceProxyAsyncShared();
       join();
+      __syncwarp();                              // (the others' arrivals came before the stores: they say nothing of this warp's lanes)
       if (lane == 0) ptx::MbarArriveRemote(ptx::MapToRank(ptx::SmemAddr(&ctl->q_full), 0));
     }
     const uint32_t t_lane = tbase + (static_cast<uint32_t>((warp & 3) * 32) << 16);

@@ -273,6 +273,8 @@ PREFILL = [
     (128, 5, 5, 257, 300, 64, True, None), (64, 32, 8, 100, 29, 0, False, None), (64, 3, 3, 300, 1000, 17, True, None), (256, 2, 2, 17, 2000, 0, False, None),
     (64, 4, 2, 513, 0, 0, True, None), (128, 2, 1, 40, 16, 1, False, None), (256, 4, 2, 128, 128, 0, False, None),
     (256, 24, 4, 16, 3000, 0, True, None), (128, 8, 2, 130, 2500, 0, False, 4), (64, 6, 2, 140, 900, 300, True, 5), (256, 2, 1, 300, 200, 0, True, 7),
+    # the kernel itself where the decode kernel would take the call
+    (256, 24, 4, 1, 0, 0, True, 1), (64, 4, 2, 5, 40, 0, True, 1), (128, 3, 1, 31, 700, 90, True, 2), (256, 5, 1, 32, 127, 0, False, 1), (128, 8, 2, 1, 4000, 0, True, 6),
 ]
 
 
@@ -431,6 +433,46 @@ def test_two_streams_at_once_and_rows_behind_the_last_one(K):
     for i, p in enumerate(pools):
         check(state[i][3][:1], attention(q[i], p.k[0], p.v[0], torch.tensor([n - 1])), p.v[0])
         assert (state[i][3][1:] == 7.0).all()
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,T,start,splits", [(256, 24, 4, 130, 0, None), (128, 8, 2, 64, 1500, 3), (64, 8, 8, 300, 37, 1)])
+def test_calls_in_a_row_see_what_the_calls_before_them_wrote(K, D, Hq, Hkv, T, start, splits):
+    """Writer, prompt and read-back one after the other on two streams, rows anew each time: the same bits as with a synchronisation after
+    every call (a kernel may start before the one in front of it has ended, but not read its rows)."""
+    g = torch.Generator().manual_seed(D + T)
+    n, rounds = start + T, 6
+    blocks = (n + 15) // 16
+    q, k, v = (torch.randn(rounds, rows_, h, D, generator=g).to(BF).cuda() for rows_, h in ((T, Hq), (n, Hkv), (n, Hkv)))
+    qg = torch.randn(rounds, T, Hq, 2 * D, generator=g).to(BF).cuda()
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    table = torch.arange(blocks, dtype=torch.int32, device="cuda").flip(0).contiguous()
+
+    def run(cache, after):
+        got = []
+        for i in range(rounds):
+            K.kv4_write(k[i], v[i], pos, table, cache)
+            after()
+            out = torch.empty(T, Hq, D, dtype=BF, device="cuda")
+            K.attn_prefill_kv4(q[i], qg[i], cache, table, out, T, Hq, Hkv, D, start, True, splits=splits)
+            after()
+            got += [out, *K.kv4_read(cache, table, pos)]
+            after()
+        return got
+
+    want = run(K.kv4_cache(blocks, Hkv, D), torch.cuda.synchronize)
+    streams, caches = [torch.cuda.Stream() for _ in range(2)], [K.kv4_cache(blocks, Hkv, D) for _ in range(2)]
+    torch.cuda.synchronize()
+    results = []
+    for stream, cache in zip(streams, caches):
+        with torch.cuda.stream(stream):
+            results.append(run(cache, lambda: None))
+    torch.cuda.synchronize()
+    K.check_gemm_status(want[0].device)
+    for got in results:
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+    check(want[0].cpu(), attention(q[0].cpu(), kv4.round_trip(k[0].cpu()).double(), kv4.round_trip(v[0].cpu()).double(), torch.arange(start, n))
+          * torch.sigmoid(qg[0, ..., D:].cpu().double()), kv4.round_trip(v[0].cpu()).double(),
+          slack=score_slack(q[0].cpu(), kv4.round_trip(k[0].cpu()).double(), kv4.round_trip(v[0].cpu()).double()))
 
 
 @pytest.fixture
