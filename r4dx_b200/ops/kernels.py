@@ -1256,11 +1256,10 @@ def kv4_read(cache, block_table, positions, k: Optional[torch.Tensor] = None, v:
     T = positions.numel()
     dev, slots, length, pool, Hkv, D = _kv4_pool(cache, block_table, row_slot, T)
     n = T * Hkv * D
-    if k is None and v is None:
-        k, v = torch.empty((2, T, Hkv, D), dtype=BF, device=cache.device).unbind()
-    else:
-        k = k if k is not None else torch.empty((T, Hkv, D), dtype=BF, device=cache.device)
-        v = v if v is not None else torch.empty((T, Hkv, D), dtype=BF, device=cache.device)
+    if k is None:                                # (the cheapest of torch's ways to an empty tensor: 1.7 us, a pair by unbind 4.4)
+        k = torch.empty_strided((T, Hkv, D), (Hkv * D, D, 1), dtype=BF, device=dev)
+    if v is None:
+        v = torch.empty_strided((T, Hkv, D), (Hkv * D, D, 1), dtype=BF, device=dev)
     if T:
         _check(_lib().r4dxb_kv4_read(
             cache.data_ptr(), block_table.data_ptr(), _p(row_slot), slots, length, pool, _kv4_ints(positions, "positions", T, dev),
@@ -1340,7 +1339,7 @@ def attn_decode_kv4(q, qg, cache, block_table, positions, out, T: int, Hq: int, 
     need = 0 if splits == 1 or cluster else n * splits // D * (D + 2)
     if need:
         if scratch is None:
-            scratch = torch.empty(need, dtype=torch.float32, device=cache.device)
+            scratch = cache.new_empty(need, dtype=torch.float32)
         elif scratch.dtype is not torch.float32 or scratch.get_device() != dev or not scratch.is_contiguous() or scratch.numel() < need \
                 or scratch.data_ptr() & 15:
             raise KernelError(f"scratch must be a contiguous, 16-byte aligned fp32 tensor of {need} or more elements on cuda:{dev}")
