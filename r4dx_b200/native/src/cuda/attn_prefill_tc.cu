@@ -20,7 +20,7 @@
 // too: 3440 clocks for 64 keys, where the products take 1024.  In pairs each product is twice as long, reads half of B and meets half
 // of the conversions.  What bounds it now is the chain scores -> softmax -> products over two score buffers (the accumulator takes the
 // other half of tensor memory): 3300 clocks from announced probabilities to the scores after next, about as many in the softmax,
-// whose 128 x 128 exponentials alone take 1024.  Output gates wait in K's buffers and output rows leave as one copy per row
+// whose 128 x 128 exponentials alone take 1024.  Output gates (of the fp8 cache) wait in K's buffers and output rows leave as one copy per row
 // half: read and written directly by the lanes that own the rows, they took 25k clocks a CTA.
 // 8192 rows, 24 heads over 4, D = 256: 1623 -> 953 us (865 TFLOP/s); 1024 rows after 29000 1499 -> 916; 333 rows 50 -> 29;
 // 32 heads over 8, D = 128, 8192 rows 1304 -> 913.
@@ -150,7 +150,7 @@ __device__ __forceinline__ void Kv4ToHalf(uint32_t w, __half2 s, __half2 lo, uin
 //   - the softmax warps bring Q, and all 16 warps write whole rows at the end, their gates loaded ahead: of a CTA of one tile (24 heads over 4 of
 //     256) 26000 clocks became 21500, half of which are start and end.
 // The same chain bounds it as the fp8 cache's (1024 rows after 8000 keys: tensor pipe 45 %, issue slots 50 %); widening codes costs the conversion
-// warps no more than widening fp8 does.  24 heads over 4 of 256: 333 rows 15.1 us, 1024 after 29000 743 to 788, 8192 810 to 904 by the power that
+// warps no more than widening fp8 does.  24 heads over 4 of 256: 333 rows 15.1 us, 1024 after 29000 721 to 788, 8192 803 to 904 by the power that
 // the chip is left; 32 over 8 of 128, 8192 rows 755; of 64 700.
 template <int D, bool KV4>
 __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) {
