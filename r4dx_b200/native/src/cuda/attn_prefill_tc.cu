@@ -85,8 +85,12 @@ struct Control {
   uint32_t tmem_base;
   int abort_flag;
   float row[2][2][kQRows];                               // [tile parity][half of the keys]: what the two warps of a row exchange
-  float inv[kQRows];                                     // 4-bit cache: 1 / l of the rows
-  int nan_groups[kQRows];                                // 4-bit cache: groups of 64 columns in which the row sees a NaN among the values
+};
+struct Kv4Control : Control {
+  float inv[kQRows];                                     // 1 / l of the rows
+  int nan_groups[kQRows];                                // groups of 64 columns in which the row sees a NaN among the values
+  uint32_t v_top[kConvWarps][4];                         // largest scales and low ends that a warp has met
+  float v_back[4];                                       // 1 / the power of two that the group's values are taken by
 };
 
 __device__ __forceinline__ uint32_t Fp8x2Bits(uint32_t v16) {
@@ -122,6 +126,18 @@ __device__ __forceinline__ void OrRemote(uint32_t addr, uint32_t bits) {
   asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(addr), "r"(bits) : "memory");
 }
 
+__device__ __forceinline__ void StoreRemote(uint32_t addr, float x) {
+  asm volatile("st.relaxed.cluster.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(x) : "memory");
+}
+// scale and low end of a pair, both times a power of two (exact)
+__device__ __forceinline__ uint32_t Mul2Bf16(uint32_t pair, uint32_t power) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(pair), "r"(power));
+  return r;
+}
+// of a pair without its signs, or the largest halves of several: is one infinite or NaN?
+__device__ __forceinline__ bool NoNumber(uint32_t pair) { return (pair & 0xffffu) >= 0x7f80u || pair >= 0x7f800000u; }
+
 // Four code pairs of a 4-bit word (codes i and i + 4 in the halves of result i) as fp16 values n s + lo: the codes enter the mantissa of
 // 1024 (or, where they lie four bits higher, as 1024 + 16 n), come back out exactly, and one fma rounds to fp16.
 __device__ __forceinline__ __half2 AsHalf2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
@@ -140,6 +156,37 @@ __device__ __forceinline__ void Kv4ToHalf(uint32_t w, __half2 s, __half2 lo, uin
     h[i] = Bits(__hfma2(n0, s, lo));
     h[i + 1] = Bits(__hfma2(n1, s, lo));
   }
+}
+
+// The largest scale and low end of a group among the values of keys `begin` .. `end` - 1 (all conversion warps; a head's block b lies at
+// cache + b page_words).  Called where values are tiny, and kept out of line: its registers are not the kernel's.
+template <int D>
+__device__ __noinline__ uint32_t MostOfGroup(Kv4Control* ctl, kv4::Table table, const uint32_t* cache, size_t page_words, int begin, int end, int tid, int group) {
+  constexpr int NG = kv4::Shape<D>::kGroups, kPieces = 4 * NG;        // pieces: 16 bytes of a block's pairs
+  const uint32_t* at = cache + kv4::Shape<D>::kPart / 4 + 2 * D + tid % kPieces * 4;
+  uint32_t top[NG] = {};
+#pragma unroll 1
+  for (int b = begin / kv4::kBlock + tid / kPieces; b * kv4::kBlock < end; b += kConvThreads / kPieces) {
+    const int blk = table.BlockAt(b);
+    if (blk < 0) continue;
+    const uint4 x = __ldg(reinterpret_cast<const uint4*>(at + blk * page_words));
+    const uint32_t w[4] = {x.x & 0x7fff7fffu, x.y & 0x7fff7fffu, x.z & 0x7fff7fffu, x.w & 0x7fff7fffu};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int kp = b * kv4::kBlock + (tid % kPieces * 4 + i) / NG;
+      if (!NoNumber(w[i]) && kp >= begin && kp < end) top[i % NG] = __vmaxu2(top[i % NG], w[i]);
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    const uint32_t t = __reduce_max_sync(0xffffffffu, top[g] & 0xffffu) | __reduce_max_sync(0xffffffffu, top[g] >> 16) << 16;
+    if (tid % 32 == 0) ctl->v_top[tid / 32][g] = t;
+  }
+  asm volatile("bar.sync 6, %0;" ::"n"(kConvThreads) : "memory");
+  uint32_t most = 0u;
+#pragma unroll
+  for (int w = 0; w < kConvWarps; ++w) most = __vmaxu2(most, ctl->v_top[w][group]);
+  return most;
 }
 
 // KV4: the 4-bit cache (kv4.cuh) in place of the fp8 one; only what the conversion warps load and store differs, and
@@ -164,7 +211,8 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
   unsigned char* Qs = smem;
   unsigned char* Ks = Qs + kQBytes;                   // [2][kKBytes]
   unsigned char* Vs = Ks + 2 * kKBytes;               // [2][kVBytes]
-  Control* ctl = reinterpret_cast<Control*>(Vs + 2 * kVBytes);
+  using Ctl = std::conditional_t<KV4, Kv4Control, Control>;
+  Ctl* ctl = reinterpret_cast<Ctl*>(Vs + 2 * kVBytes);
   volatile int* abort_flag = &ctl->abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -215,6 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
   }
   if constexpr (KV4) {
     if (threadIdx.x < kQRows) ctl->nan_groups[threadIdx.x] = 0;
+    if (threadIdx.x < 4) ctl->v_back[threadIdx.x] = 1.f;
   }
   if (warp == kMmaWarp) {
     ptx::TmemAllocPair(&ctl->tmem_base, kTmemCols);
@@ -268,10 +317,11 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
     uint32_t kcodes[NJ], kpairs[NG], vcodes[VT], vpairs[VT];
     // the blocks of the next tiles' keys and values are looked up a tile ahead: an address that waits for its table entry held a warp up
     // for a quarter of a tile's time
-    auto block_of = [&](int j, int first) {
-      if constexpr (KV4) return a.table.BlockAt(((tile0 + j) * kKvTile + first) >> 4);
+    auto block_index = [&](int b) {
+      if constexpr (KV4) return a.table.BlockAt(b);
       else return 0;
     };
+    auto block_of = [&](int j, int first) { return block_index(((tile0 + j) * kKvTile + first) >> 4); };
     const int kfirst = rank * kHalfTile + kkey;
     int kblk = block_of(0, kfirst), vblk = block_of(0, vtok);
     // where a thread's words lie in a block: the same in every tile, since tiles begin with blocks
@@ -413,17 +463,55 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
       __syncwarp();
       if (lane == 0) ptx::MbarArriveRemote(k_full + (j & 1) * 8);
     };
+    // 4-bit cache: values of ordinary size are widened as they are, none being above 2^15: fp16 keeps those above 6e-5 with all their bits and is off
+    // by 2^-25 at most below.  Where most of the first 32 keys have values below 2^-6 throughout a group of 64 columns, that is no small part of them:
+    // the pair then looks through the scales and low ends of all its keys and takes the group's values times the power of two that brings the
+    // largest to 2^14 .. 2^15, and the sums back in the end.  (Such a look ahead of every call took 10 us of a CTA of 8192 keys at D = 256: 885 us
+    // instead of 803 for 8192 rows of 24 heads over 4.  Each warp looks at the 32 keys for itself: the eight run apart, and a barrier of theirs
+    // once in the beginning, which brings them in step, took 3 %.)
+    uint32_t v_power = 0x3f803f80u;              // of this thread's group, as two bf16
+    constexpr int kOwnGroups = NG > 1 ? NG / 2 : 1;      // of this CTA's columns
+    uint32_t sample[kOwnGroups] = {};            // the pairs of one of the 32 keys
+    const int v_begin = max(kv_first, tile0 * kKvTile), v_end = min((tile0 + ntiles) * kKvTile, kv_limit);      // of the values that are loaded
+    auto load_sample = [&]() {
+      if constexpr (KV4) {
+        const int kp = v_begin + lane, blk = block_index(kp < v_end ? kp >> 4 : -1);
+#pragma unroll
+        for (int g = 0; g < kOwnGroups; ++g)
+          if (blk >= 0) sample[g] = __ldg(cache4 + blk * page_words + kv4::Shape<D>::kPart / 4 + 2 * D + (kp & 15) * NG + rank * NG / 2 + g);
+      }
+    };
+    auto bound = [](uint32_t pair) { return fmaf(15.f, BfLo(pair), BfHi(pair)); };      // of the values that a pair without signs stands for
+    auto choose_power = [&]() {
+      if constexpr (KV4) {
+        bool tiny = false;                       // (the same for all warps)
+#pragma unroll
+        for (int g = 0; g < kOwnGroups; ++g)
+          tiny |= 2 * __popc(__ballot_sync(0xffffffffu, v_begin + lane < v_end && bound(sample[g] & 0x7fff7fffu) < 0.015625f)) > min(32, v_end - v_begin);
+        if (tiny) {
+          const uint32_t most = MostOfGroup<D>(ctl, a.table, cache4, page_words, v_begin, v_end, tid, vgroup);
+          const int exponent = min(max(static_cast<int>(__float_as_uint(bound(most)) >> 23), 15), 254);
+          v_power = static_cast<uint32_t>((268 - exponent) << 7) * 0x10001u;
+          if (lane % VUnits == 0 && cw < 4 && (vword & 7) == 0) {
+            // each CTA's rows have all the columns
+            for (int peer = 0; peer < 2; ++peer)
+              StoreRemote(ptx::MapToRank(ptx::SmemAddr(&ctl->v_back[vgroup]), peer), __uint_as_float(static_cast<uint32_t>(exponent - 14) << 23));
+            asm volatile("fence.acq_rel.cluster;" ::: "memory");
+          }
+        }
+      }
+    };
     unsigned char* v_dst = Vs + (tg >> 3) * kVSlab;
     auto store_v = [&](int j) {
       if constexpr (KV4) {
         unsigned char* at = Vs + (j & 1) * kVBytes + (vtok >> 6) * kVSlab;
-        bool nan = false;
+        uint32_t top = 0u;
 #pragma unroll
-        for (int t = 0; t < VT; ++t) nan |= BfLo(vpairs[t]) != BfLo(vpairs[t]);
-        if (nan) {
+        for (int t = 0; t < VT; ++t) top = __vmaxu2(top, vpairs[t] & 0x7fff7fffu);
+        if (NoNumber(top)) {
 #pragma unroll
           for (int t = 0; t < VT; ++t)
-            if (BfLo(vpairs[t]) != BfLo(vpairs[t])) {
+            if (NoNumber(vpairs[t] & 0x7fff7fffu)) {
               vpairs[t] = 0u;
               const int kp = (tile0 + j) * kKvTile + vtok + t;
               if ((vword & 7) == 0)              // one of the threads of the group
@@ -438,6 +526,8 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
             }
           asm volatile("fence.acq_rel.cluster;" ::: "memory");
         }
+#pragma unroll
+        for (int t = 0; t < VT; ++t) vpairs[t] = Mul2Bf16(vpairs[t], v_power);
         __half2 s2[VT / 2], lo2[VT / 2];
 #pragma unroll
         for (int t = 0; t < VT / 2; ++t) {
@@ -478,6 +568,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
     };
 
     load_k(0);
+    load_sample();
     if constexpr (KV4) join();
     if constexpr (!KV4) {
       const float scale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f * a.k_descale[hkv];
@@ -505,6 +596,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
     // K runs two tiles ahead of V: K's buffer is free when the scores are done, one product earlier than V's
     store_k(0);
     load_k(1);
+    if constexpr (KV4) choose_power();
     load_v(0);
     if (ntiles > 1) {
       store_k(1);
@@ -806,6 +898,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
         const unsigned char *lo_at = from + place(row0, 2 * col), *hi_at = from + place(row0, 2 * col + 1);
         const size_t first = static_cast<size_t>(q0 + row0) * a.Hq + hq, row_step = static_cast<size_t>(kStep) * a.Hq * D;
         __nv_bfloat16* out = a.out + first * D + piece * 8;
+        const float back = ctl->v_back[piece >> 3];
         float* sums = partial ? a.part_acc + (static_cast<size_t>(blockIdx.z) * a.T * a.Hq + first) * D + piece * 8 : nullptr;
 #pragma unroll
         for (int k = 0; k < kPieces; ++k) {
@@ -814,11 +907,13 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
           float4 lo = *reinterpret_cast<const float4*>(lo_at + k * kStep * 2 * D), hi = *reinterpret_cast<const float4*>(hi_at + k * kStep * 2 * D);
           if (ctl->nan_groups[row] >> (piece >> 3) & 1) lo.x = lo.y = lo.z = lo.w = hi.x = hi.y = hi.z = hi.w = __uint_as_float(0x7fc00000u);
           if (partial) {
-            *reinterpret_cast<float4*>(sums + k * row_step) = lo;
-            *reinterpret_cast<float4*>(sums + k * row_step + 4) = hi;
+            *reinterpret_cast<float4*>(sums + k * row_step) = make_float4(lo.x * back, lo.y * back, lo.z * back, lo.w * back);
+            *reinterpret_cast<float4*>(sums + k * row_step + 4) = make_float4(hi.x * back, hi.y * back, hi.z * back, hi.w * back);
           } else {
             const float inv = ctl->inv[row];
             float x[8] = {lo.x * inv, lo.y * inv, lo.z * inv, lo.w * inv, hi.x * inv, hi.y * inv, hi.z * inv, hi.w * inv};
+#pragma unroll
+            for (int c = 0; c < 8; ++c) x[c] *= back;
             if (a.gated) {
               const uint32_t g[4] = {gate[k].x, gate[k].y, gate[k].z, gate[k].w};
 #pragma unroll
@@ -886,7 +981,7 @@ int LaunchTc(const Args<KV4>& a, cudaStream_t s) {
   constexpr int NS = D / 64;
   // kClusterAlone: so much of an SM's shared memory that no other CTA shares the SM whose cluster may wait with tensor memory in its
   // hands (sm100_ptx.cuh).  More would cost L1: 8192 rows of 32 heads of 128 columns take 808 us with 131 KB, 821 with 156, 878 with 227.
-  constexpr size_t kSmem = NS * kQRows * 128 + 2 * NS * kHalfTile * 128 + 2 * D * 128 + sizeof(Control) + 1024;
+  constexpr size_t kSmem = NS * kQRows * 128 + 2 * NS * kHalfTile * 128 + 2 * D * 128 + sizeof(std::conditional_t<KV4, Kv4Control, Control>) + 1024;
   constexpr size_t smem = kSmem > ptx::kClusterAlone ? kSmem : ptx::kClusterAlone;
   auto kern = AttnPrefillTcKernel<D, KV4>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
