@@ -193,6 +193,7 @@ __device__ __noinline__ uint32_t MostOfGroup(Kv4Control* ctl, kv4::Table table, 
 //   - keys enter with the channels of every eight in the order 0 4 1 5 2 6 3 7 (that of Kv4ToHalf), and so does Q;
 //   - a value group that is NaN is stored as zeros, and noted for the rows that see it: 0 x NaN would reach the rows that do not.
 //     (NaN keys need nothing: a score that a row does not see is replaced before it is used.)
+//   - values in front of the first row's window, whose bytes may be anything, are not loaded: 0 x infinity would reach every row;
 //   - pages that the table or pool does not have are NaN keys;
 //   - the softmax warps bring Q, and all 16 warps write whole rows at the end, their gates loaded ahead: of a CTA of one tile (24 heads over 4 of
 //     256) 26000 clocks became 21500, half of which are start and end.
@@ -384,6 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
         }
       }
     };
+    const uint32_t v_whole = max(kv_limit - kv_first - VT + 1, 0);
     auto load_v = [&](int j) {
       if constexpr (KV4) {
         const int kp0 = (tile0 + j) * kKvTile + vtok, blk = vblk;
@@ -393,7 +395,8 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
         if (j < ntiles && kp0 < kv_limit) {
           if (blk >= 0) {
             const uint32_t* at = cache4 + blk * page_words;
-            if (kp0 + VT <= kv_limit) {
+            const uint32_t from = kp0 - kv_first;                              // (of the keys from kv_first on; large in front of it)
+            if (from < v_whole) {
 #pragma unroll
               for (int t = 0; t < VT; ++t) {
                 vcodes[t] = __ldg(at + kv4::Shape<D>::kPart / 4 + vwords[t]);
@@ -402,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
             } else {
 #pragma unroll
               for (int t = 0; t < VT; ++t)
-                if (kp0 + t < kv_limit) {
+                if (from + t < static_cast<uint32_t>(kv_limit - kv_first)) {
                   vcodes[t] = __ldg(at + kv4::Shape<D>::kPart / 4 + vwords[t]);
                   vpairs[t] = __ldg(at + vpair + t * NG);
                 }

@@ -155,3 +155,21 @@ LOUD = [(D, groups, at) for D, groups in ((64, 64), (128, 128), (128, 64), (256,
 def test_prefill_of_loud_tokens_without_weight(K, D, groups, at):
     hold(K, *loud(D, 40, at, groups, 2.0 ** 20), which="prefill")
     hold(K, *loud(D, 40, at, groups, 2.0 ** 20, 1e-6), which="prefill")
+
+
+# ---- bytes that no row sees -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("free", [0x7F, 0xFF, 0x80])
+def test_bytes_in_front_of_the_window(K, D, free):
+    """Nothing was ever written there: huge scales (0x7F: 3.4e38), NaN, whatever."""
+    n, T, window, Hq, Hkv = 300, 40, 30, 4, 2
+    g = torch.Generator().manual_seed(D)
+    k, v, q = rows(g, n, Hkv, D), rows(g, n, Hkv, D), torch.randn(T, Hq, D, generator=g).to(BF)
+    pos = torch.arange(n - T, n)
+    pool = Filled(k, v, free, first=n - T - window + 1)
+    want, tol = attention(q, pool.k, pool.v, pos, window, prefill=True)
+    for splits in (1, 2):
+        assert worst(prefill(K, pool, q, n - T, window, splits=splits), want, tol) <= 1
+    want, tol = attention(q, pool.k, pool.v, pos, window)
+    assert worst(decode(K, pool, q[:8], pos[:8], window), want[:8], tol[:8]) <= 1
+    assert math.isfinite(float(want.abs().max()))
