@@ -896,37 +896,36 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
           *reinterpret_cast<uint4*>((part < 2 ? Qs : Vs) + place(r, ((part & 1) * (D / 4) + c0) / 4 + v)) = make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
       }
       asm volatile("bar.sync 5, %0;" ::"n"(kWorkers) : "memory");
-      if (*abort_flag == 0) {
-        const unsigned char* from = piece < kRowPieces / 2 ? Qs : Vs;
-        const unsigned char *lo_at = from + place(row0, 2 * col), *hi_at = from + place(row0, 2 * col + 1);
-        const size_t first = static_cast<size_t>(q0 + row0) * a.Hq + hq, row_step = static_cast<size_t>(kStep) * a.Hq * D;
-        __nv_bfloat16* out = a.out + first * D + piece * 8;
-        const float back = ctl->v_back[piece >> 3];
-        float* sums = partial ? a.part_acc + (static_cast<size_t>(blockIdx.z) * a.T * a.Hq + first) * D + piece * 8 : nullptr;
+      const bool ran_out = *abort_flag != 0;          // a wait did: the rows are NaN, never what the buffers held
+      const unsigned char* from = piece < kRowPieces / 2 ? Qs : Vs;
+      const unsigned char *lo_at = from + place(row0, 2 * col), *hi_at = from + place(row0, 2 * col + 1);
+      const size_t first = static_cast<size_t>(q0 + row0) * a.Hq + hq, row_step = static_cast<size_t>(kStep) * a.Hq * D;
+      __nv_bfloat16* out = a.out + first * D + piece * 8;
+      const float back = ctl->v_back[piece >> 3];
+      float* sums = partial ? a.part_acc + (static_cast<size_t>(blockIdx.z) * a.T * a.Hq + first) * D + piece * 8 : nullptr;
 #pragma unroll
-        for (int k = 0; k < kPieces; ++k) {
-          const int row = row0 + k * kStep;
-          if (row >= rows) break;
-          float4 lo = *reinterpret_cast<const float4*>(lo_at + k * kStep * 2 * D), hi = *reinterpret_cast<const float4*>(hi_at + k * kStep * 2 * D);
-          if (ctl->nan_groups[row] >> (piece >> 3) & 1) lo.x = lo.y = lo.z = lo.w = hi.x = hi.y = hi.z = hi.w = __uint_as_float(0x7fc00000u);
-          if (partial) {
-            *reinterpret_cast<float4*>(sums + k * row_step) = make_float4(lo.x * back, lo.y * back, lo.z * back, lo.w * back);
-            *reinterpret_cast<float4*>(sums + k * row_step + 4) = make_float4(hi.x * back, hi.y * back, hi.z * back, hi.w * back);
-          } else {
-            const float inv = ctl->inv[row];
-            float x[8] = {lo.x * inv, lo.y * inv, lo.z * inv, lo.w * inv, hi.x * inv, hi.y * inv, hi.z * inv, hi.w * inv};
+      for (int k = 0; k < kPieces; ++k) {
+        const int row = row0 + k * kStep;
+        if (row >= rows) break;
+        float4 lo = *reinterpret_cast<const float4*>(lo_at + k * kStep * 2 * D), hi = *reinterpret_cast<const float4*>(hi_at + k * kStep * 2 * D);
+        if (ran_out || (ctl->nan_groups[row] >> (piece >> 3) & 1) != 0) lo.x = lo.y = lo.z = lo.w = hi.x = hi.y = hi.z = hi.w = __uint_as_float(0x7fc00000u);
+        if (partial) {
+          *reinterpret_cast<float4*>(sums + k * row_step) = make_float4(lo.x * back, lo.y * back, lo.z * back, lo.w * back);
+          *reinterpret_cast<float4*>(sums + k * row_step + 4) = make_float4(hi.x * back, hi.y * back, hi.z * back, hi.w * back);
+        } else {
+          const float inv = ctl->inv[row];
+          float x[8] = {lo.x * inv, lo.y * inv, lo.z * inv, lo.w * inv, hi.x * inv, hi.y * inv, hi.z * inv, hi.w * inv};
 #pragma unroll
-            for (int c = 0; c < 8; ++c) x[c] *= back;
-            if (a.gated) {
-              const uint32_t g[4] = {gate[k].x, gate[k].y, gate[k].z, gate[k].w};
+          for (int c = 0; c < 8; ++c) x[c] *= back;
+          if (a.gated) {
+            const uint32_t g[4] = {gate[k].x, gate[k].y, gate[k].z, gate[k].w};
 #pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                x[2 * c] *= SigmoidApprox(BfLo(g[c]));
-                x[2 * c + 1] *= SigmoidApprox(BfHi(g[c]));
-              }
+            for (int c = 0; c < 4; ++c) {
+              x[2 * c] *= SigmoidApprox(BfLo(g[c]));
+              x[2 * c + 1] *= SigmoidApprox(BfHi(g[c]));
             }
-            *reinterpret_cast<uint4*>(out + k * row_step) = make_uint4(PackBf16(x[0], x[1]), PackBf16(x[2], x[3]), PackBf16(x[4], x[5]), PackBf16(x[6], x[7]));
           }
+          *reinterpret_cast<uint4*>(out + k * row_step) = make_uint4(PackBf16(x[0], x[1]), PackBf16(x[2], x[3]), PackBf16(x[4], x[5]), PackBf16(x[6], x[7]));
         }
       }
     }
