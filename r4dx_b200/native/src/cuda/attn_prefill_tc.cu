@@ -88,6 +88,7 @@ struct Control {
 };
 struct Kv4Control : Control {
   float inv[kQRows];                                     // 1 / l of the rows
+  float q_scale[kQRows];                                 // what takes a row's scores to the log2 domain
   int nan_groups[kQRows];                                // groups of 64 columns in which the row sees a NaN among the values
   uint32_t v_top[kConvWarps][4];                         // largest scales and low ends that a warp has met
   float v_back[4];                                       // 1 / the power of two that the group's values are taken by
@@ -189,6 +190,45 @@ __device__ __noinline__ uint32_t MostOfGroup(Kv4Control* ctl, kv4::Table table, 
   return most;
 }
 
+// Eight channels of a query row times a power of two, as fp16 in the order 0 4 1 5 2 6 3 7.
+__device__ __forceinline__ void StoreQuery(unsigned char* at, const uint4& v, float power) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t h[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) h[j] = Bits(__floats2half2_rn(BfLo(w[j]) * power, BfHi(w[j]) * power));
+  *reinterpret_cast<uint4*>(at) =
+      make_uint4(__byte_perm(h[0], h[2], 0x5410), __byte_perm(h[0], h[2], 0x7632), __byte_perm(h[1], h[3], 0x5410), __byte_perm(h[1], h[3], 0x7632));
+}
+// larger and smaller magnitudes of two pairs of bf16 (their signs mean nothing; a NaN counts for nothing)
+__device__ __forceinline__ uint32_t MaxAbs2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t MinAbs2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// A softmax warp's rows (those of its part of the loop in the kernel) once more where some value is small or very large: each row times the power
+// of two that brings its largest value to 2^14 .. 2^15, in which fp16 holds bf16 as it is, and what takes its scores back.  (Out of line: the
+// rows' maxima for every call took 1 us of the 15 of 333 rows.)
+template <int D>
+__device__ __noinline__ void ScaleQueries(unsigned char* Qs, float* q_scale, const __nv_bfloat16* q, size_t stride, int rows, float score_scale) {
+  constexpr int kLanes = D / 8;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < kQRows * kLanes; i += kSoftmaxWarps * 32) {
+    const int row = i / kLanes, c = i % kLanes;
+    const uint4 v = row < rows ? __ldg(reinterpret_cast<const uint4*>(q + row * stride + c * 8)) : make_uint4(0u, 0u, 0u, 0u);
+    uint32_t top = MaxAbs2(MaxAbs2(v.x, v.y), MaxAbs2(v.z, v.w)) & 0x7fff7fffu;
+    top = max(top >> 16, top & 0xffffu);
+#pragma unroll
+    for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const uint32_t exponent = top >> 7, p = exponent == 255u ? 127u : min(268u - exponent, 253u);
+    StoreQuery(Qs + (c >> 3) * (kQRows * 128) + Sw128(row, c & 7), v, __uint_as_float(p << 23));
+    if (c == 0) q_scale[row] = score_scale * __uint_as_float((254u - p) << 23);
+  }
+}
 // KV4: the 4-bit cache (kv4.cuh) in place of the fp8 one; only what the conversion warps load and store differs, and
 //   - keys enter with the channels of every eight in the order 0 4 1 5 2 6 3 7 (that of Kv4ToHalf), and so does Q;
 //   - a value group that is NaN is stored as zeros, and noted for the rows that see it: 0 x NaN would reach the rows that do not.
@@ -203,6 +243,7 @@ __device__ __noinline__ uint32_t MostOfGroup(Kv4Control* ctl, kv4::Table table, 
 template <int D, bool KV4>
 __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) {
   constexpr int NS = D / 64;                          // 64-dimension slabs (one 128-byte swizzle row of fp16 each)
+  [[maybe_unused]] const float score_scale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;       // of the scores of the 4-bit cache, to the log2 domain
   constexpr int kQBytes = NS * kQRows * 128;
   constexpr int kKBytes = NS * kHalfTile * 128;       // [slab][64 keys][128 B]
   constexpr int kVSlab = D / 2 * 128;                 // V^T: [64-key slab][half of the dimensions][128 B]
@@ -265,6 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
   if constexpr (KV4) {
     if (threadIdx.x < kQRows) ctl->nan_groups[threadIdx.x] = 0;
     if (threadIdx.x < 4) ctl->v_back[threadIdx.x] = 1.f;
+    if (threadIdx.x < kQRows) ctl->q_scale[threadIdx.x] = score_scale;
   }
   if (warp == kMmaWarp) {
     ptx::TmemAllocPair(&ctl->tmem_base, kTmemCols);
@@ -690,35 +732,41 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
     // ---------------- softmax warps: thread = query row = TMEM lane, two warps share a row ----------------
     const int half = warp >> 2, r = (warp & 3) * 32 + lane;
     const int qp = a.pos0 + q0 + r;                               // position of this row's query
+    [[maybe_unused]] float q_scale = 1.f;
     const int last_key = limits && r < rows ? max(qp, min(key_limit[q0 + r], kv_limit - 1)) : qp;
     if constexpr (KV4) {
       // Q, which these warps have the time to bring.  (Eight loads of a thread at a time: all 16 at D = 256 took 7300 clocks, these
-      // 3900.)
-      const float scale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f;
-      constexpr int kThreadsQ = kSoftmaxWarps * 32, kAhead = D / 8 * kQRows / kThreadsQ < 8 ? D / 8 * kQRows / kThreadsQ : 8;
+      // 3900.)  Queries of ordinary size enter as they are: fp16 holds bf16 from 6e-5 on, and is off by 2^-25 below.
+      constexpr int kThreadsQ = kSoftmaxWarps * 32, kLanes = D / 8, kAhead = kLanes * kQRows / kThreadsQ < 8 ? kLanes * kQRows / kThreadsQ : 8;
+      uint32_t least = 0x3f803f80u, most = 0u;   // of the largest of every four values that a thread has in hand; of all
 #pragma unroll 1
-      for (int i0 = threadIdx.x; i0 < kQRows * (D / 8); i0 += kAhead * kThreadsQ) {
+      for (int i0 = threadIdx.x; i0 < kQRows * kLanes; i0 += kAhead * kThreadsQ) {
         uint4 v[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
-          const int i = i0 + k * kThreadsQ, row = i / (D / 8), c = i % (D / 8);
-          v[k] = row < rows ? __ldg(reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(q0 + row) * a.Hq + hq) * D + c * 8)) : make_uint4(0u, 0u, 0u, 0u);
+          const int i = i0 + k * kThreadsQ, row = i / kLanes, c = i % kLanes;       // (rows behind the last one are ones)
+          v[k] = row < rows ? __ldg(reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(q0 + row) * a.Hq + hq) * D + c * 8)) : make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
         }
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
-          const int i = i0 + k * kThreadsQ, row = i / (D / 8), c = i % (D / 8);
-          const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-          uint32_t h[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) h[j] = Bits(__floats2half2_rn(BfLo(w[j]) * scale, BfHi(w[j]) * scale));
-          *reinterpret_cast<uint4*>(Qs + (c >> 3) * (kQRows * 128) + Sw128(row, c & 7)) =      // channels 0 4 1 5 2 6 3 7
-              make_uint4(__byte_perm(h[0], h[2], 0x5410), __byte_perm(h[0], h[2], 0x7632), __byte_perm(h[1], h[3], 0x5410), __byte_perm(h[1], h[3], 0x7632));
+          const int i = i0 + k * kThreadsQ, row = i / kLanes, c = i % kLanes;
+          StoreQuery(Qs + (c >> 3) * (kQRows * 128) + Sw128(row, c & 7), v[k], 1.f);
+          const uint32_t top = MaxAbs2(MaxAbs2(v[k].x, v[k].y), MaxAbs2(v[k].z, v[k].w));
+          least = MinAbs2(least, top);
+          most = MaxAbs2(most, top);
         }
       }
+      least &= 0x7fff7fffu;
+      most &= 0x7fff7fffu;
+      // (2^-12 at least among every four, 2^15 at most)
+      if (!__all_sync(0xffffffffu, min(least >> 16, least & 0xffffu) >= 0x3980u && max(most >> 16, most & 0xffffu) <= 0x4700u))
+        ScaleQueries<D>(Qs, ctl->q_scale, a.q + (static_cast<size_t>(q0) * a.Hq + hq) * D, static_cast<size_t>(a.Hq) * D, rows, score_scale);
       ptx::FenceProxyAsyncShared();
       join();
       __syncwarp();                              // (the others' arrivals came before the stores: they say nothing of this warp's lanes)
       if (lane == 0) ptx::MbarArriveRemote(ptx::MapToRank(ptx::SmemAddr(&ctl->q_full), 0));
+      asm volatile("bar.sync 7, %0;" ::"n"(kThreadsQ) : "memory");
+      q_scale = ctl->q_scale[r];
     }
     const uint32_t t_lane = tbase + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t p_full = ptx::MapToRank(ptx::SmemAddr(&ctl->p_full[0]), 0);
@@ -760,6 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
           mx2 = fmaxf(mx2, fmaxf(__uint_as_float(s0[c + 1]), __uint_as_float(s1[c + 1])));
         }
         mx = fmaxf(mx, mx2);
+        if constexpr (KV4) mx *= q_scale;
       }
       mx = fmaxf(mx, exchange(b, mx));
       if (!ok) continue;
@@ -793,7 +842,8 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
         uint32_t p[16];
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
-          const float e0 = Exp2Approx(__uint_as_float(sv[2 * c]) - mref), e1 = Exp2Approx(__uint_as_float(sv[2 * c + 1]) - mref);
+          const float x0 = __uint_as_float(sv[2 * c]), x1 = __uint_as_float(sv[2 * c + 1]);
+          const float e0 = Exp2Approx(KV4 ? fmaf(x0, q_scale, -mref) : x0 - mref), e1 = Exp2Approx(KV4 ? fmaf(x1, q_scale, -mref) : x1 - mref);
           sum += e0;
           sum2 += e1;
           const __half2 h = __floats2half2_rn(e0, e1);

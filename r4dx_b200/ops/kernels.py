@@ -1394,7 +1394,8 @@ def attn_prefill_kv4(q, qg, cache, block_table, out, T: int, Hq: int, Hkv: int, 
                      key_limit: Optional[torch.Tensor] = None, splits: Optional[int] = None):
     """Causal attention of T rows at positions pos0 .. over a 4-bit cache that already holds them (``attn_prefill`` for that cache, on
     tcgen05 for every head dimension, key limits included).  Keys are widened to fp16, in which magnitudes below 6e-5 lose bits; values too, whose
-    groups of 64 channels are taken times a power of two where most of the first 32 keys' are below 2^-6 (else: off by 2^-25 at most).  Rows that see a block which the table or pool does not have are NaN; pos0 may not lie behind the table.
+    groups of 64 channels are taken times a power of two where most of the first 32 keys' are below 2^-6 (else: off by 2^-25 at most), and
+    queries, rows of which are where some have values below 2^-12 or above 2^15.  Rows that see a block which the table or pool does not have are NaN; pos0 may not lie behind the table.
     ``splits``: CTA pairs that share the keys of a row tile (by ``kv4_prefill_splits`` unless given)."""
     dev, slots, length, pool, heads, dim = _kv4_pool(cache, block_table, None, T)
     if T < 1 or Hkv != heads or D != dim or Hq < 1 or Hq % Hkv or window < 0 or pos0 < 0 or pos0 > 16 * length or pos0 + T > 1 << 30:

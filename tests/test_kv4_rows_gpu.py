@@ -157,6 +157,29 @@ def test_prefill_of_loud_tokens_without_weight(K, D, groups, at):
     hold(K, *loud(D, 40, at, groups, 2.0 ** 20, 1e-6), which="prefill")
 
 
+# ---- queries and keys of any size ---------------------------------------------------------------------------------------------------
+LARGE = [(64, 1e7, 1e-4), (128, 1e5, 0.01), (256, 1e6, 1e-3), (64, 1e7, 1.0), (128, 1e-20, 1e4)]
+
+
+@pytest.mark.parametrize("D,q_size,k_size", LARGE)
+def test_prefill_of_queries_of_any_size(K, D, q_size, k_size):
+    k, v, q, pos = inputs(D, 300, 40, 4, 2, D)
+    hold(K, (k.float().clamp(-2, 2) * k_size).to(BF), v, (q.float() * q_size).to(BF), pos, which="prefill")
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("which", ["prefill"])
+def test_rows_of_queries_of_different_sizes(K, D, which):
+    """Each row has a size of its own, an outlying channel a hundred times the others'; one row is zero."""
+    k, v, q, pos = inputs(D, 300, 8, 4, 2, D)
+    q = q.float()
+    q[..., 5] *= 100
+    k = k.float()
+    k[..., 5] /= 100
+    q = q * torch.tensor([1e-12, 1e-3, 1.0, 30.0, 1e-6, 1e-4, 0.0, 1e-30])[:, None, None]
+    hold(K, k.to(BF), v, q.to(BF), pos, which=which)
+
+
 # ---- bytes that no row sees -------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("free", [0x7F, 0xFF, 0x80])
