@@ -90,7 +90,8 @@ struct Kv4Control : Control {
   float inv[kQRows];                                     // 1 / l of the rows
   float q_scale[kQRows];                                 // what takes a row's scores to the log2 domain
   int nan_groups[kQRows];                                // groups of 64 columns in which the row sees a NaN among the values
-  uint32_t v_top[kConvWarps][4];                         // largest scales and low ends that a warp has met
+  uint32_t tops[kConvWarps][4];                          // largest scales and low ends that a warp has met
+  float k_back;                                          // 1 / the power of two that the keys are taken by
   float v_back[4];                                       // 1 / the power of two that the group's values are taken by
 };
 
@@ -159,18 +160,19 @@ __device__ __forceinline__ void Kv4ToHalf(uint32_t w, __half2 s, __half2 lo, uin
   }
 }
 
-// The largest scale and low end of a group among the values of keys `begin` .. `end` - 1 (all conversion warps; a head's block b lies at
-// cache + b page_words).  Called where values are tiny, and kept out of line: its registers are not the kernel's.
+// The largest of what scales and low ends may stand for among the keys (or values) of positions `begin` .. `end` - 1, in one group of channels (or all:
+// -1), as the exponent of a float, 15 .. 254; by all conversion warps.  The pairs of a head's block b lie at pairs + b page_words.  Called where
+// keys or values are tiny, and kept out of line: its registers are not the kernel's.
+__device__ __forceinline__ float Bound(uint32_t pair) { return fmaf(15.f, BfLo(pair), BfHi(pair)); }       // of a pair without signs
 template <int D>
-__device__ __noinline__ uint32_t MostOfGroup(Kv4Control* ctl, kv4::Table table, const uint32_t* cache, size_t page_words, int begin, int end, int tid, int group) {
+__device__ __noinline__ int TopExponent(Kv4Control* ctl, kv4::Table table, const uint32_t* pairs, size_t page_words, int begin, int end, int tid, int group) {
   constexpr int NG = kv4::Shape<D>::kGroups, kPieces = 4 * NG;        // pieces: 16 bytes of a block's pairs
-  const uint32_t* at = cache + kv4::Shape<D>::kPart / 4 + 2 * D + tid % kPieces * 4;
   uint32_t top[NG] = {};
 #pragma unroll 1
   for (int b = begin / kv4::kBlock + tid / kPieces; b * kv4::kBlock < end; b += kConvThreads / kPieces) {
     const int blk = table.BlockAt(b);
     if (blk < 0) continue;
-    const uint4 x = __ldg(reinterpret_cast<const uint4*>(at + blk * page_words));
+    const uint4 x = __ldg(reinterpret_cast<const uint4*>(pairs + blk * page_words) + tid % kPieces);
     const uint32_t w[4] = {x.x & 0x7fff7fffu, x.y & 0x7fff7fffu, x.z & 0x7fff7fffu, x.w & 0x7fff7fffu};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -178,16 +180,20 @@ __device__ __noinline__ uint32_t MostOfGroup(Kv4Control* ctl, kv4::Table table, 
       if (!NoNumber(w[i]) && kp >= begin && kp < end) top[i % NG] = __vmaxu2(top[i % NG], w[i]);
     }
   }
+  asm volatile("bar.sync 6, %0;" ::"n"(kConvThreads) : "memory");      // (the last call's are read)
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     const uint32_t t = __reduce_max_sync(0xffffffffu, top[g] & 0xffffu) | __reduce_max_sync(0xffffffffu, top[g] >> 16) << 16;
-    if (tid % 32 == 0) ctl->v_top[tid / 32][g] = t;
+    if (tid % 32 == 0) ctl->tops[tid / 32][g] = t;
   }
   asm volatile("bar.sync 6, %0;" ::"n"(kConvThreads) : "memory");
   uint32_t most = 0u;
 #pragma unroll
-  for (int w = 0; w < kConvWarps; ++w) most = __vmaxu2(most, ctl->v_top[w][group]);
-  return most;
+  for (int w = 0; w < kConvWarps; ++w)
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+      if (group < 0 || group == g) most = __vmaxu2(most, ctl->tops[w][g]);
+  return min(max(static_cast<int>(__float_as_uint(Bound(most)) >> 23), 15), 254);
 }
 
 // Eight channels of a query row times a power of two, as fp16 in the order 0 4 1 5 2 6 3 7.
@@ -306,6 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
   if constexpr (KV4) {
     if (threadIdx.x < kQRows) ctl->nan_groups[threadIdx.x] = 0;
     if (threadIdx.x < 4) ctl->v_back[threadIdx.x] = 1.f;
+    if (threadIdx.x == 0) ctl->k_back = 1.f;
     if (threadIdx.x < kQRows) ctl->q_scale[threadIdx.x] = score_scale;
   }
   if (warp == kMmaWarp) {
@@ -476,10 +483,62 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
           }
       }
     };
+    // 4-bit cache: keys and values of ordinary size are widened as they are, none being above 2^15: fp16 keeps those above 6e-5 with all their bits and is
+    // off by 2^-25 at most below.  Where most of the first 32 keys are below 2^-12 throughout, or their values below 2^-6 throughout a group of 64
+    // columns, that is no small part of them: the pair then looks through the scales and low ends of all of them and takes the keys, or the
+    // group's values, times the power of two that brings the largest to 2^14 .. 2^15, and the scores, or the sums, back in the end.  (Such a look
+    // ahead of every call took 10 us of a CTA of 8192 keys at D = 256: 885 us instead of 803 for 8192 rows of 24 heads over 4; a look at every tile's
+    // keys, with a power each, 3 to 10 %.  Each warp looks at the 32 keys for itself: the eight run apart, and a barrier of theirs once in the
+    // beginning, which brings them in step, took 3 %.)
+    const int v_begin = max(kv_first, tile0 * kKvTile), v_end = min((tile0 + ntiles) * kKvTile, kv_limit);      // of the keys whose values are loaded
+    constexpr int kOwnGroups = NG > 1 ? NG / 2 : 1;      // of this CTA's columns of the values
+    uint32_t k_power = 0x3f803f80u, v_power = 0x3f803f80u;                 // as two bf16; of this thread's group
+    uint32_t k_sample[NG] = {}, v_sample[kOwnGroups] = {};                 // the pairs of one of the 32 keys
+    auto load_sample = [&]() {
+      if constexpr (KV4) {
+        const int kp = v_begin + lane, blk = block_index(kp < v_end ? kp >> 4 : -1);
+        if (blk >= 0) {
+          const uint32_t* at = cache4 + blk * page_words + 2 * D + (kp & 15) * NG;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) k_sample[g] = __ldg(at + g);
+#pragma unroll
+          for (int g = 0; g < kOwnGroups; ++g) v_sample[g] = __ldg(at + kv4::Shape<D>::kPart / 4 + rank * NG / 2 + g);
+        }
+      }
+    };
+    auto choose_powers = [&]() {
+      if constexpr (KV4) {
+        auto most_of = [&](bool some) { return 2 * __popc(__ballot_sync(0xffffffffu, some && v_begin + lane < v_end)) > min(32, v_end - v_begin); };
+        uint32_t top = 0u;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) top = __vmaxu2(top, k_sample[g] & 0x7fff7fffu);
+        bool tiny = false;                       // (the same for all warps, and the first the same for both CTAs)
+#pragma unroll
+        for (int g = 0; g < kOwnGroups; ++g) tiny |= most_of(Bound(v_sample[g] & 0x7fff7fffu) < 0.015625f);
+        if (most_of(Bound(top) < 0.000244140625f)) {
+          const int exponent = TopExponent<D>(ctl, a.table, cache4 + 2 * D, page_words, v_begin, v_end, tid, -1);
+          k_power = static_cast<uint32_t>((268 - exponent) << 7) * 0x10001u;
+          if (tid == 0) ctl->k_back = __uint_as_float(static_cast<uint32_t>(exponent - 14) << 23);
+        }
+        asm volatile("bar.arrive 7, %0;" ::"n"((kSoftmaxWarps + kConvWarps) * 32) : "memory");
+        if (tiny) {
+          const int exponent = TopExponent<D>(ctl, a.table, cache4 + kv4::Shape<D>::kPart / 4 + 2 * D, page_words, v_begin, v_end, tid, vgroup);
+          v_power = static_cast<uint32_t>((268 - exponent) << 7) * 0x10001u;
+          if (lane % VUnits == 0 && cw < 4 && (vword & 7) == 0) {
+            // each CTA's rows have all the columns
+            for (int peer = 0; peer < 2; ++peer)
+              StoreRemote(ptx::MapToRank(ptx::SmemAddr(&ctl->v_back[vgroup]), peer), __uint_as_float(static_cast<uint32_t>(exponent - 14) << 23));
+            asm volatile("fence.acq_rel.cluster;" ::: "memory");
+          }
+        }
+      }
+    };
     unsigned char* k_dst = Ks + (ch >> 2) * (kHalfTile * 128);
     auto store_k = [&](int j) {
       if constexpr (KV4) {
         unsigned char* at = Ks + (j & 1) * kKBytes;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) kpairs[i] = Mul2Bf16(kpairs[i], k_power);
 #pragma unroll
         for (int i = 0; i < NJ; ++i) {
           const uint32_t pair = kpairs[i >> 1];
@@ -507,44 +566,6 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
       ptx::FenceProxyAsyncShared();
       __syncwarp();
       if (lane == 0) ptx::MbarArriveRemote(k_full + (j & 1) * 8);
-    };
-    // 4-bit cache: values of ordinary size are widened as they are, none being above 2^15: fp16 keeps those above 6e-5 with all their bits and is off
-    // by 2^-25 at most below.  Where most of the first 32 keys have values below 2^-6 throughout a group of 64 columns, that is no small part of them:
-    // the pair then looks through the scales and low ends of all its keys and takes the group's values times the power of two that brings the
-    // largest to 2^14 .. 2^15, and the sums back in the end.  (Such a look ahead of every call took 10 us of a CTA of 8192 keys at D = 256: 885 us
-    // instead of 803 for 8192 rows of 24 heads over 4.  Each warp looks at the 32 keys for itself: the eight run apart, and a barrier of theirs
-    // once in the beginning, which brings them in step, took 3 %.)
-    uint32_t v_power = 0x3f803f80u;              // of this thread's group, as two bf16
-    constexpr int kOwnGroups = NG > 1 ? NG / 2 : 1;      // of this CTA's columns
-    uint32_t sample[kOwnGroups] = {};            // the pairs of one of the 32 keys
-    const int v_begin = max(kv_first, tile0 * kKvTile), v_end = min((tile0 + ntiles) * kKvTile, kv_limit);      // of the values that are loaded
-    auto load_sample = [&]() {
-      if constexpr (KV4) {
-        const int kp = v_begin + lane, blk = block_index(kp < v_end ? kp >> 4 : -1);
-#pragma unroll
-        for (int g = 0; g < kOwnGroups; ++g)
-          if (blk >= 0) sample[g] = __ldg(cache4 + blk * page_words + kv4::Shape<D>::kPart / 4 + 2 * D + (kp & 15) * NG + rank * NG / 2 + g);
-      }
-    };
-    auto bound = [](uint32_t pair) { return fmaf(15.f, BfLo(pair), BfHi(pair)); };      // of the values that a pair without signs stands for
-    auto choose_power = [&]() {
-      if constexpr (KV4) {
-        bool tiny = false;                       // (the same for all warps)
-#pragma unroll
-        for (int g = 0; g < kOwnGroups; ++g)
-          tiny |= 2 * __popc(__ballot_sync(0xffffffffu, v_begin + lane < v_end && bound(sample[g] & 0x7fff7fffu) < 0.015625f)) > min(32, v_end - v_begin);
-        if (tiny) {
-          const uint32_t most = MostOfGroup<D>(ctl, a.table, cache4, page_words, v_begin, v_end, tid, vgroup);
-          const int exponent = min(max(static_cast<int>(__float_as_uint(bound(most)) >> 23), 15), 254);
-          v_power = static_cast<uint32_t>((268 - exponent) << 7) * 0x10001u;
-          if (lane % VUnits == 0 && cw < 4 && (vword & 7) == 0) {
-            // each CTA's rows have all the columns
-            for (int peer = 0; peer < 2; ++peer)
-              StoreRemote(ptx::MapToRank(ptx::SmemAddr(&ctl->v_back[vgroup]), peer), __uint_as_float(static_cast<uint32_t>(exponent - 14) << 23));
-            asm volatile("fence.acq_rel.cluster;" ::: "memory");
-          }
-        }
-      }
     };
     unsigned char* v_dst = Vs + (tg >> 3) * kVSlab;
     auto store_v = [&](int j) {
@@ -639,9 +660,9 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
       if (lane == 0) ptx::MbarArriveRemote(q_full);
     }
     // K runs two tiles ahead of V: K's buffer is free when the scores are done, one product earlier than V's
+    if constexpr (KV4) choose_powers();
     store_k(0);
     load_k(1);
-    if constexpr (KV4) choose_power();
     load_v(0);
     if (ntiles > 1) {
       store_k(1);
@@ -765,8 +786,8 @@ __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) 
       join();
       __syncwarp();                              // (the others' arrivals came before the stores: they say nothing of this warp's lanes)
       if (lane == 0) ptx::MbarArriveRemote(ptx::MapToRank(ptx::SmemAddr(&ctl->q_full), 0));
-      asm volatile("bar.sync 7, %0;" ::"n"(kThreadsQ) : "memory");
-      q_scale = ctl->q_scale[r];
+      asm volatile("bar.sync 7, %0;" ::"n"((kSoftmaxWarps + kConvWarps) * 32) : "memory");      // the rows' factors are there, and that of the keys
+      q_scale = ctl->q_scale[r] * ctl->k_back;
     }
     const uint32_t t_lane = tbase + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t p_full = ptx::MapToRank(ptx::SmemAddr(&ctl->p_full[0]), 0);

@@ -1393,9 +1393,10 @@ def kv4_prefill_splits(T: int, Hq: int, Hkv: int, D: int, pos0: int, window: int
 def attn_prefill_kv4(q, qg, cache, block_table, out, T: int, Hq: int, Hkv: int, D: int, pos0: int, gated: bool = True, window: int = 0,
                      key_limit: Optional[torch.Tensor] = None, splits: Optional[int] = None):
     """Causal attention of T rows at positions pos0 .. over a 4-bit cache that already holds them (``attn_prefill`` for that cache, on
-    tcgen05 for every head dimension, key limits included).  Keys are widened to fp16, in which magnitudes below 6e-5 lose bits; values too, whose
-    groups of 64 channels are taken times a power of two where most of the first 32 keys' are below 2^-6 (else: off by 2^-25 at most), and
-    queries, rows of which are where some have values below 2^-12 or above 2^15.  Rows that see a block which the table or pool does not have are NaN; pos0 may not lie behind the table.
+    tcgen05 for every head dimension, key limits included).  Keys, values and queries enter the products as fp16, off by 2^-25 at most below 6e-5.
+    Where that is no small part of them - most of the first 32 keys below 2^-12, or their values below 2^-6 in a group of 64 channels; four
+    neighbours of a query below 2^-12 - they are taken times powers of two, and so are queries with values above 2^15.
+    Rows that see a block which the table or pool does not have are NaN; pos0 may not lie behind the table.
     ``splits``: CTA pairs that share the keys of a row tile (by ``kv4_prefill_splits`` unless given)."""
     dev, slots, length, pool, heads, dim = _kv4_pool(cache, block_table, None, T)
     if T < 1 or Hkv != heads or D != dim or Hq < 1 or Hq % Hkv or window < 0 or pos0 < 0 or pos0 > 16 * length or pos0 + T > 1 << 30:

@@ -158,11 +158,18 @@ def test_prefill_of_loud_tokens_without_weight(K, D, groups, at):
 
 
 # ---- queries and keys of any size ---------------------------------------------------------------------------------------------------
+SIZES = [(64, 1e-5, 1e4), (128, 1e-7, 2e4), (256, 2e-6, 1.6e4), (128, 3e6, 1e-6), (256, 1e20, 1e-20), (64, 1e30, 3e-31)]
 LARGE = [(64, 1e7, 1e-4), (128, 1e5, 0.01), (256, 1e6, 1e-3), (64, 1e7, 1.0), (128, 1e-20, 1e4)]
 
 
 @pytest.mark.parametrize("D,q_size,k_size", LARGE)
 def test_prefill_of_queries_of_any_size(K, D, q_size, k_size):
+    k, v, q, pos = inputs(D, 300, 40, 4, 2, D)
+    hold(K, (k.float().clamp(-2, 2) * k_size).to(BF), v, (q.float() * q_size).to(BF), pos, which="prefill")
+
+
+@pytest.mark.parametrize("D,q_size,k_size", SIZES)
+def test_prefill_of_queries_and_keys_of_any_size(K, D, q_size, k_size):
     k, v, q, pos = inputs(D, 300, 40, 4, 2, D)
     hold(K, (k.float().clamp(-2, 2) * k_size).to(BF), v, (q.float() * q_size).to(BF), pos, which="prefill")
 
