@@ -8,9 +8,10 @@
 //            sum_g lo sum(q): one product of the pairs as they lie (bf16) with the sums' upper and lower parts.
 //   softmax  running maximum per row in the log2 domain, moved only when a score is more than 8 above it (p <= 2^8), so that most blocks
 //            need no exchange between lanes; sums in fp32 per lane.
-//   values   O^T[D x 8 rows] += n (p s):  A = codes of token pairs, again as subnormals; B = p s times a power of two that brings the largest
-//            scale met so far to 1 .. 2, rounded to fp16 (2^-11 of 15 steps at most), turned from scores' to operand order with movmatrix.
-//            sum p lo per group in fp32.
+//   values   O^T[D x 8 rows] += n (p s):  A = codes of token pairs, again as subnormals; B = p s times a power of two of the warp and the group of
+//            channels, rounded to fp16, turned from scores' to operand order with movmatrix.  The power is made smaller where a product reaches
+//            2^7 (to 1), larger again where all rows' maxima rise, so it follows products, not scales: loud tokens without weight
+//            leave it alone.  Off by 2^-12 of a product, or by 2^-25 of the largest of the group among the rows of the tile.  sum p lo in fp32.
 // The warps' results meet in shared memory; the splits' in the shared memory of a cluster of up to 16 CTAs, or, for long tables, in a second
 // kernel.  A sequence short enough for one CTA is finished by it.
 // A row with no visible token (position -1) gives zeros; a block that the table or pool does not have gives NaN to the rows that see it.
@@ -31,6 +32,7 @@ namespace {
 
 constexpr int kMaxCluster = 16;
 constexpr float kRescaleStep = 8.f;
+constexpr int kMostPower = 253;            // exponent of the largest power of two that p s is taken by: 2^126
 constexpr float kUnit = 1.f / (1 << 28);       // of the scores before the softmax: 2^-4 from q, 2^-24 from the codes
 
 struct DecodeArgs {
@@ -304,8 +306,9 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
       for (int e = 0; e < 4; ++e) acc[nt][j][e] = {{0.f, 0.f, 0.f, 0.f}};
     }
   }
-  float limit = __uint_as_float(39u << 23);      // scales from which the sums need a smaller power of two ..
-  float power = __uint_as_float((254u - 32u) << 23);      // .. than this: 2^-(exponent of the largest scale), at first 2^95
+  float power[NG];                               // what the groups' weights times scales are taken by
+#pragma unroll
+  for (int j = 0; j < NG; ++j) power[j] = __uint_as_float(static_cast<uint32_t>(kMostPower) << 23);
 
   // N consecutive blocks from token kp0 on, as they lie in the ring
   auto blocks = [&](auto count, uint32_t* const run, const int kp0) {
@@ -393,17 +396,22 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
             if (!sees(pos[nt][e & 1], kp0 + n * kv4::kBlock + g + (e >> 1) * 8)) sc[n][nt].x[e] = -INFINITY;
     }
 
-    // ---- running maximum, power of two of the scales, probabilities ----
+    // ---- running maximum, powers of two of the groups, probabilities ----
     uint32_t pa[N][NG], pb[N][NG];
-    float largest = 0.f, top[NT][2];
+    bool move = false;
+    float top[NT][2];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       LoadWords<NG>(run + n * kWords + kValues + 2 * D + g * NG, pa[n]);
       LoadWords<NG>(run + n * kWords + kValues + 2 * D + (g + 8) * NG, pb[n]);
-#pragma unroll
-      for (int j = 0; j < NG; ++j) largest = fmaxf(largest, fmaxf(BfLo(pa[n][j]), BfLo(pb[n][j])));
     }
-    bool move = largest >= limit;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      float largest = 0.f;
+#pragma unroll
+      for (int n = 0; n < N; ++n) largest = fmaxf(largest, fmaxf(BfLo(pa[n][j]), BfLo(pb[n][j])));
+      move = move || largest * power[j] >= 128.f;                 // (a probability is 2^8 at most)
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -414,36 +422,52 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
         move = move || top[nt][r] > m[nt][r] + rise;
       }
     if (__any_sync(0xffffffffu, move)) {
-      const uint32_t bits = __reduce_max_sync(0xffffffffu, largest < INFINITY ? __float_as_uint(largest) : 0u);
-      float shrink = 1.f;
-      if (bits >= __float_as_uint(limit)) {
-        const uint32_t e = bits >> 23;
-        const float now = __uint_as_float((254u - e) << 23);
-        shrink = now / power;
-        power = now;
-        limit = __uint_as_float((e + 7u) << 23);
-      }
+      float f[NT][2], keep = 0.f;                // what the rows' sums are taken by; the most of it among rows that have sums
+      float pm[N][2];                            // the largest probabilities of tokens g, g + 8 among this lane's rows
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float f[2];
+      for (int n = 0; n < N; ++n) pm[n][0] = pm[n][1] = 0.f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          float n = fmaxf(m[nt][r], top[nt][r]);
+          float t = fmaxf(m[nt][r], top[nt][r]);
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, o));
-          f[r] = n == -INFINITY ? 1.f : Exp2((m[nt][r] - n) * scale);
-          m[nt][r] = n;
-          ms[nt][r] = n == -INFINITY ? 0.f : n * scale;
-          l[nt][r] *= f[r];
+          for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+          f[nt][r] = t == -INFINITY ? 1.f : Exp2((m[nt][r] - t) * scale);
+          const bool there = pos[nt][r] >= 0;    // (columns behind the last row have queries of zero and count for nothing)
+          if (there && m[nt][r] != -INFINITY) keep = fmaxf(keep, f[nt][r]);
+          m[nt][r] = t;
+          ms[nt][r] = t == -INFINITY ? 0.f : t * scale;
+          l[nt][r] *= f[nt][r];
+#pragma unroll
+          for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (there) pm[n][h] = fmaxf(pm[n][h], Exp2(fmaf(sc[n][nt].x[2 * h + r], scale, -ms[nt][r])));
         }
+      // where the sums of all rows become small, the products that are added to them need not be
+      keep = fmaxf(keep, __shfl_xor_sync(0xffffffffu, keep, 1));
+      keep = fmaxf(keep, __shfl_xor_sync(0xffffffffu, keep, 2));
+      const int grow = max(126 - static_cast<int>(__float_as_uint(keep) >> 23), 0);
 #pragma unroll
-        for (int j = 0; j < NG; ++j) {
-          base[nt][j][0] *= f[0];
-          base[nt][j][1] *= f[1];
+      for (int j = 0; j < NG; ++j) {
+        float product = 0.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+        for (int n = 0; n < N; ++n) product = fmaxf(product, fmaxf(pm[n][0] * BfLo(pa[n][j]), pm[n][1] * BfLo(pb[n][j])));
+        const int e = static_cast<int>(__reduce_max_sync(0xffffffffu, product < INFINITY ? __float_as_uint(product) : 0u) >> 23);
+        const int old = static_cast<int>(__float_as_uint(power[j]) >> 23);
+        int now = min(old + grow, kMostPower);
+        if (e + now >= 254 + 7) now = max(254 - e, 1);            // a product of 2^7 or more: to 1 .. 2
+        power[j] = __uint_as_float(static_cast<uint32_t>(now) << 23);
+        const float other = __uint_as_float(static_cast<uint32_t>(min(max(127 + now - old, 0), 254)) << 23);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) acc[nt][j][e].x[x] *= f[x & 1] * shrink;
+        for (int nt = 0; nt < NT; ++nt) {
+          base[nt][j][0] *= f[nt][0];
+          base[nt][j][1] *= f[nt][1];
+#pragma unroll
+          for (int e4 = 0; e4 < 4; ++e4)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) acc[nt][j][e4].x[x] *= f[nt][x & 1] * other;
         }
       }
     }
@@ -480,7 +504,7 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
       }
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
-        const float sa = BfLo(pa[n][j]) * power, sb = BfLo(pb[n][j]) * power, la = BfHi(pa[n][j]), lb = BfHi(pb[n][j]);
+        const float sa = BfLo(pa[n][j]) * power[j], sb = BfLo(pb[n][j]) * power[j], la = BfHi(pa[n][j]), lb = BfHi(pb[n][j]);
         uint32_t w0[NT], w1[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -566,7 +590,6 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
   // warps that had blocks (the first ones)
   const int used = max(1, min(kWarps, (b1 - b0 + take - 1) / take));
   if (warp < used) {
-    const float back = 16777216.f / power, back16 = back * 0.0625f;             // codes n 2^-24, n 2^-20
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       // sum p lo over the lanes g: each round halves the values that a lane still adds up, until lane g has the sum of its own one
@@ -591,7 +614,8 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
       float* dst = merge + (warp * kRows + 8 * nt + 2 * c) * P::kStride + 8 * g;
       const int h0 = (c & 1) * 4, h1 = 4 - h0;
 #pragma unroll
-      for (int j = 0; j < NG; ++j)
+      for (int j = 0; j < NG; ++j) {
+        const float back = 16777216.f / power[j], back16 = back * 0.0625f;      // codes n 2^-24, n 2^-20
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const Frag(&o)[4] = acc[nt][j];
@@ -599,6 +623,7 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
           *reinterpret_cast<float4*>(at + h0) = make_float4(o[0].x[r] * back, o[1].x[r] * back16, o[2].x[r] * back, o[3].x[r] * back16);
           *reinterpret_cast<float4*>(at + h1) = make_float4(o[0].x[2 + r] * back, o[1].x[2 + r] * back16, o[2].x[2 + r] * back, o[3].x[2 + r] * back16);
         }
+      }
       if (g == 0) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) ml[warp * kRows + 8 * nt + 2 * c + r] = make_float2(m[nt][r] * scale, l[nt][r]);

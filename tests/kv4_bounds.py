@@ -5,7 +5,7 @@ within six times the root of the sum, plus what is a bound on all of them.  With
 low ends of their groups:
   both      o is rounded to bf16: 2^-8 of it at most, and so is its norm.  Scores are sums in 32 bits: 2^-21 of the sum of |q k|, which moves the row by twice that of
             sum p |v - o|.  The final normalisation and an approximate exponential: 2^-19.
-  decode    p s is rounded to fp16 (2^-11), the share p n s = p (v - lo) of each value with it, and not below 2^-32 of the largest p s.  Tensor-core
+  decode    p s is rounded to fp16 (2^-11), the share p n s = p (v - lo) of each value with it, and not below 2^-25 of the largest p s.  Tensor-core
             sums round towards zero, by up to 2^-24 of sum p n s at each of the (at most 256) blocks of a warp.
   prefill   p and v are rounded to fp16, and p not below 2^-25 of the largest; keys too, which moves a score by 2^-11 of q k in each channel.
 """
@@ -45,7 +45,7 @@ def attention(q, k, v, pos, window=0, limit=None, gate=None, prefill=False, keys
                 bound = torch.zeros_like(var)
             else:
                 most = torch.stack([(p * step[:, g]).amax(-1) for g in range(D // 64)], -1)
-                var += 2.0 ** -64 / 3 * most.square() * 225 * 64 * keys.sum(-1, keepdim=True)
+                var += 2.0 ** -50 / 3 * most.square() * 225 * 64 * keys.sum(-1, keepdim=True)
                 bound = 2.0 ** -16 * norms(p @ share).sqrt()
             off = 2.0 ** -21 * ((q[:, i].abs() @ kh.abs().T) / math.sqrt(D)).masked_fill(~keys, 0.0).amax(-1, keepdim=True)
             bound += (2 * off + 2.0 ** -19) * (p @ norms(vh).sqrt() + norms(o).sqrt()) + 2.0 ** -8 * norms(o).sqrt()

@@ -122,6 +122,12 @@ def test_prefill_of_values_of_any_size(K, D, size):
     hold(K, k, (v.float() * size).to(BF), q, pos, window=50, which="prefill")
 
 
+@pytest.mark.parametrize("D,size", VALUES)
+def test_decode_of_values_of_any_size(K, D, size):
+    k, v, q, pos = inputs(D, 300, 8, 4, 2, D)
+    hold(K, k, (v.float() * size).to(BF), q, pos, which="decode")
+
+
 def uneven(D, which, ratio):
     k, v, q, pos = inputs(D, 700, 8 if which == "decode" else 40, 4, 2, D)
     v = v.float()
@@ -134,6 +140,12 @@ def uneven(D, which, ratio):
 @pytest.mark.parametrize("ratio", [2.0 ** 14, 2.0 ** 20, 2.0 ** -20])
 def test_prefill_of_value_groups_far_apart(K, D, ratio):
     hold(K, *uneven(D, "prefill", ratio / 1024), which="prefill")
+
+
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("ratio", [2.0 ** 14, 2.0 ** 20, 2.0 ** -20])
+def test_decode_of_value_groups_far_apart(K, D, ratio):
+    hold(K, *uneven(D, "decode", ratio / 1024), which="decode")
 
 
 def loud(D, T, at, groups, ratio, size=1 / 64):
@@ -155,6 +167,24 @@ LOUD = [(D, groups, at) for D, groups in ((64, 64), (128, 128), (128, 64), (256,
 def test_prefill_of_loud_tokens_without_weight(K, D, groups, at):
     hold(K, *loud(D, 40, at, groups, 2.0 ** 20), which="prefill")
     hold(K, *loud(D, 40, at, groups, 2.0 ** 20, 1e-6), which="prefill")
+
+
+@pytest.mark.parametrize("D,groups,at", LOUD)
+def test_decode_of_loud_tokens_without_weight(K, D, groups, at):
+    hold(K, *loud(D, 8, at, groups, 2.0 ** 20), which="decode")
+    hold(K, *loud(D, 8, at, groups, 2.0 ** 20, 1e-6), which="decode")
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_loud_tokens_whose_weight_fades(K, D):
+    """The first token has a row's whole weight until others, 2^20 quieter, are met whose scores lie far above it (and again)."""
+    g = torch.Generator().manual_seed(D)
+    Hq, Hkv, n = 4, 2, 3000
+    q = (1 + 0.25 * torch.randn(1, Hq, D, generator=g)).to(BF)
+    k, v = (0.1 * torch.randn(n, Hkv, D, generator=g)).to(BF), (torch.randn(n, Hkv, D, generator=g) / 64).to(BF)
+    k[:1000], k[1000:2000] = (k[:1000].float() - 10).to(BF), (k[1000:2000].float() - 5).to(BF)
+    v[:1000], v[1000:2000] = (v[:1000].float() * 2.0 ** 20).to(BF), (v[1000:2000].float() * 2.0 ** 10).to(BF)
+    hold(K, k, v, q, torch.tensor([n - 1]))
 
 
 # ---- queries and keys of any size ---------------------------------------------------------------------------------------------------
