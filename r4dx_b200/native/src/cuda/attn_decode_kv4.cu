@@ -3,8 +3,10 @@
 // Split-KV: a CTA has 8 NT query rows of a kv head (of the G = rows x query heads per kv head) and a share of the sequence's blocks; each
 // of its warps walks blocks of its own, which arrive as one bulk copy per block into the warp's ring of shared memory.  Per block
 //   scores   S^T[16 tokens x 8 rows] = K Q^T on mma.m16n8k16 (fp16): A = the codes as they lie, since four bits at the bottom of a half are
-//            the subnormal n 2^-24 and four bits above them n 2^-20: one AND for two codes, and no conversion at all.  B = the query rows
-//            times 2^-4 (2^-8 under the codes that carry a 16), exact down to 2^-6.  A group gives 2^-28 sum q n; then s (that) in fp32.
+//            the subnormal n 2^-24 and four bits above them n 2^-20: one AND for two codes, and no conversion at all.  B = the query rows times
+//            2^4 (1 under the codes that carry a 16), exact down to 2^-14 and off by 2^-25 below; where some are above 2^11, or eight neighbours
+//            below 2^-12, each row times the power of two that brings its largest value to 2^14 .. 2^15.  (That for every call: 0.2 us.)
+//            A group gives 2^-24 sum q n; then s (that) in fp32.
 //            sum_g lo sum(q): one product of the pairs as they lie (bf16) with the sums' upper and lower parts.
 //   softmax  running maximum per row in the log2 domain, moved only when a score is more than 8 above it (p <= 2^8), so that most blocks
 //            need no exchange between lanes; sums in fp32 per lane.
@@ -33,7 +35,9 @@ namespace {
 constexpr int kMaxCluster = 16;
 constexpr float kRescaleStep = 8.f;
 constexpr int kMostPower = 253;            // exponent of the largest power of two that p s is taken by: 2^126
-constexpr float kUnit = 1.f / (1 << 28);       // of the scores before the softmax: 2^-4 from q, 2^-24 from the codes
+constexpr float kUnit = 1.f / (1 << 24);       // of the scores before the softmax, from the codes
+constexpr uint32_t kOrdinary = 131u;           // exponent of the power of two that queries of ordinary size are taken by: 2^4
+constexpr float kNone = -3e38f;                // the maximum of a row that has seen nothing: finite, so that 2^(-inf - kNone) is 0
 
 struct DecodeArgs {
   const __nv_bfloat16* q;      // [T, Hq, D]
@@ -75,7 +79,7 @@ struct Plan {
   static constexpr int kBase = kWarps * kRows * (D / 64) * 4;    // sum p lo of each warp, row and group
   static constexpr int kOut = kRows * D * 4;                     // a CTA's rows, for the other CTAs of its cluster
   static constexpr int kBody = kRing > kMerge + kBase + kOut ? kRing : kMerge + kBase + kOut;
-  static constexpr int kSums = NT * (D / 32) * 8 * 4;            // of a row's query over 32 channels
+  static constexpr int kSums = 2 * NT * (D / 32) * 8 * 4;        // of a row's query over 32 channels: sums, largest magnitudes
   static constexpr size_t kSmem = kBody + kQuery + kSums + kWarps * kStages * 8 + kWarps * kRows * 8 + kRows * 20 + 16;
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
@@ -182,13 +186,15 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
     a.table.entries += static_cast<size_t>(known ? slot : 0) * a.table.length;
   }
   const int gqa = a.Hq / a.Hkv, G = gqa * a.T;
-  // A warp lays out 32 channels of a row tile's queries; the first of its tasks is on its way while positions and table are.
-  auto load_query = [&](int task) {
-    const int r = row0 + task / NJ * 8 + g, t = a.Row(r);
-    return r < G ? *reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(t) * a.Hq + hkv * gqa + r - t * gqa) * D + task % NJ * 32 + 8 * c)
-                 : make_uint4(0u, 0u, 0u, 0u);
-  };
-  uint4 query_next = warp < NT * NJ ? load_query(warp) : make_uint4(0u, 0u, 0u, 0u);
+  // A warp lays out 32 channels of a row tile's queries, one or two times; they are on their way while positions and table are.
+  constexpr int kTasks = (NT * NJ + kWarps - 1) / kWarps;
+  uint4 own_query[kTasks];
+#pragma unroll
+  for (int i = 0; i < kTasks; ++i) {
+    const int task = warp + i * kWarps, r = row0 + task / NJ * 8 + g, t = a.Row(r);
+    own_query[i] = task < NT * NJ && r < G ? *reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(t) * a.Hq + hkv * gqa + r - t * gqa) * D + task % NJ * 32 + 8 * c)
+                                           : make_uint4(0u, 0u, 0u, 0u);
+  }
   const Span span = Visible(a);
   if (split >= (CLUSTER && span.active > 1 ? a.splits : span.active)) return;       // (a cluster stays together, its CTAs without blocks merge too)
   const int per = (span.blocks + span.active - 1) / span.active;
@@ -240,25 +246,61 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
     const int p = __shfl_sync(0xffffffffu, span.position, r < G ? a.Row(r) : 0);
     return r < G ? p : -1;
   };
-  for (int task = warp; task < NT * NJ; task += kWarps) {
-    const uint4 v = query_next;
-    if (task + kWarps < NT * NJ) query_next = load_query(task + kWarps);
-    // channels i and i + 4 for i = 0 .. 3; every second pair meets codes that carry a factor 16
-    const float x[8] = {BfLo(v.x), BfHi(v.x), BfLo(v.y), BfHi(v.y), BfLo(v.z), BfHi(v.z), BfLo(v.w), BfHi(v.w)};
-    uint32_t b[4];
-    float sum = 0.f;
+  uint32_t tops[kTasks];                         // the largest magnitude of eight channels, as the bits of bf16
+  bool ordinary = true;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float f = i & 1 ? 0.00390625f : 0.0625f;
-      b[i] = PackHalf(x[i] * f, x[i + 4] * f);
-      sum += x[i] + x[i + 4];
-    }
-    query[task * 32 + lane] = make_uint4(b[0], b[1], b[2], b[3]);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    if (c == 0) sums[task * 8 + g] = sum * kUnit;
+  for (int i = 0; i < kTasks; ++i) {
+    const uint4 v = own_query[i];
+    const uint32_t top = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+    tops[i] = max(top >> 16, top & 0xffffu);
+    const int task = warp + i * kWarps;
+    if (task < NT * NJ && row0 + task / NJ * 8 + g < G) ordinary = ordinary && tops[i] - 0x3980u <= 0x4500u - 0x3980u;      // 2^-12 .. 2^11
   }
-  __syncthreads();
+  auto lay_out = [&](auto exponent) {            // of a row's power of two, as of a float
+#pragma unroll
+    for (int i = 0; i < kTasks; ++i) {
+      const int task = warp + i * kWarps;
+      if (task < NT * NJ) {
+        const uint4 v = own_query[i];
+        const float power = __uint_as_float(exponent(task / NJ * 8 + g) << 23), power16 = power * 0.0625f;
+        // channels i and i + 4 for i = 0 .. 3; every second pair meets codes that carry a factor 16
+        const float x[8] = {BfLo(v.x), BfHi(v.x), BfLo(v.y), BfHi(v.y), BfLo(v.z), BfHi(v.z), BfLo(v.w), BfHi(v.w)};
+        uint32_t b[4];
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          b[k] = PackHalf(x[k] * (k & 1 ? power16 : power), x[k + 4] * (k & 1 ? power16 : power));
+          sum += x[k] + x[k + 4];
+        }
+        query[task * 32 + lane] = make_uint4(b[0], b[1], b[2], b[3]);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (c == 0) sums[task * 8 + g] = sum * power * kUnit;
+      }
+    }
+  };
+  lay_out([](int) { return kOrdinary; });
+  const bool by_row = __syncthreads_or(!ordinary) != 0;
+  uint32_t* row_tops = reinterpret_cast<uint32_t*>(sums + NT * NJ * 8);         // [row][32 channels]
+  auto exponent_of = [&](int row) {
+    uint32_t top = 0u;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) top = max(top, row_tops[row * NJ + j]);
+    const uint32_t e = top >> 7;
+    return e == 255u ? 127u : min(max(268u - e, 24u), 253u);      // to 2^14 .. 2^15 (infinite or NaN: as it is)
+  };
+  if (by_row) {
+#pragma unroll
+    for (int i = 0; i < kTasks; ++i) {
+      const int task = warp + i * kWarps;
+      uint32_t top = max(tops[i], __shfl_xor_sync(0xffffffffu, tops[i], 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      if (c == 0 && task < NT * NJ) row_tops[(task / NJ * 8 + g) * NJ + task % NJ] = top;
+    }
+    __syncthreads();
+    lay_out(exponent_of);
+    __syncthreads();
+  }
   // operand B of sum_g lo sum(q): pairs (0, sum) in two (D = 256, 128) or four (64) parts of bf16
   uint32_t qpair[NT][2];
 #pragma unroll
@@ -277,12 +319,15 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
     qpair[nt][1] = NG == 4 ? PackBf16(0.f, next) : 0u;
   }
 
-  const float scale = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f / kUnit, rise = kRescaleStep / scale;
   int pos[NT][2], p_min = 0x7fffffff, p_max = -1;
+  float scale[NT][2];                            // of the rows' scores, to the log2 domain
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     pos[nt][0] = position(row0 + 8 * nt + 2 * c);
     pos[nt][1] = position(row0 + 8 * nt + 2 * c + 1);
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      scale[nt][r] = rsqrtf(static_cast<float>(D)) * 1.4426950408889634f / kUnit * __uint_as_float((254u - (by_row ? exponent_of(8 * nt + 2 * c + r) : kOrdinary)) << 23);
     // among the rows that there are, for blocks that all of them see whole
     const int r = row0 + 8 * nt + g, p = position(r);
     p_min = min(p_min, r < G ? p : 0x7fffffff);
@@ -292,13 +337,13 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
   p_max = __reduce_max_sync(0xffffffffu, p_max);
   auto sees = [&](int at, int kp) { return kp <= at && (a.window == 0 || kp > at - a.window); };
 
-  float m[NT][2], ms[NT][2], l[NT][2];           // rows 8 nt + 2 c, + 1: maximum, the same times the scale (0 for -inf), sum over this lane's tokens
+  float m[NT][2], l[NT][2];                      // rows 8 nt + 2 c, + 1: maximum in the log2 domain, sum over this lane's tokens
   Frag acc[NT][NG][4];
   float base[NT][NG][2];                         // sum p lo of this lane's tokens
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    m[nt][0] = m[nt][1] = -INFINITY;
-    ms[nt][0] = ms[nt][1] = l[nt][0] = l[nt][1] = 0.f;
+    m[nt][0] = m[nt][1] = kNone;
+    l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       base[nt][j][0] = base[nt][j][1] = 0.f;
@@ -419,7 +464,8 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
         top[nt][r] = fmaxf(sc[0][nt].x[r], sc[0][nt].x[2 + r]);
 #pragma unroll
         for (int n = 1; n < N; ++n) top[nt][r] = fmaxf(top[nt][r], fmaxf(sc[n][nt].x[r], sc[n][nt].x[2 + r]));
-        move = move || top[nt][r] > m[nt][r] + rise;
+        top[nt][r] *= scale[nt][r];
+        move = move || top[nt][r] > m[nt][r] + kRescaleStep;
       }
     if (__any_sync(0xffffffffu, move)) {
       float f[NT][2], keep = 0.f;                // what the rows' sums are taken by; the most of it among rows that have sums
@@ -433,17 +479,16 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
           float t = fmaxf(m[nt][r], top[nt][r]);
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
-          f[nt][r] = t == -INFINITY ? 1.f : Exp2((m[nt][r] - t) * scale);
+          f[nt][r] = Exp2(m[nt][r] - t);
           const bool there = pos[nt][r] >= 0;    // (columns behind the last row have queries of zero and count for nothing)
-          if (there && m[nt][r] != -INFINITY) keep = fmaxf(keep, f[nt][r]);
+          if (there && m[nt][r] != kNone) keep = fmaxf(keep, f[nt][r]);
           m[nt][r] = t;
-          ms[nt][r] = t == -INFINITY ? 0.f : t * scale;
           l[nt][r] *= f[nt][r];
 #pragma unroll
           for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              if (there) pm[n][h] = fmaxf(pm[n][h], Exp2(fmaf(sc[n][nt].x[2 * h + r], scale, -ms[nt][r])));
+              if (there) pm[n][h] = fmaxf(pm[n][h], Exp2(fmaf(sc[n][nt].x[2 * h + r], scale[nt][r], -m[nt][r])));
         }
       // where the sums of all rows become small, the products that are added to them need not be
       keep = fmaxf(keep, __shfl_xor_sync(0xffffffffu, keep, 1));
@@ -478,7 +523,7 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[nt][e] = Exp2(fmaf(sc[n][nt].x[e], scale, -ms[nt][e & 1]));
+        for (int e = 0; e < 4; ++e) p[nt][e] = Exp2(fmaf(sc[n][nt].x[e], scale[nt][e & 1], -m[nt][e & 1]));
         l[nt][0] += p[nt][0] + p[nt][2];
         l[nt][1] += p[nt][1] + p[nt][3];
       }
@@ -626,7 +671,7 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
       }
       if (g == 0) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) ml[warp * kRows + 8 * nt + 2 * c + r] = make_float2(m[nt][r] * scale, l[nt][r]);
+        for (int r = 0; r < 2; ++r) ml[warp * kRows + 8 * nt + 2 * c + r] = make_float2(m[nt][r] == kNone ? -INFINITY : m[nt][r], l[nt][r]);
       }
     }
   }

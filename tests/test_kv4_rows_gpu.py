@@ -192,6 +192,12 @@ SIZES = [(64, 1e-5, 1e4), (128, 1e-7, 2e4), (256, 2e-6, 1.6e4), (128, 3e6, 1e-6)
 LARGE = [(64, 1e7, 1e-4), (128, 1e5, 0.01), (256, 1e6, 1e-3), (64, 1e7, 1.0), (128, 1e-20, 1e4)]
 
 
+@pytest.mark.parametrize("D,q_size,k_size", SIZES + LARGE)
+def test_decode_of_queries_and_keys_of_any_size(K, D, q_size, k_size):
+    k, v, q, pos = inputs(D, 300, 8, 4, 2, D)
+    hold(K, (k.float().clamp(-2, 2) * k_size).to(BF), v, (q.float() * q_size).to(BF), pos, which="decode")
+
+
 @pytest.mark.parametrize("D,q_size,k_size", LARGE)
 def test_prefill_of_queries_of_any_size(K, D, q_size, k_size):
     k, v, q, pos = inputs(D, 300, 40, 4, 2, D)
@@ -205,7 +211,7 @@ def test_prefill_of_queries_and_keys_of_any_size(K, D, q_size, k_size):
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
-@pytest.mark.parametrize("which", ["prefill"])
+@pytest.mark.parametrize("which", ["prefill", "decode"])
 def test_rows_of_queries_of_different_sizes(K, D, which):
     """Each row has a size of its own, an outlying channel a hundred times the others'; one row is zero."""
     k, v, q, pos = inputs(D, 300, 8, 4, 2, D)
@@ -215,6 +221,19 @@ def test_rows_of_queries_of_different_sizes(K, D, which):
     k[..., 5] /= 100
     q = q * torch.tensor([1e-12, 1e-3, 1.0, 30.0, 1e-6, 1e-4, 0.0, 1e-30])[:, None, None]
     hold(K, k.to(BF), v, q.to(BF), pos, which=which)
+
+
+@pytest.mark.parametrize("D", [128, 256])
+def test_keys_whose_offsets_cancel(K, D):
+    """Half of the tokens have keys of 20000 in one group and -20000 in another, whose products with q cancel."""
+    g = torch.Generator().manual_seed(D)
+    Hq, Hkv, n = 4, 2, 300
+    q = torch.randn(1, Hq, D, generator=g)
+    q = (q * 64).round() / 64
+    q = torch.cat([q[..., :64], q[..., :64].flip(-1), q[..., 128:]], -1)[..., :D].to(BF)          # equal sums over the first two groups
+    k, v = torch.randn(n, Hkv, D, generator=g), rows(g, n, Hkv, D)
+    k[::2, :, :64], k[::2, :, 64:128] = 20000.0, -20000.0
+    hold(K, k.to(BF), v, q, torch.tensor([n - 1]), which="decode")
 
 
 # ---- bytes that no row sees -------------------------------------------------------------------------------------------------------
