@@ -580,7 +580,10 @@ __global__ void __launch_bounds__(Plan<D, NT>::kWarps * 32, Plan<D, NT>::kCtas) 
   uint32_t phase = 0u;
 #pragma unroll 1
   for (; i < steps; ++i) {
-    if (!__all_sync(0xffffffffu, ptx::MbarTestWaitAt(full_at + slot * 8, phase))) ok = ptx::WarpMbarWait(full + slot, phase, abort_flag, 1);
+    if (!__all_sync(0xffffffffu, ptx::MbarTestWaitAt(full_at + slot * 8, phase))) {
+      ok = ptx::WarpMbarWait(full + slot, phase, abort_flag, 1);
+      __syncwarp();                              // (one lane has seen the copy done; a shuffle orders no memory for the others)
+    }
     if (!ok) break;
     uint32_t* run = reinterpret_cast<uint32_t*>(ring + slot * kSlot);
     const int b = mine + i * turn, there = min(take, b1 - b);

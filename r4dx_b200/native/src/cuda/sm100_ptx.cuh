@@ -75,6 +75,8 @@ __device__ __forceinline__ bool MbarWait(uint64_t* bar, uint32_t parity, volatil
 // The same for a whole (converged) warp: one lane polls, the others sleep in the shuffle.  Thirty-two lanes
 // polling one barrier word serialise in the shared-memory pipe and slow down every other barrier
 // operation of the SM (measured: a satisfied test_wait of another warp went from 15 to ~300 clocks).
+// (A shuffle orders no memory: lanes that go on to read what the barrier announces, other than by warp-wide loads of tensor memory behind a
+// fence, take a __syncwarp first.)
 __device__ __forceinline__ bool WarpMbarWait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code) {
   int ok = 1;
   if ((threadIdx.x & 31) == 0) ok = MbarWait(bar, parity, abort_flag, code) ? 1 : 0;

@@ -341,6 +341,7 @@ TrellisGemvMmaKernel(MmaArgs a, TpPush tp) {
       if (ok) ok = ptx::WarpMbarWait(&ctl->full[s], sphase, abort_flag, 2);
       // the buffer's columns are free once the MMAs that read their previous contents have finished
       if (ok) ok = ptx::WarpMbarWait(&ctl->a_empty[buf], use_par ^ 1u, abort_flag, 5);
+      __syncwarp();                                  // (one lane has seen the copy done; a shuffle orders no memory for the others)
       if (ok) {
         ptx::TcFenceAfter();
         const uint32_t* sw = reinterpret_cast<const uint32_t*>(wst + static_cast<size_t>(s) * kStageBytes) + ntile * NW;
