@@ -126,14 +126,11 @@ class BatchModel:
         self.alloc.release(slot)
         self.active[slot] = False
 
-    def _attn_fp8(self, i: int, qg, kk, vv, q, core, B: int, positions, row_slot, splits: int, part_acc, part_ml) -> None:
-        """One layer's cache write and attention of B rows over the fp8 cache."""
-        from .. import native
-        L = self._L = self._L or native.cuda()
+    def _attn_fp8(self, L, st: int, i: int, qg, kk, vv, q, core, B: int, positions, row_slot, splits: int, part_acc, part_ml) -> None:
+        """One layer's cache write and attention of B rows over the fp8 cache, by library L on stream st."""
         cfg, w, pa = self.cfg, self.base.w, f"text.layers.{i}.attn."
         Hq, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         qn, kn = w.get(pa + "q_norm"), w.get(pa + "k_norm")
-        st = torch.cuda.current_stream().cuda_stream
         rc = L.r4dxb_attn_precore_batch(qg.data_ptr(), kk.data_ptr(), vv.data_ptr(), qn.data_ptr() if qn is not None else None,
                                         kn.data_ptr() if kn is not None else None, w[pa + "k_descale"].data_ptr(), w[pa + "v_descale"].data_ptr(),
                                         positions.data_ptr(), self.alloc.tables.data_ptr(), row_slot.data_ptr(),
@@ -197,7 +194,7 @@ class BatchModel:
                 if b.kv_cache == "int4":
                     self._attn_int4(i, qg, kk, vv, q, core, B, positions, row_slot)
                 else:
-                    self._attn_fp8(i, qg, kk, vv, q, core, B, positions, row_slot, splits, part_acc, part_ml)
+                    self._attn_fp8(L, st, i, qg, kk, vv, q, core, B, positions, row_slot, splits, part_acc, part_ml)
                 lin(pa + "o", core, x, residual=x)
             else:
                 pg = p + "gdn."
