@@ -4,10 +4,11 @@
 // of its warps walks blocks of its own, which arrive as one bulk copy per block into the warp's ring of shared memory.  Per block
 //   scores   S^T[16 tokens x 8 rows] = K Q^T on mma.m16n8k16 (fp16): A = the codes as they lie, since four bits at the bottom of a half are
 //            the subnormal n 2^-24 and four bits above them n 2^-20: one AND for two codes, and no conversion at all.  B = the query rows times
-//            2^4 (1 under the codes that carry a 16), exact down to 2^-14 and off by 2^-25 below; where some are above 2^11, or eight neighbours
+//            2^4 (1 under the codes that carry a 16), exact down to 2^-17 and off by 2^-25 below; where some are above 2^11, or eight neighbours
 //            below 2^-12, each row times the power of two that brings its largest value to 2^14 .. 2^15.  (That for every call: 0.2 us.)
 //            A group gives 2^-24 sum q n; then s (that) in fp32.
-//            sum_g lo sum(q): one product of the pairs as they lie (bf16) with the sums' upper and lower parts.
+//            sum_g lo sum(q): one product of the pairs as they lie (bf16) with the sums in two parts of bf16 (four at D = 64): 2^-17 of them is
+//            lost, which only keys of thousands whose products cancel would show.
 //   softmax  running maximum per row in the log2 domain, moved only when a score is more than 8 above it (p <= 2^8), so that most blocks
 //            need no exchange between lanes; sums in fp32 per lane.
 //   values   O^T[D x 8 rows] += n (p s):  A = codes of token pairs, again as subnormals; B = p s times a power of two of the warp and the group of
@@ -19,10 +20,10 @@
 // A row with no visible token (position -1) gives zeros; a block that the table or pool does not have gives NaN to the rows that see it.
 //
 // What bounds it: unpacking.  One token over 131071 keys: 24 heads over 4 of 256 35 us, 32 over 8 of 128 36 us, 4.3 TB/s of a copy's 6.5, with the
-// half-rate integer unit 49 / 54 % busy, the issue slots 48 / 55 %, the tensor pipe a quarter.  The first kernel, which made a number of every
+// half-rate integer unit 50 / 53 % busy, the issue slots 49 / 55 %, the tensor pipe a quarter.  The first kernel, which made a number of every
 // code before the products, took 68 us (32 over 8).  As many warps as the registers allow (8 at D = 256, 12 at 128) each with two blocks in work keep the units
 // fed, more of them with fewer registers spill (D = 256, 12 warps: 37 us; D = 128, 14: 40).  Short tables are bound by start and merge: 8192 keys of the
-// first 9.5 us, of which about 4 until the first scores and 2 for the second kernel; four rows (three row tiles) 13.
+// first 9.6 us, of which about 4 until the first scores and 2 for the second kernel; four rows (three row tiles) 13.
 #include <atomic>
 #include <type_traits>
 

@@ -235,6 +235,7 @@ __device__ __noinline__ void ScaleQueries(unsigned char* Qs, float* q_scale, con
     if (c == 0) q_scale[row] = score_scale * __uint_as_float((254u - p) << 23);
   }
 }
+
 // KV4: the 4-bit cache (kv4.cuh) in place of the fp8 one; only what the conversion warps load and store differs, and
 //   - keys enter with the channels of every eight in the order 0 4 1 5 2 6 3 7 (that of Kv4ToHalf), and so does Q;
 //   - a value group that is NaN is stored as zeros, and noted for the rows that see it: 0 x NaN would reach the rows that do not.
@@ -243,9 +244,9 @@ __device__ __noinline__ void ScaleQueries(unsigned char* Qs, float* q_scale, con
 //   - pages that the table or pool does not have are NaN keys;
 //   - the softmax warps bring Q, and all 16 warps write whole rows at the end, their gates loaded ahead: of a CTA of one tile (24 heads over 4 of
 //     256) 26000 clocks became 21500, half of which are start and end.
-// The same chain bounds it as the fp8 cache's (1024 rows after 8000 keys: tensor pipe 45 %, issue slots 50 %); widening codes costs the conversion
-// warps no more than widening fp8 does.  24 heads over 4 of 256: 333 rows 15.1 us, 1024 after 29000 721 to 788, 8192 803 to 904 by the power that
-// the chip is left; 32 over 8 of 128, 8192 rows 755; of 64 700.
+// The same chain bounds it as the fp8 cache's (1024 rows after 8000 keys: tensor pipe 44 %, issue slots 51 %); widening codes costs the conversion
+// warps no more than widening fp8 does.  24 heads over 4 of 256: 333 rows 15.4 us, 1024 after 29000 722 to 767, 8192 819 to 899 by the power that
+// the chip is left; 32 over 8 of 128, 8192 rows 759; of 64 712.
 template <int D, bool KV4>
 __global__ void __launch_bounds__(kThreads, 1) AttnPrefillTcKernel(Args<KV4> a) {
   constexpr int NS = D / 64;                          // 64-dimension slabs (one 128-byte swizzle row of fp16 each)
